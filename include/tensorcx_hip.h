@@ -502,6 +502,107 @@ int tcx_hip_flash_attention_f32_ws(const float* q, const float* k, const float* 
                                    const tcx_hip_flash_attention_desc_t* desc, void* workspace,
                                    size_t workspace_bytes, tcx_stream_t stream);
 
+/* ------------------------------------------------------------------ decoding
+ * Operators of a decoding loop, past the reference's: attention that sees a
+ * window of the last keys and a few first ones, a cache of keys and values in
+ * 4 bits with the attention that reads it, beam search's choice and the states
+ * that follow it. They enqueue on the stream, allocate nothing and can be
+ * captured in a graph. Sizes and strides are checked here; indexes that lie in
+ * device memory (lengths, positions, beams) are read on the device, where one
+ * out of range never moves an access out of its tensor: a length counts as 0
+ * or cols, a token without a slot is dropped, a row without a source is zeros.
+ * Where a flag is given, such an index sets it to 1. */
+
+/* A zeroed int32 in pinned host memory that kernels can set, for the `flag`
+ * arguments below: read it once the stream has run the call. */
+int tcx_hip_flag_acquire(int32_t** flag);
+void tcx_hip_flag_release(int32_t* flag);
+
+typedef struct {
+  int64_t batch, heads, kv_heads; /* heads a multiple of kv_heads: query head h reads head h / (heads / kv_heads) */
+  int64_t rows, cols, features;   /* queries and keys of a sequence; features of a head */
+  int64_t window;                 /* keys that a query sees, itself included; 0: all of them */
+  int64_t sinks;                  /* first keys that stay visible outside the window */
+  float scale;                    /* of the scores; finite */
+  const int32_t* lengths;         /* device [batch]: keys of each sequence; NULL: cols */
+  int32_t* flag;                  /* may be NULL */
+  /* Elements from one sequence, head and token to the next; the features lie
+   * together. All zero: contiguous (batch, heads, tokens, features). */
+  int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3];
+} tcx_hip_window_attention_desc_t;
+/* 1 when tcx_hip_window_attention_f32 handles these features (a multiple of 8
+ * from 16 to 128), else 0. */
+int tcx_hip_window_attention_supported(int64_t features);
+/* Query i of a sequence of n keys stands at key p = n - rows + i (its last query
+ * at its last key) and sees key j of 0 <= j <= p when the window is 0, j > p -
+ * window or j < sinks: out = softmax over those of scale * q.k, times v. A query
+ * that sees no key gets zeros. Hidden keys have no influence, whatever they
+ * hold; a row that sees a NaN is NaN, and what infinities that it sees make of
+ * it is not specified. Pointers are 16-byte aligned, strides multiples of 4, rows *
+ * heads / kv_heads, cols and batch * kv_heads below 2^30. The workspace (16-byte
+ * aligned, may be NULL) takes the states of keys split over blocks, as far as
+ * it has room; the query says how much such a call can use, and it must stay
+ * allocated until the stream has run the call. */
+size_t tcx_hip_window_attention_workspace_bytes(const tcx_hip_window_attention_desc_t* desc);
+int tcx_hip_window_attention_f32(const float* q, const float* k, const float* v, float* out,
+                                 const tcx_hip_window_attention_desc_t* desc, void* workspace, size_t workspace_bytes,
+                                 tcx_stream_t stream);
+
+/* The 4-bit cache: int32 [batch, kv_heads, capacity, words], words = features /
+ * 8 + features / 32 for 32, 64 or 128 features (tcx_hip_cache4_words; 0 for
+ * others). 32 features share a low end and a step: low is their minimum rounded
+ * down to bfloat16, step is (maximum - low) / 15 rounded up to bfloat16, and a
+ * feature x is held as round((x - low) / step) in 0..15, which stands for low +
+ * step * code, at most half a step off. A row is features / 2 bytes of codes,
+ * byte n * (features / 32) + g with feature 32 g + n in its low half and 32 g +
+ * 16 + n in its high one (n < 16), then a word for each g, low in the upper 16
+ * bits, step in the lower. A group with a NaN, an infinity or a range past
+ * float32 is held as NaN. */
+int64_t tcx_hip_cache4_words(int64_t features);
+typedef struct {
+  int64_t batch, kv_heads, tokens, capacity, features;
+  int32_t* flag; /* may be NULL */
+  int64_t key_strides[3], value_strides[3]; /* as above; all zero: contiguous */
+} tcx_hip_cache4_store_desc_t;
+/* Stores token t of sequence b at slot positions[b] + t of the caches (device
+ * int32 [batch]); every other slot is left as it was. */
+int tcx_hip_cache4_store(const float* key, const float* value, int32_t* key_cache, int32_t* value_cache,
+                         const int32_t* positions, const tcx_hip_cache4_store_desc_t* desc, tcx_stream_t stream);
+/* Slots [start, start + count) of `heads` (batch * kv_heads) rows of a cache as
+ * float32: out [heads, count, features]. */
+int tcx_hip_cache4_load(const int32_t* cache, float* out, int64_t heads, int64_t capacity, int64_t start, int64_t count,
+                        int64_t features, tcx_stream_t stream);
+/* tcx_hip_window_attention_f32 over caches of capacity cols (16-byte aligned;
+ * desc's k_strides and v_strides are not read). */
+size_t tcx_hip_cache4_attention_workspace_bytes(const tcx_hip_window_attention_desc_t* desc);
+int tcx_hip_cache4_attention_f32(const float* q, const int32_t* key_cache, const int32_t* value_cache, float* out,
+                                 const tcx_hip_window_attention_desc_t* desc, void* workspace, size_t workspace_bytes,
+                                 tcx_stream_t stream);
+
+#define TCX_HIP_BEAM_MAX_COUNT 256
+/* Beam search's choice: of the candidates (beam k, token v) of each sequence, at
+ * scores[b, k] + logits[b, k, v] - log(sum over the beam of exp(logits)), the
+ * `count` best in descending order: their scores, beams and tokens, [batch,
+ * count] each. Candidates are compared in 64 bits; of one beam the larger logit
+ * comes first, then the lower token, and of equal scores the lower beam. NaN
+ * comes before every number; a beam whose logits are all -inf offers -inf. A
+ * beam with finished[b, k] != 0 (may be NULL) offers token `eos` at its own
+ * score and -inf for the others. beams * vocabulary is below 2^31, count at most
+ * TCX_HIP_BEAM_MAX_COUNT and beams * vocabulary. The workspace (16-byte aligned,
+ * of at least the query's bytes) must stay allocated until the stream has run
+ * the call. */
+size_t tcx_hip_beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocabulary, int64_t count);
+int tcx_hip_beam_select_f32(const float* logits, const float* scores, const uint8_t* finished, int32_t eos,
+                            float* out_scores, int32_t* out_beams, int32_t* out_tokens, int64_t batch, int64_t beams,
+                            int64_t vocabulary, int64_t count, void* workspace, size_t workspace_bytes,
+                            tcx_stream_t stream);
+/* The states of the chosen beams: row b * count + n of out[i] is row b * beams +
+ * index[b, n] of in[i], for `tensors` tensors of rows of row_bytes[i] bytes (any
+ * address and number). Inputs and outputs do not overlap. */
+int tcx_hip_beam_reorder(const void* const* in, void* const* out, const int64_t* row_bytes, int32_t tensors,
+                         const int32_t* index, int64_t batch, int64_t beams, int64_t count, int32_t* flag,
+                         tcx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

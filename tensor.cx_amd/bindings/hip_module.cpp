@@ -99,6 +99,26 @@ HipTensor builtin(const std::string& entry, std::vector<const HipTensor*> args, 
   return HipTensor{std::move(outputs[0])};
 }
 
+// A built-in kernel with outputs that the caller allocated (or updates in place).
+void kernel(const std::string& entry, const std::vector<const HipTensor*>& args, const std::vector<std::uint32_t>& scalars,
+            const std::vector<const HipTensor*>& out) {
+  std::vector<Tensor> outputs;
+  for (const HipTensor* t : out) outputs.push_back(t->tensor);
+  std::vector<KernelArgument> kargs;
+  for (const HipTensor* t : args) kargs.push_back(KernelArgument{KernelArgumentKind::kTensor, &t->tensor, 0});
+  for (std::uint32_t v : scalars) kargs.push_back(KernelArgument{KernelArgumentKind::kUInt32, nullptr, v});
+  Status status;
+  {
+    py::gil_scoped_release release;
+    BackendExecution e{BackendOpClass::kKernel, OpDesc{},
+                       {}, outputs, LaunchConfig{1, 1, 1, 1, 1, 1},
+                       CompilationTarget{KernelArtifactKind::kStaticLibrary, hip::kStaticArtifact, entry}, kargs};
+    hip::HipBackend backend;
+    status = backend.execute(e);
+  }
+  if (!status.ok()) throw_status(status);
+}
+
 py::array to_numpy(const HipTensor& t) {
   std::vector<py::ssize_t> shape(t.tensor.shape.begin(), t.tensor.shape.end());
   py::array out;
@@ -250,6 +270,9 @@ PYBIND11_MODULE(_core, m) {
   m.def("bias_act", [](const HipTensor& x, const HipTensor& b, std::uint32_t act) {
     return builtin("bias_act", {&x, &b}, act, x.tensor.shape);
   });
+
+  m.def("_kernel", &kernel, py::arg("entry"), py::arg("inputs"), py::arg("scalars"), py::arg("outputs"));
+  m.def("_cache4_words", [](std::int64_t features) { return tcx_hip_cache4_words(features); });
 
   for (const auto& [name, kind] : std::vector<std::pair<const char*, OpKind>>{
            {"sum", OpKind::kSum}, {"max", OpKind::kMax}, {"mean", OpKind::kMean}}) {

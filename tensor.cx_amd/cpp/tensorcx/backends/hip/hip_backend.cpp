@@ -12,10 +12,12 @@
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <iterator>
 #include <limits>
 #include <mutex>
 #include <stdexcept>
 #include <string>
+#include <string_view>
 #include <utility>
 #include <vector>
 
@@ -1195,13 +1197,276 @@ Tensor masked_select(const Tensor& x, const Tensor& mask, Stream& s) {
   return out;
 }
 
+// ------------------------------------------------------------ decoding
+// The operators of a decoding loop, which the reference has no OpKind for: they
+// are built-in kernels (execute_builtin_kernel), with the outputs given.
+
+// A flag that device code sets for an index out of range, in pinned host memory.
+class IndexFlag {
+ public:
+  IndexFlag() { ok_or_throw(tcx_hip_flag_acquire(&flag_), "HIP flag"); }
+  ~IndexFlag() { tcx_hip_flag_release(flag_); }
+  IndexFlag(const IndexFlag&) = delete;
+  IndexFlag& operator=(const IndexFlag&) = delete;
+  std::int32_t* get() const { return flag_; }
+  // Waits for the stream, then throws if an index was out of range.
+  void finish(tcx_stream_t s, const char* message) const {
+    synchronize(s);
+    if (*static_cast<volatile std::int32_t*>(flag_) != 0) throw std::invalid_argument(message);
+  }
+
+ private:
+  std::int32_t* flag_{nullptr};
+};
+
+// What a built-in kernel was called with.
+struct KernelCall {
+  const char* name;
+  std::vector<const Tensor*> tensors;
+  std::vector<std::uint32_t> scalars;
+  std::span<Tensor> outputs;
+
+  [[noreturn]] void refuse(const std::string& what) const { throw std::invalid_argument(std::string(name) + " " + what); }
+  void expect(std::size_t least, std::size_t most, std::size_t scalar_count, std::size_t output_count) const {
+    if (tensors.size() < least || tensors.size() > most) refuse("takes another number of tensors");
+    if (scalars.size() != scalar_count) refuse("takes another number of scalars");
+    if (outputs.size() != output_count) refuse("writes another number of outputs");
+  }
+  void expect_dtype(const Tensor& t, DType dtype, const char* what) const {
+    if (t.dtype != dtype) refuse(std::string(what) + " must be " + std::string(dtype_name(dtype)));
+  }
+  void expect_shape(const Tensor& t, const Shape& shape, const char* what) const {
+    if (t.shape != shape) refuse(std::string("has no matching ") + what);
+  }
+  void expect_rank(const Tensor& t, std::size_t rank, const char* what) const {
+    if (t.shape.size() != rank) refuse(std::string(what) + " must have rank " + std::to_string(rank));
+  }
+  // Outputs are written while inputs are read: no two may share storage.
+  void expect_apart() const {
+    for (std::size_t i = 0; i < outputs.size(); ++i) {
+      if (!outputs[i].buffer || outputs[i].buffer->nbytes() == 0) continue;
+      for (const Tensor* t : tensors)
+        if (t->buffer && t->buffer->nbytes() != 0 &&
+            outputs[i].buffer->storage_relation(*t->buffer) != StorageRelation::kDisjoint)
+          refuse("inputs and outputs must not share storage");
+      for (std::size_t j = 0; j < i; ++j)
+        if (outputs[j].buffer && outputs[j].buffer->nbytes() != 0 &&
+            outputs[i].buffer->storage_relation(*outputs[j].buffer) != StorageRelation::kDisjoint)
+          refuse("outputs must not share storage");
+    }
+  }
+};
+
+// The tensor, or a copy of it on a 16-byte boundary where borrowed storage lies on none.
+Tensor on_boundary(const Tensor& t) {
+  if (aligned16(device_ptr(t))) return t;
+  auto copy = clone(t);
+  if (!copy) throw std::runtime_error(copy.status().message());
+  return copy.move_value();
+}
+
+float float_of(std::uint32_t bits) {
+  float value;
+  static_assert(sizeof(value) == sizeof(bits));
+  std::memcpy(&value, &bits, sizeof(value));
+  return value;
+}
+
+// Runs launch(pointer, bytes) with a workspace that is held until the stream has
+// finished, or with none where that allocation fails and `needed` is false.
+template <typename F>
+void with_workspace(std::size_t bytes, bool needed, F&& launch, const IndexFlag& flag, Stream& s, const char* message) {
+  std::shared_ptr<HipBuffer> workspace;
+  if (bytes != 0) {
+    auto created = HipBuffer::create(bytes);
+    if (created) workspace = created.move_value();
+    else if (needed) throw std::runtime_error(created.status().message());
+  }
+  launch(workspace ? workspace->data() : nullptr, workspace ? bytes : 0);
+  flag.finish(s, message);
+}
+
+// "window_attention": query, key, value[, lengths]; window, sinks, scale bits.
+// "cache4_attention": query, key cache, value cache, lengths; the same.
+void decode_attention(const KernelCall& c, bool cache, Stream& s) {
+  c.expect(cache ? 4 : 3, 4, 3, 1);
+  const Tensor &q = *c.tensors[0], &k = *c.tensors[1], &v = *c.tensors[2];
+  const DType stored = cache ? DType::kInt32 : DType::kFloat32;
+  c.expect_dtype(q, DType::kFloat32, "query");
+  c.expect_dtype(k, stored, "key");
+  c.expect_dtype(v, stored, "value");
+  c.expect_dtype(c.outputs[0], DType::kFloat32, "output");
+  c.expect_rank(q, 4, "query");
+  c.expect_rank(k, 4, "key");
+  c.expect_shape(v, k.shape, "key and value shapes");
+  c.expect_shape(c.outputs[0], q.shape, "output");
+  if (k.shape[0] != q.shape[0]) c.refuse("needs as many key sequences as query sequences");
+  const Dim words = cache ? tcx_hip_cache4_words(q.shape[3]) : q.shape[3];
+  if (cache && words == 0) c.refuse("takes 32, 64 or 128 features");
+  if (k.shape[3] != words) c.refuse(cache ? "caches must hold the query's features" : "key features must be the query's");
+  tcx_hip_window_attention_desc_t d{};
+  d.batch = q.shape[0];
+  d.heads = q.shape[1];
+  d.kv_heads = k.shape[1];
+  d.rows = q.shape[2];
+  d.cols = k.shape[2];
+  d.features = q.shape[3];
+  d.window = c.scalars[0];
+  d.sinks = c.scalars[1];
+  d.scale = float_of(c.scalars[2]);
+  if (c.tensors.size() == 4) {
+    c.expect_dtype(*c.tensors[3], DType::kInt32, "lengths");
+    c.expect_shape(*c.tensors[3], Shape{d.batch}, "lengths (batch,)");
+    d.lengths = static_cast<const std::int32_t*>(device_ptr(*c.tensors[3]));
+  }
+  c.expect_apart();
+  if (numel(q.shape) == 0) return;
+  const Tensor qa = on_boundary(q), ka = on_boundary(k), va = on_boundary(v);
+  if (!aligned16(out_ptr(c.outputs[0]))) c.refuse("output must be 16-byte aligned");
+  const IndexFlag flag;
+  d.flag = flag.get();
+  const std::size_t ws = cache ? tcx_hip_cache4_attention_workspace_bytes(&d) : tcx_hip_window_attention_workspace_bytes(&d);
+  auto* out = static_cast<float*>(out_ptr(c.outputs[0]));
+  with_workspace(ws, false, [&](void* p, std::size_t bytes) {
+    if (cache)
+      ok_or_throw(tcx_hip_cache4_attention_f32(f32(qa), static_cast<const std::int32_t*>(device_ptr(ka)),
+                                               static_cast<const std::int32_t*>(device_ptr(va)), out, &d, p, bytes, s),
+                  "HIP cache attention");
+    else
+      ok_or_throw(tcx_hip_window_attention_f32(f32(qa), f32(ka), f32(va), out, &d, p, bytes, s), "HIP window attention");
+  }, flag, s, "attention lengths must lie between 0 and the number of keys");
+}
+
+// "cache4_store": key, value, positions; outputs: the key and the value cache, in place.
+void cache_store(const KernelCall& c, Stream& s) {
+  c.expect(3, 3, 0, 2);
+  const Tensor &key = *c.tensors[0], &value = *c.tensors[1], &positions = *c.tensors[2];
+  c.expect_dtype(key, DType::kFloat32, "key");
+  c.expect_dtype(value, DType::kFloat32, "value");
+  c.expect_dtype(positions, DType::kInt32, "positions");
+  for (const Tensor& cache : c.outputs) c.expect_dtype(cache, DType::kInt32, "cache");
+  c.expect_rank(key, 4, "key");
+  c.expect_shape(value, key.shape, "key and value shapes");
+  c.expect_rank(c.outputs[0], 4, "cache");
+  tcx_hip_cache4_store_desc_t d{};
+  d.batch = key.shape[0];
+  d.kv_heads = key.shape[1];
+  d.tokens = key.shape[2];
+  d.features = key.shape[3];
+  d.capacity = c.outputs[0].shape[2];
+  const Dim words = tcx_hip_cache4_words(d.features);
+  if (words == 0) c.refuse("takes 32, 64 or 128 features");
+  for (const Tensor& cache : c.outputs) c.expect_shape(cache, Shape{d.batch, d.kv_heads, d.capacity, words}, "cache");
+  c.expect_shape(positions, Shape{d.batch}, "positions (batch,)");
+  c.expect_apart();
+  if (numel(key.shape) == 0) return;
+  for (const Tensor& cache : c.outputs)
+    if (!aligned16(device_ptr(cache))) c.refuse("caches must be 16-byte aligned");
+  const Tensor ka = on_boundary(key), va = on_boundary(value);
+  const IndexFlag flag;
+  d.flag = flag.get();
+  ok_or_throw(tcx_hip_cache4_store(f32(ka), f32(va), static_cast<std::int32_t*>(out_ptr(c.outputs[0])),
+                                   static_cast<std::int32_t*>(out_ptr(c.outputs[1])),
+                                   static_cast<const std::int32_t*>(device_ptr(positions)), &d, s),
+              "HIP cache store");
+  flag.finish(s, "cache store positions must leave every token a slot");
+}
+
+// "cache4_load": cache; first slot; output (batch, heads, count, features).
+void cache_load(const KernelCall& c, Stream& s) {
+  c.expect(1, 1, 1, 1);
+  const Tensor &cache = *c.tensors[0], &out = c.outputs[0];
+  c.expect_dtype(cache, DType::kInt32, "cache");
+  c.expect_dtype(out, DType::kFloat32, "output");
+  c.expect_rank(cache, 4, "cache");
+  c.expect_rank(out, 4, "output");
+  const Dim words = tcx_hip_cache4_words(out.shape[3]);
+  if (words == 0 || cache.shape[3] != words || out.shape[0] != cache.shape[0] || out.shape[1] != cache.shape[1])
+    c.refuse("output must match the cache");
+  c.expect_apart();
+  const Tensor from = on_boundary(cache);
+  ok_or_throw(tcx_hip_cache4_load(static_cast<const std::int32_t*>(device_ptr(from)), static_cast<float*>(out_ptr(out)),
+                                  numel(Shape{cache.shape[0], cache.shape[1]}), cache.shape[2], c.scalars[0], out.shape[2],
+                                  out.shape[3], s),
+              "HIP cache load");
+  if (s.used()) synchronize(s);
+}
+
+// "beam_select": logits, scores[, finished]; end token; outputs scores, beams, tokens.
+void beam_select(const KernelCall& c, Stream& s) {
+  c.expect(2, 3, 1, 3);
+  const Tensor &logits = *c.tensors[0], &scores = *c.tensors[1];
+  c.expect_dtype(logits, DType::kFloat32, "logits");
+  c.expect_dtype(scores, DType::kFloat32, "scores");
+  c.expect_rank(logits, 3, "logits");
+  c.expect_shape(scores, Shape{logits.shape[0], logits.shape[1]}, "scores (batch, beams)");
+  if (c.tensors.size() == 3) {
+    c.expect_dtype(*c.tensors[2], DType::kBool, "finished");
+    c.expect_shape(*c.tensors[2], scores.shape, "finished (batch, beams)");
+  }
+  c.expect_dtype(c.outputs[0], DType::kFloat32, "score output");
+  c.expect_rank(c.outputs[0], 2, "output");
+  for (std::size_t i = 1; i < 3; ++i) c.expect_dtype(c.outputs[i], DType::kInt32, "index output");
+  const Dim batch = logits.shape[0], beams = logits.shape[1], vocabulary = logits.shape[2], count = c.outputs[0].shape[1];
+  for (const Tensor& out : c.outputs) c.expect_shape(out, Shape{batch, count}, "output");
+  c.expect_apart();
+  const std::size_t ws = tcx_hip_beam_select_workspace_bytes(batch, beams, vocabulary, count);
+  std::shared_ptr<HipBuffer> workspace;
+  if (ws != 0) workspace = scratch(ws);
+  ok_or_throw(tcx_hip_beam_select_f32(
+                  f32(logits), f32(scores),
+                  c.tensors.size() == 3 ? static_cast<const std::uint8_t*>(device_ptr(*c.tensors[2])) : nullptr,
+                  static_cast<std::int32_t>(c.scalars[0]), static_cast<float*>(out_ptr(c.outputs[0])),
+                  static_cast<std::int32_t*>(out_ptr(c.outputs[1])), static_cast<std::int32_t*>(out_ptr(c.outputs[2])), batch,
+                  beams, vocabulary, count, workspace ? workspace->data() : nullptr, ws, s),
+              "HIP beam selection");
+  if (s.used()) synchronize(s);
+}
+
+// "beam_reorder": the states, beams; outputs: the states of the chosen beams.
+void beam_reorder(const KernelCall& c, Stream& s) {
+  if (c.tensors.size() < 2 || c.outputs.size() + 1 != c.tensors.size() || !c.scalars.empty())
+    c.refuse("takes states and beams and writes an output for each state");
+  const Tensor& index = *c.tensors.back();
+  c.expect_dtype(index, DType::kInt32, "beams");
+  c.expect_rank(index, 2, "beams");
+  const Dim batch = index.shape[0], count = index.shape[1];
+  Dim beams = -1;
+  std::vector<const void*> in;
+  std::vector<void*> out;
+  std::vector<std::int64_t> row_bytes;
+  for (std::size_t i = 0; i < c.outputs.size(); ++i) {
+    const Tensor& state = *c.tensors[i];
+    if (state.shape.empty() || (batch == 0 ? state.shape[0] != 0 : state.shape[0] % batch != 0) ||
+        (beams >= 0 && state.shape[0] != beams * batch))
+      c.refuse("states must have batch * beams leading rows");
+    beams = batch == 0 ? 0 : state.shape[0] / batch;
+    Shape shape = state.shape;
+    shape[0] = batch * count;
+    c.expect_dtype(c.outputs[i], state.dtype, "output");
+    c.expect_shape(c.outputs[i], shape, "output");
+    shape[0] = 1;
+    in.push_back(device_ptr(state));
+    out.push_back(out_ptr(c.outputs[i]));
+    row_bytes.push_back(static_cast<std::int64_t>(byte_size(shape, state.dtype)));
+  }
+  c.expect_apart();
+  const IndexFlag flag;
+  ok_or_throw(tcx_hip_beam_reorder(in.data(), out.data(), row_bytes.data(), static_cast<int32_t>(in.size()),
+                                   static_cast<const std::int32_t*>(device_ptr(index)), batch, beams, count, flag.get(), s),
+              "HIP beam reorder");
+  flag.finish(s, "beam reorder indices must name a beam");
+}
+
 // ------------------------------------------------------------ kernel class
 Status execute_builtin_kernel(const BackendExecution& e) {
   if (Status s = validate_kernel_execution_contract(e); !s.ok()) return s;
   const auto& target = *e.compilation_target;
   if (target.artifact_kind != KernelArtifactKind::kStaticLibrary || target.artifact != kStaticArtifact)
     return Status(StatusCode::kInvalidArgument, "HIP kernels must name the tensorcx_hip static library");
-  if (target.entry_point != "linear_bias_act" && target.entry_point != "bias_act")
+  static constexpr std::string_view kEntries[] = {"linear_bias_act", "bias_act", "window_attention", "cache4_attention",
+                                                  "cache4_store", "cache4_load", "beam_select", "beam_reorder"};
+  if (std::find(std::begin(kEntries), std::end(kEntries), target.entry_point) == std::end(kEntries))
     return Status(StatusCode::kInvalidArgument, "unknown HIP built-in kernel entry point");
   std::vector<const Tensor*> tensors;
   std::vector<std::uint32_t> scalars;
@@ -1210,6 +1475,19 @@ Status execute_builtin_kernel(const BackendExecution& e) {
       tensors.push_back(a.tensor);
     else
       scalars.push_back(a.uint32_value);
+  }
+  if (target.entry_point != "linear_bias_act" && target.entry_point != "bias_act") {
+    for (const Tensor* t : tensors) (void)device_ptr(*t);
+    for (const Tensor& t : e.outputs) (void)device_ptr(t);
+    const KernelCall call{target.entry_point.c_str(), std::move(tensors), std::move(scalars), e.outputs};
+    Stream s;
+    if (target.entry_point == "window_attention") decode_attention(call, false, s);
+    else if (target.entry_point == "cache4_attention") decode_attention(call, true, s);
+    else if (target.entry_point == "cache4_store") cache_store(call, s);
+    else if (target.entry_point == "cache4_load") cache_load(call, s);
+    else if (target.entry_point == "beam_select") beam_select(call, s);
+    else beam_reorder(call, s);
+    return Status::Ok();
   }
   if (e.outputs.size() != 1) return Status(StatusCode::kInvalidArgument, "HIP built-in kernels write one output");
   const Tensor& out = e.outputs[0];

@@ -88,6 +88,15 @@ Expected<void*> export_storage(const Tensor& tensor);
 //                      outputs[0] = preallocated act(x @ weight^T + bias)
 //   "bias_act":        kernel_arguments = x, bias, uint32 activation;
 //                      outputs[0] = preallocated act(x + bias)
+// and the operators of a decoding loop (the C ABI's of the same names, where a
+// float32 scalar is passed by its bits):
+//   "window_attention": query, key, value[, lengths], window (0: none), sinks, scale;
+//                       outputs[0] = (batch, heads, rows, features)
+//   "cache4_attention": query, key cache, value cache, lengths, window, sinks, scale
+//   "cache4_store":     key, value, positions; outputs = key and value cache, in place
+//   "cache4_load":      cache, first slot; outputs[0] = (batch, kv_heads, count, features)
+//   "beam_select":      logits, scores[, finished], end token; outputs = scores, beams, tokens
+//   "beam_reorder":     states..., beams; outputs = the chosen beams' states
 inline constexpr const char* kStaticArtifact = "tensorcx_hip";
 
 }  // namespace tensorcx::hip

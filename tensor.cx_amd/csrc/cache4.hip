@@ -1,0 +1,297 @@
+// The 4-bit cache of keys and values: storing float32 tokens in it, reading
+// them back, and attention over it.
+//
+// Of 32 features x: low = min x rounded down to bfloat16, step = (max x - low)
+// / 15 rounded up to bfloat16, code = round((x - low) / step) in 0..15, which
+// stands for low + step * code. Rounding the ends outwards keeps every x inside
+// [low, low + 15 step], so that a value is at most half a step off; bfloat16
+// costs the step at most 2^-7 of the range plus 2^-7 |low| / 15, and saves a
+// fifth of the bytes that float32 ends would make of a row of 128 (80 against
+// 96). A row holds its codes in the order that matrix instructions take them:
+// lane n of sixteen finds the features 16 e + n in its own D / 32 bytes, byte g
+// holding e = 2 g in its low half and e = 2 g + 1 in its high one.
+
+#include <algorithm>
+
+#include "decode_stream.hpp"
+
+namespace tcx {
+namespace {
+
+// The codes of one lane: D / 32 bytes.
+template <int D>
+struct LaneCodes;
+template <>
+struct LaneCodes<128> {
+  using type = std::uint32_t;
+};
+template <>
+struct LaneCodes<64> {
+  using type = std::uint16_t;
+};
+template <>
+struct LaneCodes<32> {
+  using type = std::uint8_t;
+};
+
+template <int D>
+struct CacheRow {
+  static constexpr int kGroups = D / 32, kWords = D / 8 + kGroups;
+  using Codes = typename LaneCodes<D>::type;
+  using Scales = std::uint32_t __attribute__((ext_vector_type(kGroups)));
+};
+template <>
+struct CacheRow<32> {
+  static constexpr int kGroups = 1, kWords = 5;
+  using Codes = std::uint8_t;
+  using Scales = std::uint32_t;
+};
+
+__device__ __forceinline__ std::uint32_t scale_word(std::uint32_t v, int) { return v; }
+template <typename V>
+__device__ __forceinline__ std::uint32_t scale_word(const V& v, int g) {
+  return v[g];
+}
+
+template <int D>
+struct CacheRows {
+  using Row = CacheRow<D>;
+  static constexpr int kFeatures = D / 16;
+  struct Raw {
+    std::uint32_t codes;
+    typename Row::Scales scales;
+  };
+  static __device__ __forceinline__ int feature(int li, int e) { return 16 * e + li; }
+  std::int64_t k_base, v_base;
+  int li;
+  __device__ CacheRows(const DecodeArgs& a, int b, int kv, int lane)
+      : k_base(b * a.k_stride[0] + kv * a.k_stride[1]), v_base(b * a.v_stride[0] + kv * a.v_stride[1]), li(lane) {}
+  __device__ __forceinline__ void load(const void* p, std::int64_t base, std::int64_t stride, std::int64_t key,
+                                       Raw& raw) const {
+    const std::int32_t* row = static_cast<const std::int32_t*>(p) + base + key * stride;
+    raw.codes = reinterpret_cast<const typename Row::Codes*>(row)[li];
+    raw.scales = *reinterpret_cast<const typename Row::Scales*>(row + D / 8);
+  }
+  __device__ __forceinline__ void values(const Raw& raw, float (&x)[kFeatures]) const {
+#pragma unroll
+    for (int e = 0; e < kFeatures; ++e) {
+      const std::uint32_t word = scale_word(raw.scales, e / 2);
+      const float low = __uint_as_float(word & 0xffff0000U), step = __uint_as_float(word << 16);
+      x[e] = fmaf(step, static_cast<float>((raw.codes >> (4 * e)) & 15U), low);
+    }
+  }
+};
+
+// The largest (or smallest) of sixteen lanes' values, in all of them.
+template <bool kLargest>
+__device__ __forceinline__ float lanes16_extreme(float x) {
+  auto with = [&]<int kControl>() {
+    const float y = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), kControl, 0xf, 0xf, true));
+    x = kLargest ? fmaxf(x, y) : fminf(x, y);
+  };
+  with.template operator()<0xb1>();
+  with.template operator()<0x4e>();
+  with.template operator()<0x141>();
+  with.template operator()<0x140>();
+  return x;
+}
+
+struct StoreArgs {
+  const float* x[2];  // keys, values
+  std::int32_t* cache[2];
+  const std::int32_t* positions;
+  std::int32_t* flag;
+  std::int64_t stride[2][3];
+  std::int64_t tokens_all;  // batch * kv_heads * tokens
+  int kv_heads, tokens;
+  std::int64_t capacity;
+};
+
+// Sixteen lanes a token, in grid.y = 2 for the keys and the values.
+template <int D>
+__global__ __launch_bounds__(256) void cache_store_kernel(StoreArgs a) {
+  using Row = CacheRow<D>;
+  constexpr int kF = D / 16;
+  const int li = threadIdx.x & 15, which = blockIdx.y;
+  const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * 16;
+  for (std::int64_t i = static_cast<std::int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4); i < a.tokens_all; i += step) {
+    const std::int64_t head = i / a.tokens, t = i % a.tokens, b = head / a.kv_heads, kv = head % a.kv_heads;
+    const float* row = a.x[which] + b * a.stride[which][0] + kv * a.stride[which][1] + t * a.stride[which][2];
+    const std::int64_t slot = a.positions[b] + t;
+    float x[kF];
+#pragma unroll
+    for (int e = 0; e < kF; ++e) x[e] = row[16 * e + li];
+    std::uint32_t codes = 0, words[Row::kGroups];
+#pragma unroll
+    for (int g = 0; g < Row::kGroups; ++g) {
+      const float u = x[2 * g], v = x[2 * g + 1];
+      const bool bad = !(fabsf(u) < __builtin_inff()) || !(fabsf(v) < __builtin_inff());
+      const float least = lanes16_extreme<false>(fminf(u, v)) + 0.F;  // no -0
+      const float most = lanes16_extreme<true>(fmaxf(u, v));
+      const std::uint32_t bits = __float_as_uint(least);
+      std::uint32_t low = bits & 0xffff0000U;
+      if (low != bits && (bits >> 31)) low += 0x10000U;
+      const float span = (most - __uint_as_float(low)) * (1.F / 15.F) + 0.F;
+      std::uint32_t size = (__float_as_uint(span) + 0xffffU) & 0xffff0000U;
+      // The sixteen lanes of this token in the wave's ballot.
+      const bool any_bad = (__ballot(bad) >> (threadIdx.x & 48)) & 0xffffU;
+      const bool lost = any_bad || (low & 0x7f800000U) == 0x7f800000U || (size & 0x7f800000U) == 0x7f800000U;
+      if (lost) low = size = 0x7fc00000U;
+      const float from = __uint_as_float(low), by = __uint_as_float(size);
+      auto code = [&](float value) {
+        const float c = fminf(fmaxf(rintf((value - from) / by), 0.F), 15.F);
+        return by > 0.F ? static_cast<std::uint32_t>(c) : 0U;  // NaN and a step of 0: code 0
+      };
+      codes |= (code(u) | (code(v) << 4)) << (8 * g);
+      words[g] = low | (size >> 16);
+    }
+    if (slot < 0 || slot >= a.capacity) {
+      if (a.flag != nullptr) __hip_atomic_store(a.flag, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+      continue;
+    }
+    std::int32_t* out = a.cache[which] + (head * a.capacity + slot) * Row::kWords;
+    reinterpret_cast<typename Row::Codes*>(out)[li] = static_cast<typename Row::Codes>(codes);
+#pragma unroll
+    for (int g = 0; g < Row::kGroups; ++g)
+      if (li == g) out[D / 8 + g] = static_cast<std::int32_t>(words[g]);
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void cache_load_kernel(const std::int32_t* __restrict__ cache, float* __restrict__ out,
+                                                         std::int64_t n, std::int64_t capacity, std::int64_t start,
+                                                         std::int64_t count) {
+  using Row = CacheRow<D>;
+  const int li = threadIdx.x & 15;
+  const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * 16;
+  for (std::int64_t i = static_cast<std::int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4); i < n; i += step) {
+    const std::int64_t head = i / count, slot = start + i % count;
+    const std::int32_t* row = cache + (head * capacity + slot) * Row::kWords;
+    const std::uint32_t codes = reinterpret_cast<const typename Row::Codes*>(row)[li];
+    const auto scales = *reinterpret_cast<const typename Row::Scales*>(row + D / 8);
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) {
+      const std::uint32_t word = scale_word(scales, e / 2);
+      out[i * D + 16 * e + li] = fmaf(__uint_as_float(word << 16), static_cast<float>((codes >> (4 * e)) & 15U),
+                                      __uint_as_float(word & 0xffff0000U));
+    }
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15U) == 0; }
+
+int cache_splits(const DecodeArgs& a, std::size_t workspace_bytes) {
+  const int rows = stream_rows(a);
+  const std::int64_t blocks = static_cast<std::int64_t>(a.batch) * a.kv_heads * ((a.rows * a.share + rows - 1) / rows);
+  return plan_splits(a, blocks, 128, workspace_bytes);
+}
+
+}  // namespace
+}  // namespace tcx
+
+extern "C" {
+
+int64_t tcx_hip_cache4_words(int64_t features) {
+  return features == 32 || features == 64 || features == 128 ? features / 8 + features / 32 : 0;
+}
+
+int tcx_hip_cache4_store(const float* key, const float* value, int32_t* key_cache, int32_t* value_cache,
+                         const int32_t* positions, const tcx_hip_cache4_store_desc_t* desc, tcx_stream_t stream) {
+  using namespace tcx;
+  if (desc == nullptr) return fail(TCX_INVALID_ARGUMENT, "cache store descriptor is null");
+  const auto& d = *desc;
+  if (d.batch < 0 || d.kv_heads < 0 || d.tokens < 0 || d.capacity < 0)
+    return fail(TCX_INVALID_ARGUMENT, "cache store extents must be non-negative");
+  if (tcx_hip_cache4_words(d.features) == 0)
+    return fail(TCX_INVALID_ARGUMENT, "a 4-bit cache holds 32, 64 or 128 features");
+  if (d.batch == 0 || d.kv_heads == 0 || d.tokens == 0) return TCX_OK;
+  constexpr std::int64_t kMost = std::int64_t{1} << 30;
+  if (d.capacity >= kMost || d.tokens >= kMost || d.batch >= kMost / d.kv_heads)
+    return fail(TCX_INVALID_ARGUMENT, "cache store sizes must be below 2^30");
+  if (key == nullptr || value == nullptr || positions == nullptr ||
+      (d.capacity > 0 && (key_cache == nullptr || value_cache == nullptr)))
+    return fail(TCX_INVALID_ARGUMENT, "cache store buffers are null");
+  if (!aligned16(key) || !aligned16(value) || !aligned16(key_cache) || !aligned16(value_cache))
+    return fail(TCX_INVALID_ARGUMENT, "cache store buffers must be 16-byte aligned");
+  StoreArgs a{};
+  for (int w = 0; w < 2; ++w) {
+    const std::int64_t(&in)[3] = w == 0 ? d.key_strides : d.value_strides;
+    const bool contiguous = in[0] == 0 && in[1] == 0 && in[2] == 0;
+    a.stride[w][2] = contiguous ? d.features : in[2];
+    a.stride[w][1] = contiguous ? d.tokens * d.features : in[1];
+    a.stride[w][0] = contiguous ? d.kv_heads * d.tokens * d.features : in[0];
+    for (std::int64_t s : a.stride[w])
+      if (s < 0 || s % 4 != 0)
+        return fail(TCX_INVALID_ARGUMENT, "cache store strides must be non-negative multiples of 4");
+  }
+  if (int rc = ready(); rc != TCX_OK) return rc;
+  a.x[0] = key;
+  a.x[1] = value;
+  a.cache[0] = key_cache;
+  a.cache[1] = value_cache;
+  a.positions = positions;
+  a.flag = d.flag;
+  a.tokens_all = d.batch * d.kv_heads * d.tokens;
+  a.kv_heads = static_cast<int>(d.kv_heads);
+  a.tokens = static_cast<int>(d.tokens);
+  a.capacity = d.capacity;
+  const dim3 grid(grid_for(a.tokens_all, 16, kStrideBlocks), 2);
+  const auto s = static_cast<hipStream_t>(stream);
+  if (d.features == 32) hipLaunchKernelGGL(cache_store_kernel<32>, grid, dim3(256), 0, s, a);
+  else if (d.features == 64) hipLaunchKernelGGL(cache_store_kernel<64>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(cache_store_kernel<128>, grid, dim3(256), 0, s, a);
+  return check(hipGetLastError(), "cache store launch");
+}
+
+int tcx_hip_cache4_load(const int32_t* cache, float* out, int64_t heads, int64_t capacity, int64_t start, int64_t count,
+                        int64_t features, tcx_stream_t stream) {
+  using namespace tcx;
+  if (heads < 0 || capacity < 0 || start < 0 || count < 0)
+    return fail(TCX_INVALID_ARGUMENT, "cache load extents must be non-negative");
+  if (tcx_hip_cache4_words(features) == 0)
+    return fail(TCX_INVALID_ARGUMENT, "a 4-bit cache holds 32, 64 or 128 features");
+  if (start > capacity || count > capacity - start)
+    return fail(TCX_INVALID_ARGUMENT, "cache load slots lie past the capacity");
+  if (heads == 0 || count == 0) return TCX_OK;
+  if (cache == nullptr || out == nullptr) return fail(TCX_INVALID_ARGUMENT, "cache load buffers are null");
+  if (!aligned16(cache) || !aligned16(out))
+    return fail(TCX_INVALID_ARGUMENT, "cache load buffers must be 16-byte aligned");
+  if (int rc = ready(); rc != TCX_OK) return rc;
+  const std::int64_t n = heads * count;
+  const dim3 grid(grid_for(n, 16, kStrideBlocks));
+  const auto s = static_cast<hipStream_t>(stream);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, cache, out, n, capacity, start, count); };
+  if (features == 32) go(cache_load_kernel<32>);
+  else if (features == 64) go(cache_load_kernel<64>);
+  else go(cache_load_kernel<128>);
+  return check(hipGetLastError(), "cache load launch");
+}
+
+size_t tcx_hip_cache4_attention_workspace_bytes(const tcx_hip_window_attention_desc_t* desc) {
+  using namespace tcx;
+  DecodeArgs a{};
+  bool done = false;
+  alignas(16) static float any[4];  // an aligned address; not touched
+  if (decode_args(any, any, any, any, desc, true, a, done) != TCX_OK || done) return 0;
+  return split_bytes(a, cache_splits(a, SIZE_MAX));
+}
+
+int tcx_hip_cache4_attention_f32(const float* q, const int32_t* key_cache, const int32_t* value_cache, float* out,
+                                 const tcx_hip_window_attention_desc_t* desc, void* workspace, size_t workspace_bytes,
+                                 tcx_stream_t stream) {
+  using namespace tcx;
+  DecodeArgs a{};
+  bool done = false;
+  if (int rc = decode_args(q, key_cache, value_cache, out, desc, true, a, done); rc != TCX_OK || done) return rc;
+  if (!aligned16(workspace)) return fail(TCX_INVALID_ARGUMENT, "attention workspace must be 16-byte aligned");
+  if (int rc = ready(); rc != TCX_OK) return rc;
+  const auto s = static_cast<hipStream_t>(stream);
+  place_split(a, cache_splits(a, workspace != nullptr ? workspace_bytes : 0), workspace);
+  int rc = a.features == 32 ? launch_stream<CacheRows<32>>(a, s)
+           : a.features == 64 ? launch_stream<CacheRows<64>>(a, s)
+                              : launch_stream<CacheRows<128>>(a, s);
+  if (rc == TCX_OK && a.splits > 1) rc = join_splits(a, s);
+  return rc;
+}
+
+}  // extern "C"

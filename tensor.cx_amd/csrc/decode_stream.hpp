@@ -1,0 +1,190 @@
+// Attention of a few rows over a long run of keys that streams past them.
+//
+// A block takes kRows rows of one key head (queries of the heads that share it,
+// neighbours first) and a share of the keys that they see. Sixteen lanes hold a
+// key, D / 16 features each, so that a wave takes four keys at a time and a
+// block sixteen; each group of lanes keeps an online softmax of its own (the
+// running maximum m in units of log2, the sum l, the outputs o) and the sixteen
+// states are joined at the end, in registers across a wave's groups and in LDS
+// across the waves.
+#pragma once
+
+#include "decoding.hpp"
+
+namespace tcx {
+
+template <class Source, int kRows, int kEach>
+__global__ __launch_bounds__(256) void stream_attention_kernel(DecodeArgs a, std::int64_t items, int row_tiles) {
+  constexpr int kF = Source::kFeatures, D = 16 * kF;
+  constexpr float kLog2e = 1.44269502F;
+  __shared__ float part_o[4][kRows][D];
+  __shared__ float part_m[4][kRows], part_l[4][kRows];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, li = lane & 15, group = t >> 4;
+  const float neg_inf = -__builtin_inff();
+  const int total = a.rows * a.share;
+  for (std::int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int split = static_cast<int>(item % a.splits);
+    const std::int64_t rest = item / a.splits;
+    const int tile = static_cast<int>(rest % row_tiles), head = static_cast<int>(rest / row_tiles);
+    const int b = head / a.kv_heads, kv = head % a.kv_heads;
+    const int r0 = tile * kRows, r1 = min(r0 + kRows, total) - 1;
+    const int n = checked_length(a, b);
+    const int i0 = r0 / a.share, i1 = r1 / a.share;
+    const SeenKeys seen = seen_keys(n, a.rows, i0, i1, a.window, a.sinks);
+    const int u0 = static_cast<int>(static_cast<std::int64_t>(seen.count()) * split / a.splits);
+    const int u1 = static_cast<int>(static_cast<std::int64_t>(seen.count()) * (split + 1) / a.splits);
+
+    float q[kRows][kF], o[kRows][kF], m[kRows], l[kRows];
+    int p_row[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const RowPlace at = row_place(a, kv, min(r0 + r, r1));
+      const float* row = a.q + b * a.q_stride[0] + at.head * a.q_stride[1] + at.query * a.q_stride[2];
+#pragma unroll
+      for (int e = 0; e < kF; ++e) {
+        const int f = Source::feature(li, e);
+        // The scale and log2 e go into the query: scores come out in units of log2.
+        q[r][e] = f < a.features ? row[f] * (a.scale * kLog2e) : 0.F;
+        o[r][e] = 0.F;
+      }
+      p_row[r] = n - a.rows + at.query;
+      m[r] = neg_inf;
+      l[r] = 0.F;
+    }
+    const Source source(a, b, kv, li);
+
+    // Keys of [u0, u1) from `base` on. kMasked: some key is not seen by all of
+    // the rows, or lies past the end; its value is left out, not weighted with 0,
+    // which would let a NaN through.
+    auto pass = [&]<bool kMasked>(int base) {
+      typename Source::Raw kr[kEach], vr[kEach];
+      int key[kEach];
+#pragma unroll
+      for (int u = 0; u < kEach; ++u) {
+        key[u] = seen.key(min(base + 16 * u + group, u1 - 1));
+        source.load(a.k, source.k_base, a.k_stride[2], key[u], kr[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kEach; ++u) source.load(a.v, source.v_base, a.v_stride[2], key[u], vr[u]);
+      float s[kRows][kEach];
+#pragma unroll
+      for (int u = 0; u < kEach; ++u) {
+        float x[kF];
+        source.values(kr[u], x);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          float dot = 0.F;
+#pragma unroll
+          for (int e = 0; e < kF; ++e) dot = fmaf(q[r][e], x[e], dot);
+          s[r][u] = lanes16_sum(dot);
+          if (kMasked && !(base + 16 * u + group < u1 && sees(p_row[r], key[u], a.window, a.sinks))) s[r][u] = neg_inf;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        float top = m[r];
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) top = fmaxf(top, s[r][u]);
+        const float at = top == neg_inf ? 0.F : top;  // nothing seen yet
+        const float f = __builtin_amdgcn_exp2f(m[r] - at);
+        m[r] = top;
+        l[r] *= f;
+#pragma unroll
+        for (int e = 0; e < kF; ++e) o[r][e] *= f;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+          s[r][u] = __builtin_amdgcn_exp2f(s[r][u] - at);
+          l[r] += s[r][u];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kEach; ++u) {
+        float x[kF];
+        source.values(vr[u], x);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          const bool in =
+              !kMasked || (base + 16 * u + group < u1 && sees(p_row[r], key[u], a.window, a.sinks));
+#pragma unroll
+          for (int e = 0; e < kF; ++e) o[r][e] = in ? fmaf(s[r][u], x[e], o[r][e]) : o[r][e];
+        }
+      }
+    };
+    int base = u0;
+    if (i0 == i1)
+      for (; base + 16 * kEach <= u1; base += 16 * kEach) pass.template operator()<false>(base);
+    for (; base < u1; base += 16 * kEach) pass.template operator()<true>(base);
+
+    // The wave's four groups, then the block's four waves.
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      float top = fmaxf(m[r], __shfl_xor(m[r], 16, kWave));
+      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      const float f = __builtin_amdgcn_exp2f(m[r] - (top == neg_inf ? 0.F : top));
+      l[r] *= f;
+      l[r] += __shfl_xor(l[r], 16, kWave);
+      l[r] += __shfl_xor(l[r], 32, kWave);
+#pragma unroll
+      for (int e = 0; e < kF; ++e) {
+        float v = o[r][e] * f;
+        v += __shfl_xor(v, 16, kWave);
+        v += __shfl_xor(v, 32, kWave);
+        if (lane < 16) part_o[wave][r][Source::feature(li, e)] = v;
+      }
+      if (lane == 0) {
+        part_m[wave][r] = top;
+        part_l[wave][r] = l[r];
+      }
+    }
+    __syncthreads();
+    for (int i = t; i < (r1 - r0 + 1) * D; i += 256) {
+      const int r = i / D, f = i % D;
+      if (f >= a.features) continue;
+      float top = part_m[0][r];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) top = fmaxf(top, part_m[w][r]);
+      const float at = top == neg_inf ? 0.F : top;
+      float sum = 0.F, value = 0.F;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float weight = __builtin_amdgcn_exp2f(part_m[w][r] - at);
+        sum = fmaf(part_l[w][r], weight, sum);
+        value = fmaf(part_o[w][r][f], weight, value);
+      }
+      if (a.splits == 1) {
+        const RowPlace place = row_place(a, kv, r0 + r);
+        a.out[b * a.out_stride[0] + place.head * a.out_stride[1] + place.query * a.out_stride[2] + f] =
+            sum == 0.F ? 0.F : value / sum;  // a row that sees nothing: zeros
+      } else {
+        const std::int64_t row = (static_cast<std::int64_t>(split) * a.batch * a.kv_heads + head) * total + r0 + r;
+        a.part[row * a.features + f] = value;
+        if (f == 0) {
+          a.part_ml[2 * row] = top;
+          a.part_ml[2 * row + 1] = sum;
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Rows a block of stream_attention_kernel takes.
+inline int stream_rows(const DecodeArgs& a) {
+  const int total = a.rows * a.share;
+  return total <= 1 ? 1 : total <= 2 ? 2 : total <= 4 ? 4 : 8;
+}
+
+template <class Source>
+int launch_stream(const DecodeArgs& a, hipStream_t s) {
+  const int rows = stream_rows(a), tiles = (a.rows * a.share + rows - 1) / rows;
+  const std::int64_t items = static_cast<std::int64_t>(a.batch) * a.kv_heads * tiles * a.splits;
+  const unsigned grid = grid_for(items, 1, 1 << 22);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, a, items, tiles); };
+  if (rows == 1) go(stream_attention_kernel<Source, 1, 4>);
+  else if (rows == 2) go(stream_attention_kernel<Source, 2, 4>);
+  else if (rows == 4) go(stream_attention_kernel<Source, 4, 2>);
+  else go(stream_attention_kernel<Source, 8, 2>);
+  return check(hipGetLastError(), "attention launch");
+}
+
+}  // namespace tcx

@@ -576,4 +576,18 @@ int tcx_hip_event_destroy(void* event) {
   return tcx::check(hipEventDestroy(static_cast<hipEvent_t>(event)), "hipEventDestroy");
 }
 
+int tcx_hip_flag_acquire(int32_t** flag) {
+  if (flag == nullptr) return tcx::fail(TCX_INVALID_ARGUMENT, "flag output is null");
+  *flag = nullptr;
+  if (int rc = tcx::ready(); rc != TCX_OK) return rc;
+  *flag = tcx::acquire_host_flag();
+  if (*flag == nullptr) return tcx::fail(TCX_INTERNAL, "no pinned host memory for a flag");
+  **flag = 0;
+  return TCX_OK;
+}
+
+void tcx_hip_flag_release(int32_t* flag) {
+  if (flag != nullptr) tcx::release_host_flag(flag);
+}
+
 }  // extern "C"

@@ -1,0 +1,228 @@
+// Attention with a sliding window and sinks over float32 keys and values, and
+// what the attentions of a decoding loop share on the host: checked arguments,
+// key splits and their join.
+
+#include <algorithm>
+#include <cmath>
+#include <limits>
+
+#include "decode_stream.hpp"
+
+namespace tcx {
+namespace {
+
+// Rows of float32, `features` of them (a multiple of 8) in D: a lane holds the
+// chunks of four (two for D = 32) at 16 lanes' distance.
+template <int D>
+struct FloatRows {
+  static constexpr int kFeatures = D / 16, kChunk = D >= 64 ? 4 : 2, kChunks = kFeatures / kChunk;
+  using Chunk = float __attribute__((ext_vector_type(kChunk)));
+  struct Raw {
+    Chunk c[kChunks];
+  };
+  static __device__ __forceinline__ int feature(int li, int e) {
+    return kChunk * (16 * (e / kChunk) + li) + e % kChunk;
+  }
+  std::int64_t k_base, v_base;
+  int li, features;
+  __device__ FloatRows(const DecodeArgs& a, int b, int kv, int lane)
+      : k_base(b * a.k_stride[0] + kv * a.k_stride[1]), v_base(b * a.v_stride[0] + kv * a.v_stride[1]), li(lane),
+        features(a.features) {}
+  __device__ __forceinline__ void load(const void* p, std::int64_t base, std::int64_t stride, int key, Raw& raw) const {
+    const float* row = static_cast<const float*>(p) + base + key * stride;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      const int f = feature(li, c * kChunk);
+      // Chunks past the last feature read chunk 0 and count as zero.
+      raw.c[c] = stream_load(reinterpret_cast<const Chunk*>(row + (f < features ? f : 0)));
+      if (f >= features) raw.c[c] = Chunk{};
+    }
+  }
+  __device__ __forceinline__ void values(const Raw& raw, float (&x)[kFeatures]) const {
+#pragma unroll
+    for (int e = 0; e < kFeatures; ++e) x[e] = raw.c[e / kChunk][e % kChunk];
+  }
+};
+
+// Joins the split states of a row: a wave each, a lane a split for the weights.
+__global__ __launch_bounds__(256) void join_splits_kernel(DecodeArgs a, std::int64_t rows) {
+  const int lane = threadIdx.x & 63, total = a.rows * a.share;
+  const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * 4;
+  for (std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); row < rows; row += step) {
+    const std::int64_t at = lane < a.splits ? lane * rows + row : row;
+    const float m = lane < a.splits ? a.part_ml[2 * at] : -__builtin_inff();
+    const float l = lane < a.splits ? a.part_ml[2 * at + 1] : 0.F;
+    float top = m;
+#pragma unroll
+    for (int offset = 32; offset > 0; offset >>= 1) top = fmaxf(top, __shfl_xor(top, offset, kWave));
+    const float weight = __builtin_amdgcn_exp2f(m - (top == -__builtin_inff() ? 0.F : top));
+    const float sum = wave_sum(l * weight);
+    const int head = static_cast<int>(row / total), b = head / a.kv_heads;
+    const RowPlace place = row_place(a, head % a.kv_heads, static_cast<int>(row % total));
+    float* out = a.out + b * a.out_stride[0] + place.head * a.out_stride[1] + place.query * a.out_stride[2];
+    const bool low = lane < a.features, high = lane + 64 < a.features;
+    float x = 0.F, y = 0.F;
+    for (int s = 0; s < a.splits; ++s) {
+      const float w = __shfl(weight, s, kWave);
+      const float* part = a.part + (s * rows + row) * a.features;
+      if (low) x = fmaf(part[lane], w, x);
+      if (high) y = fmaf(part[lane + 64], w, y);
+    }
+    if (low) out[lane] = sum == 0.F ? 0.F : x / sum;
+    if (high) out[lane + 64] = sum == 0.F ? 0.F : y / sum;
+  }
+}
+
+constexpr std::int64_t kMostIndex = std::int64_t{1} << 30;
+
+bool all_zero(const std::int64_t (&s)[3]) { return s[0] == 0 && s[1] == 0 && s[2] == 0; }
+
+// The strides asked for, or the contiguous ones of (batch, heads, tokens, features).
+bool fill_strides(const std::int64_t (&in)[3], std::int64_t heads, std::int64_t tokens, std::int64_t features,
+                  std::int64_t (&out)[3]) {
+  if (all_zero(in)) {
+    out[2] = features;
+    out[1] = tokens * features;
+    out[0] = heads * tokens * features;
+    return true;
+  }
+  for (int i = 0; i < 3; ++i) {
+    if (in[i] < 0 || in[i] % 4 != 0) return false;
+    out[i] = in[i];
+  }
+  return true;
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15U) == 0; }
+
+// Splits of the keys: enough blocks to fill the CUs several times, with at
+// least kSplitKeys keys in each.
+constexpr int kMostSplits = 64;  // join_splits_kernel: a lane each
+
+}  // namespace
+
+int decode_args(const float* q, const void* k, const void* v, float* out, const tcx_hip_window_attention_desc_t* desc,
+                bool cache, DecodeArgs& a, bool& done) {
+  if (desc == nullptr) return fail(TCX_INVALID_ARGUMENT, "attention descriptor is null");
+  const auto& d = *desc;
+  if (d.batch < 0 || d.heads < 0 || d.kv_heads < 0 || d.rows < 0 || d.cols < 0)
+    return fail(TCX_INVALID_ARGUMENT, "attention extents must be non-negative");
+  if (cache ? tcx_hip_cache4_words(d.features) == 0 : !tcx_hip_window_attention_supported(d.features))
+    return fail(TCX_INVALID_ARGUMENT, cache ? "a 4-bit cache holds 32, 64 or 128 features"
+                                            : "window attention takes a multiple of 8 features from 16 to 128");
+  if (d.kv_heads == 0 ? d.heads != 0 : d.heads % d.kv_heads != 0)
+    return fail(TCX_INVALID_ARGUMENT, "attention heads must be a multiple of the key heads");
+  if (d.window < 0 || d.sinks < 0) return fail(TCX_INVALID_ARGUMENT, "attention window and sinks must be non-negative");
+  if (!std::isfinite(d.scale)) return fail(TCX_INVALID_ARGUMENT, "attention scale must be finite");
+  done = d.batch == 0 || d.heads == 0 || d.rows == 0;
+  if (done) return TCX_OK;
+  const std::int64_t share = d.heads / d.kv_heads;
+  if (d.cols >= kMostIndex || d.rows >= kMostIndex / share || d.batch >= kMostIndex / d.kv_heads)
+    return fail(TCX_INVALID_ARGUMENT, "attention sizes must be below 2^30");
+  // Lengths may leave cols keys unread, but a call of no keys needs none.
+  if (q == nullptr || out == nullptr || (d.cols > 0 && (k == nullptr || v == nullptr)))
+    return fail(TCX_INVALID_ARGUMENT, "attention buffers are null");
+  if (!aligned(q) || !aligned(k) || !aligned(v) || !aligned(out))
+    return fail(TCX_INVALID_ARGUMENT, "attention buffers must be 16-byte aligned");
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.lengths = d.lengths;
+  a.flag = d.flag;
+  a.batch = static_cast<int>(d.batch);
+  a.heads = static_cast<int>(d.heads);
+  a.kv_heads = static_cast<int>(d.kv_heads);
+  a.share = static_cast<int>(share);
+  a.rows = static_cast<int>(d.rows);
+  a.cols = static_cast<int>(d.cols);
+  a.features = static_cast<int>(d.features);
+  // A window of cols keys hides none.
+  a.window = d.window >= d.cols ? 0 : static_cast<int>(d.window);
+  a.sinks = static_cast<int>(std::min(d.sinks, d.cols));
+  a.scale = d.scale;
+  const std::int64_t words = cache ? tcx_hip_cache4_words(d.features) : 0;
+  static constexpr std::int64_t kContiguous[3] = {0, 0, 0};
+  if (!fill_strides(d.q_strides, d.heads, d.rows, d.features, a.q_stride) ||
+      !fill_strides(d.out_strides, d.heads, d.rows, d.features, a.out_stride) ||
+      !fill_strides(cache ? kContiguous : d.k_strides, d.kv_heads, d.cols, cache ? words : d.features, a.k_stride) ||
+      !fill_strides(cache ? kContiguous : d.v_strides, d.kv_heads, d.cols, cache ? words : d.features, a.v_stride))
+    return fail(TCX_INVALID_ARGUMENT, "attention strides must be non-negative multiples of 4");
+  a.splits = 1;
+  a.part = a.part_ml = nullptr;
+  return TCX_OK;
+}
+
+std::size_t split_bytes(const DecodeArgs& a, int splits) {
+  if (splits <= 1) return 0;
+  return sizeof(float) * static_cast<std::size_t>(splits) * a.batch * a.kv_heads * a.rows * a.share * (a.features + 2);
+}
+
+void place_split(DecodeArgs& a, int splits, void* workspace) {
+  a.splits = splits;
+  if (splits <= 1) return;
+  a.part = static_cast<float*>(workspace);
+  a.part_ml = a.part + static_cast<std::size_t>(splits) * a.batch * a.kv_heads * a.rows * a.share * a.features;
+}
+
+int plan_splits(const DecodeArgs& a, std::int64_t blocks, int split_keys, std::size_t workspace_bytes) {
+  std::int64_t keys = a.cols;  // a block's rows see at most this many
+  if (a.window > 0) keys = std::min<std::int64_t>(keys, std::int64_t{a.window} + a.sinks + a.rows - 1);
+  std::int64_t splits = std::min<std::int64_t>({kMostSplits, 1024 / std::max<std::int64_t>(1, blocks), keys / split_keys});
+  while (splits > 1 && split_bytes(a, static_cast<int>(splits)) > workspace_bytes) --splits;
+  return static_cast<int>(std::max<std::int64_t>(1, splits));
+}
+
+int join_splits(const DecodeArgs& a, hipStream_t s) {
+  const std::int64_t rows = static_cast<std::int64_t>(a.batch) * a.kv_heads * a.rows * a.share;
+  hipLaunchKernelGGL(join_splits_kernel, dim3(grid_for(rows, 4, kStrideBlocks)), dim3(256), 0, s, a, rows);
+  return check(hipGetLastError(), "attention join launch");
+}
+
+namespace {
+
+int window_splits(const DecodeArgs& a, std::size_t workspace_bytes) {
+  const int rows = stream_rows(a);
+  const std::int64_t blocks = static_cast<std::int64_t>(a.batch) * a.kv_heads * ((a.rows * a.share + rows - 1) / rows);
+  return plan_splits(a, blocks, 128, workspace_bytes);
+}
+
+}  // namespace
+}  // namespace tcx
+
+extern "C" {
+
+int tcx_hip_window_attention_supported(int64_t features) {
+  return features >= 16 && features <= 128 && features % 8 == 0 ? 1 : 0;
+}
+
+size_t tcx_hip_window_attention_workspace_bytes(const tcx_hip_window_attention_desc_t* desc) {
+  using namespace tcx;
+  DecodeArgs a{};
+  bool done = false;
+  // Any aligned address passes for the buffers, which are not touched.
+  alignas(16) static float any[4];
+  if (decode_args(any, any, any, any, desc, false, a, done) != TCX_OK || done) return 0;
+  return split_bytes(a, window_splits(a, SIZE_MAX));
+}
+
+int tcx_hip_window_attention_f32(const float* q, const float* k, const float* v, float* out,
+                                 const tcx_hip_window_attention_desc_t* desc, void* workspace, size_t workspace_bytes,
+                                 tcx_stream_t stream) {
+  using namespace tcx;
+  DecodeArgs a{};
+  bool done = false;
+  if (int rc = decode_args(q, k, v, out, desc, false, a, done); rc != TCX_OK || done) return rc;
+  if (workspace != nullptr && (reinterpret_cast<std::uintptr_t>(workspace) & 15U))
+    return fail(TCX_INVALID_ARGUMENT, "attention workspace must be 16-byte aligned");
+  if (int rc = ready(); rc != TCX_OK) return rc;
+  const auto s = static_cast<hipStream_t>(stream);
+  place_split(a, window_splits(a, workspace != nullptr ? workspace_bytes : 0), workspace);
+  int rc = a.features <= 32 ? launch_stream<FloatRows<32>>(a, s)
+           : a.features <= 64 ? launch_stream<FloatRows<64>>(a, s)
+                              : launch_stream<FloatRows<128>>(a, s);
+  if (rc == TCX_OK && a.splits > 1) rc = join_splits(a, s);
+  return rc;
+}
+
+}  // extern "C"

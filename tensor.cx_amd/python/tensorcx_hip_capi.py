@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
+from typing import NamedTuple
 
 import numpy as np
 
@@ -47,6 +48,11 @@ EXPORTS = [
     "tcx_hip_flash_attention_plan", "tcx_hip_flash_attention_f32_ws",
     "tcx_hip_gather_strided", "tcx_hip_copy_blocks", "tcx_hip_concat", "tcx_hip_cast", "tcx_hip_scalar_op", "tcx_hip_predicate",
     "tcx_hip_bool_reduce", "tcx_hip_mask_chunks", "tcx_hip_mask_count", "tcx_hip_masked_select",
+    "tcx_hip_flag_acquire", "tcx_hip_flag_release", "tcx_hip_window_attention_supported",
+    "tcx_hip_window_attention_workspace_bytes", "tcx_hip_window_attention_f32", "tcx_hip_cache4_words",
+    "tcx_hip_cache4_store", "tcx_hip_cache4_load", "tcx_hip_cache4_attention_workspace_bytes",
+    "tcx_hip_cache4_attention_f32", "tcx_hip_beam_select_workspace_bytes", "tcx_hip_beam_select_f32",
+    "tcx_hip_beam_reorder",
 ]
 
 
@@ -73,6 +79,18 @@ class GemmDesc(ctypes.Structure):
                 ("lhs_batch_strides", ctypes.c_int64 * MAX_BATCH_RANK),
                 ("rhs_batch_strides", ctypes.c_int64 * MAX_BATCH_RANK),
                 ("bias", ctypes.c_void_p), ("activation", ctypes.c_int32)]
+
+
+class WindowAttentionDesc(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int64) for name in (
+        "batch", "heads", "kv_heads", "rows", "cols", "features", "window", "sinks")] + [
+        ("scale", ctypes.c_float), ("lengths", ctypes.c_void_p), ("flag", ctypes.c_void_p)] + [
+        (name, ctypes.c_int64 * 3) for name in ("q_strides", "k_strides", "v_strides", "out_strides")]
+
+
+class Cache4StoreDesc(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int64) for name in ("batch", "kv_heads", "tokens", "capacity", "features")] + [
+        ("flag", ctypes.c_void_p), ("key_strides", ctypes.c_int64 * 3), ("value_strides", ctypes.c_int64 * 3)]
 
 
 ALLOCATE_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.POINTER(ctypes.c_void_p), ctypes.c_size_t)
@@ -150,6 +168,23 @@ def lib() -> ctypes.CDLL:
         L.tcx_hip_flash_attention_ws_supported.argtypes = [i64, i64]
         L.tcx_hip_flash_attention_f32.argtypes = [vp, vp, vp, vp, i64, i64, i64, i64, ctypes.c_float,
                                                   ctypes.c_int, vp]
+        desc = ctypes.POINTER(WindowAttentionDesc)
+        L.tcx_hip_flag_acquire.argtypes = [ctypes.POINTER(vp)]
+        L.tcx_hip_flag_release.argtypes = [vp]
+        L.tcx_hip_flag_release.restype = None
+        L.tcx_hip_window_attention_supported.argtypes = [i64]
+        for name in ("tcx_hip_window_attention", "tcx_hip_cache4_attention"):
+            query = getattr(L, name + "_workspace_bytes")
+            query.argtypes, query.restype = [desc], sz
+            getattr(L, name + "_f32").argtypes = [vp, vp, vp, vp, desc, vp, sz, vp]
+        L.tcx_hip_cache4_words.argtypes = [i64]
+        L.tcx_hip_cache4_words.restype = i64
+        L.tcx_hip_cache4_store.argtypes = [vp, vp, vp, vp, vp, ctypes.POINTER(Cache4StoreDesc), vp]
+        L.tcx_hip_cache4_load.argtypes = [vp, vp, i64, i64, i64, i64, i64, vp]
+        L.tcx_hip_beam_select_workspace_bytes.argtypes = [i64, i64, i64, i64]
+        L.tcx_hip_beam_select_workspace_bytes.restype = sz
+        L.tcx_hip_beam_select_f32.argtypes = [vp, vp, vp, ctypes.c_int32, vp, vp, vp, i64, i64, i64, i64, vp, sz, vp]
+        L.tcx_hip_beam_reorder.argtypes = [vp, vp, vp, ctypes.c_int32, vp, i64, i64, i64, vp, vp]
         _LIB = L
     return _LIB
 
@@ -365,3 +400,97 @@ def flash_attention(q, k, v, out, batch: int, rows: int, cols: int, features: in
     """Fused attention on device pointers (tcx_hip_flash_attention_f32)."""
     check(lib().tcx_hip_flash_attention_f32(q, k, v, out, batch, rows, cols, features, scale, int(causal),
                                             stream_ or stream()), "flash_attention")
+
+
+# ------------------------------------------------------------------ decoding
+class Workspace(NamedTuple):
+    """Scratch memory of the caller's (any 16-byte aligned device memory)."""
+    address: int
+    nbytes: int
+
+
+def _on(s: int | None) -> int:
+    """A stream handle: the thread's for None; 0 is HIP's default stream."""
+    return stream() if s is None else s
+
+
+def window_attention_desc(batch, heads, kv_heads, rows, cols, features, *, window=0, sinks=0, scale=None,
+                          lengths: int | None = None, flag: int | None = None, q_strides=(0, 0, 0),
+                          k_strides=(0, 0, 0), v_strides=(0, 0, 0), out_strides=(0, 0, 0)) -> WindowAttentionDesc:
+    """Arguments of window_attention and cache4_attention (cols is the cache's capacity)."""
+    d = WindowAttentionDesc(batch, heads, kv_heads, rows, cols, features, window, sinks)
+    d.scale = scale if scale is not None else features ** -0.5 if features > 0 else 1.0
+    d.lengths, d.flag = lengths, flag
+    d.q_strides[:], d.k_strides[:], d.v_strides[:], d.out_strides[:] = q_strides, k_strides, v_strides, out_strides
+    return d
+
+
+def window_attention_workspace(desc: WindowAttentionDesc, cache: bool = False) -> DeviceBuffer | None:
+    """The workspace that window_attention (cache4_attention with `cache`) can use (None when it needs none)."""
+    query = lib().tcx_hip_cache4_attention_workspace_bytes if cache else lib().tcx_hip_window_attention_workspace_bytes
+    nbytes = query(ctypes.byref(desc))
+    return DeviceBuffer(nbytes) if nbytes else None
+
+
+def window_attention(q: int, k: int, v: int, out: int, desc: WindowAttentionDesc, workspace=None, s=None) -> None:
+    check(lib().tcx_hip_window_attention_f32(q, k, v, out, ctypes.byref(desc), *_ws_args(workspace), _on(s)),
+          "window_attention")
+
+
+def cache4_words(features: int) -> int:
+    """int32 words of a cached token and head (0: these features are not taken)."""
+    return lib().tcx_hip_cache4_words(features)
+
+
+def cache4_store_desc(batch, kv_heads, tokens, capacity, features, *, flag: int | None = None, key_strides=(0, 0, 0),
+                      value_strides=(0, 0, 0)) -> Cache4StoreDesc:
+    d = Cache4StoreDesc(batch, kv_heads, tokens, capacity, features, flag)
+    d.key_strides[:], d.value_strides[:] = key_strides, value_strides
+    return d
+
+
+def cache4_store(key: int, value: int, key_cache: int, value_cache: int, positions: int, desc: Cache4StoreDesc,
+                 s=None) -> None:
+    check(lib().tcx_hip_cache4_store(key, value, key_cache, value_cache, positions, ctypes.byref(desc), _on(s)),
+          "cache4_store")
+
+
+def cache4_load(cache: int, out: int, heads: int, capacity: int, start: int, count: int, features: int, s=None) -> None:
+    check(lib().tcx_hip_cache4_load(cache, out, heads, capacity, start, count, features, _on(s)), "cache4_load")
+
+
+def cache4_attention(q: int, key_cache: int, value_cache: int, out: int, desc: WindowAttentionDesc, workspace=None,
+                     s=None) -> None:
+    check(lib().tcx_hip_cache4_attention_f32(q, key_cache, value_cache, out, ctypes.byref(desc), *_ws_args(workspace),
+                                             _on(s)), "cache4_attention")
+
+
+def beam_select_workspace(batch: int, beams: int, vocabulary: int, count: int) -> DeviceBuffer | None:
+    nbytes = lib().tcx_hip_beam_select_workspace_bytes(batch, beams, vocabulary, count)
+    return DeviceBuffer(nbytes) if nbytes else None
+
+
+def beam_select(logits: int, scores: int, out_scores: int, out_beams: int, out_tokens: int, batch: int, beams: int,
+                vocabulary: int, count: int, *, finished: int | None = None, eos: int = 0, workspace=None, s=None) -> None:
+    check(lib().tcx_hip_beam_select_f32(logits, scores, finished, eos, out_scores, out_beams, out_tokens, batch, beams,
+                                        vocabulary, count, *_ws_args(workspace), _on(s)), "beam_select")
+
+
+class BeamReorderPlan(NamedTuple):
+    sources: ctypes.Array
+    targets: ctypes.Array
+    row_bytes: ctypes.Array
+
+
+def beam_reorder_plan(sources, targets, row_bytes) -> BeamReorderPlan:
+    """The tensors of a reorder: addresses, and the bytes of a row of each."""
+    n = len(sources)
+    if len(targets) != n or len(row_bytes) != n:
+        raise ValueError("a reorder has as many targets and row sizes as sources")
+    return BeamReorderPlan((ctypes.c_void_p * n)(*sources), (ctypes.c_void_p * n)(*targets), (ctypes.c_int64 * n)(*row_bytes))
+
+
+def beam_reorder(plan: BeamReorderPlan, index: int, batch: int, beams: int, count: int, flag: int | None = None,
+                 s=None) -> None:
+    check(lib().tcx_hip_beam_reorder(plan.sources, plan.targets, plan.row_bytes, len(plan.sources), index, batch, beams,
+                                     count, flag, _on(s)), "beam_reorder")
