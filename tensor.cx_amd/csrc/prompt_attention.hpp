@@ -1,0 +1,715 @@
+// Windowed attention of many rows (prompts, chunks) on matrix instructions.
+//
+// Products. The inputs are float32, and a float32 matrix instruction does 256
+// operations a cycle and CU where a float16 one does 4096. So every factor is
+// held as two float16 numbers, hi = half(x) and lo = half(x - hi), 22 bits
+// together, and a product is hi hi' + hi lo' + lo hi' with float32 sums: what is
+// left out, lo lo', and what lo rounds off are 2^-22 of the product, less than
+// what float32 sums of 64 and more terms lose. float16 has five bits of
+// exponent, so what is split is first multiplied by a power of two (exact) that
+// brings its largest magnitude into [2^14, 2^15): a query and a key row as a
+// whole, the values of a key as a whole. A number down to 2^-29 of the largest
+// in its row still keeps its 22 bits, and below that an absolute error of 2^-40
+// of the largest.
+//
+// Weights. With s the score in units of log2 and V_j = 2^e_j V'_j, the sum over
+// keys of 2^s_j V_j is one of 2^(s_j + e_j) V'_j: the running maximum M is that
+// of x_j = s_j + e_j, which is each row's own, so that no row's precision depends
+// on values that it does not see. P = 2^(x - M + 15) is at most 2^15, split as
+// above; the softmax's sum takes 2^-e_j P.
+//
+// Layout. A block takes 16 kQ rows a wave of one key head (row r: query r / share,
+// head r % share, so that neighbours see the same keys) and walks the keys that
+// its rows see, sinks and window in one run, in tiles of 64. Scores are computed
+// transposed, S^T = K Q^T: lane (n, g) = (lane % 16, lane / 16) then holds query
+// n's scores of keys 16 b + 4 g + v, which are the k indices 8 g .. 8 g + 7 that
+// it has to supply as P^T in O^T = V^T P^T once V's columns in LDS are in the
+// order (b even 4 g + v, b odd 4 g + v): the weights never leave their lane, and
+// neither do the query's maximum, sum and rescaling. V is transposed on its way
+// into LDS (rows are features, feature 4 c + e in row e D / 4 + c, so that the
+// lanes of a store and of a load meet 16 different slots of 16 bytes).
+//
+// Stages. K and V have one buffer each. Between barriers A and B a tile's V goes
+// from registers into LDS while its scores are computed and the next K is on its
+// way; between B and the next A that K goes into LDS while P V is computed and
+// the next V is on its way.
+#pragma once
+
+#include "decoding.hpp"
+
+namespace tcx {
+
+using half2_t = _Float16 __attribute__((ext_vector_type(2)));
+using half4_t = _Float16 __attribute__((ext_vector_type(4)));
+using half8_t = _Float16 __attribute__((ext_vector_type(8)));
+using float2v_t = float __attribute__((ext_vector_type(2)));
+using acc_t = float __attribute__((ext_vector_type(4)));
+
+// hi and lo halves of N scaled numbers.
+template <int N, typename H>
+__device__ __forceinline__ void split_halves(const float (&x)[N], H& hi, H& lo) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const half2_t h = __builtin_convertvector((float2v_t{x[i], x[i + 1]}), half2_t);
+    const half2_t l = __builtin_convertvector(
+        (float2v_t{x[i] - static_cast<float>(h[0]), x[i + 1] - static_cast<float>(h[1])}), half2_t);
+    hi[i] = h[0];
+    hi[i + 1] = h[1];
+    lo[i] = l[0];
+    lo[i + 1] = l[1];
+  }
+}
+
+__device__ __forceinline__ std::uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffU; }
+
+// The largest of kLanes neighbouring lanes' words, in all of them.
+template <int kLanes>
+__device__ __forceinline__ std::uint32_t lanes_most(std::uint32_t x) {
+  auto with = [&]<int kControl>() {
+    x = max(x, static_cast<std::uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), kControl, 0xf, 0xf, true)));
+  };
+  with.template operator()<0xb1>();
+  with.template operator()<0x4e>();
+  if constexpr (kLanes >= 8) with.template operator()<0x141>();
+  if constexpr (kLanes >= 16) with.template operator()<0x140>();
+  if constexpr (kLanes >= 32)
+    x = max(x, static_cast<std::uint32_t>(__builtin_amdgcn_ds_swizzle(static_cast<int>(x), 0x401f)));
+  return x;
+}
+
+// The exponent field of the power of two that brings a magnitude into [2^14,
+// 2^15), at most `most`.
+__device__ __forceinline__ int scale_field(std::uint32_t magnitude_bits, int most) {
+  return min(268 - static_cast<int>(magnitude_bits >> 23), most);
+}
+__device__ __forceinline__ float power_field(int field) { return __int_as_float(field << 23); }
+constexpr int kMostKeyField = 253;   // its inverse is a normal number
+constexpr int kMostValueField = 217; // 2^90: a sum of 2^20 weights stays finite
+
+// The slot of chunk c of 8 features of key row j, and of the 16 bytes of 8 keys at
+// chunk c of value row f: xored so that the lanes of a fragment meet different
+// banks.
+template <int D>
+__device__ __forceinline__ int key_slot(int j, int c) {
+  constexpr int kChunks = D / 8, kShift = D >= 128 ? 0 : D == 64 ? 1 : 2;
+  return j * kChunks + (c ^ ((j >> kShift) & (kChunks - 1) & 15));
+}
+__device__ __forceinline__ int value_slot(int row, int chunk) { return row * 8 + (chunk ^ ((row >> 1) & 7)); }
+
+// Chunk c of key j, from registers into the tile's buffers; D / 8 neighbouring
+// lanes hold a key.
+template <int D>
+__device__ __forceinline__ void pack_keys(const float4_t (&in)[2], int j, int c, half8_t* key_hi, half8_t* key_lo,
+                                          float* key_factor) {
+  float x[8];
+  std::uint32_t most = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    x[e] = in[e / 4][e % 4];
+    most = max(most, magnitude(x[e]));
+  }
+  const int field = scale_field(lanes_most<D / 8>(most), kMostKeyField);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] *= power_field(field);
+  half8_t hi, lo;
+  split_halves<8>(x, hi, lo);
+  if (j < 64) {
+    key_hi[key_slot<D>(j, c)] = hi;
+    key_lo[key_slot<D>(j, c)] = lo;
+    if (c == 0) key_factor[j] = power_field(254 - field);
+  }
+}
+
+// The powers of two of quad c (4 features) of the values of keys 4 h .. 4 h + 3;
+// D / 4 neighbouring lanes hold a key. Values that are not finite are taken out
+// and marked: a product with them would reach rows that do not see them.
+template <int D>
+__device__ __forceinline__ void measure_values(float4_t (&in)[4], int h, int c, int (&field)[4], float* value_exp,
+                                               float* value_unit, int* bad) {
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    std::uint32_t most = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) most = max(most, magnitude(in[v][e]));
+    if (__any(most >= 0x7f800000U)) {
+      if (most >= 0x7f800000U) {
+        most = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (magnitude(in[v][e]) >= 0x7f800000U) in[v][e] = 0.F;
+          most = max(most, magnitude(in[v][e]));
+        }
+        *bad = 1;
+      }
+    }
+    field[v] = scale_field(lanes_most<D / 4>(most), kMostValueField);
+    if (c == 0 && h < 16) {
+      value_exp[4 * h + v] = static_cast<float>(140 - field[v]);
+      value_unit[4 * h + v] = power_field(field[v] - 13);
+    }
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void pack_values(const float4_t (&in)[4], int h, int c, const int (&field)[4],
+                                            half4_t* value_hi, half4_t* value_lo) {
+  if (h >= 16) return;
+  // Keys 16 b + 4 g .. of h = 4 b + g: half b % 2 of chunk 4 (b / 2) + g.
+  const int chunk = 4 * (h >> 3) + (h & 3), half = (h >> 2) & 1;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float x[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) x[v] = in[v][e] * power_field(field[v]);
+    half4_t hi, lo;
+    split_halves<4>(x, hi, lo);
+    const int slot = 2 * value_slot(e * (D / 4) + c, chunk) + half;
+    value_hi[slot] = hi;
+    value_lo[slot] = lo;
+  }
+}
+
+// A wave's 16 kQ rows: queries as B operands, the running maxima, sums and outputs.
+template <int D, int kQ>
+struct PromptRows {
+  static constexpr int kSteps = D / 32, kT = D / 16, kQuads = D / 4;
+  half8_t q_hi[kQ][kSteps], q_lo[kQ][kSteps];  // lane (n, g): features 32 s + 8 g .. + 7 of query n
+  float row_factor[kQ];
+  int p_row[kQ];
+  acc_t o[kQ][kT];  // feature 4 (r % (D / 4)) + r / (D / 4) of query n at r = 16 i + 4 g + v
+  float m[kQ], l[kQ];
+  int first_row, last_row;  // the keys of the wave's first and last queries
+  int row0, n16, g;
+
+  __device__ __forceinline__ void start(const DecodeArgs& a, int b, int kv, int n, int r0, int r1, int lane) {
+    constexpr float kLog2e = 1.44269502F;
+    row0 = r0;
+    n16 = lane & 15;
+    g = lane >> 4;
+    first_row = n - a.rows + min(r0, r1) / a.share;
+    last_row = n - a.rows + min(r0 + kQ * 16 - 1, r1) / a.share;
+#pragma unroll
+    for (int x = 0; x < kQ; ++x) {
+      const RowPlace at = row_place(a, kv, min(r0 + 16 * x + n16, r1));
+      const float* row = a.q + b * a.q_stride[0] + at.head * a.q_stride[1] + at.query * a.q_stride[2];
+      p_row[x] = n - a.rows + at.query;
+      float q[kSteps][8];
+      std::uint32_t most = 0;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int f = 32 * s + 8 * g + 4 * c;
+          const float4_t w = f < a.features ? *reinterpret_cast<const float4_t*>(row + f) : float4_t{0.F, 0.F, 0.F, 0.F};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            q[s][4 * c + e] = w[e];
+            most = max(most, magnitude(w[e]));
+          }
+        }
+      most = max(most, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(most), 16, kWave)));
+      most = max(most, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(most), 32, kWave)));
+      const int field = scale_field(most, kMostKeyField);
+      row_factor[x] = power_field(254 - field) * (a.scale * kLog2e);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[s][e] *= power_field(field);
+        split_halves<8>(q[s], q_hi[x][s], q_lo[x][s]);
+      }
+#pragma unroll
+      for (int i = 0; i < kT; ++i) o[x][i] = acc_t{0.F, 0.F, 0.F, 0.F};
+      m[x] = -__builtin_inff();
+      l[x] = 0.F;
+    }
+  }
+
+  // Whether some row sees a key of [j0, j0 + 64), and whether each sees them all.
+  __device__ __forceinline__ bool any_seen(const DecodeArgs& a, int j0) const {
+    return j0 <= last_row && (a.window == 0 || j0 + 63 > first_row - a.window || j0 < a.sinks);
+  }
+  __device__ __forceinline__ bool all_seen(const DecodeArgs& a, int j0) const {
+    return j0 + 63 <= first_row && (a.window == 0 || j0 > last_row - a.window || j0 + 63 < a.sinks);
+  }
+
+  // A tile's weights, as B operands of the P V products. key_of(k): the key at
+  // place k of the tile, or one past every query.
+  template <typename F>
+  __device__ __forceinline__ void scores(const DecodeArgs& a, const half8_t* key_hi, const half8_t* key_lo,
+                                         const float* key_factor, const float* value_exp, const float* value_unit,
+                                         bool whole, F&& key_of, half8_t (&p_hi)[kQ][2], half8_t (&p_lo)[kQ][2]) {
+    const float neg_inf = -__builtin_inff();
+    acc_t s[kQ][4];
+#pragma unroll
+    for (int x = 0; x < kQ; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[x][i] = acc_t{0.F, 0.F, 0.F, 0.F};
+    // Two blocks of keys at a time, so that no product waits for the one before it.
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        half8_t kh[2], kl[2];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const int slot = key_slot<D>(16 * (i + w) + n16, 4 * st + g);
+          kh[w] = key_hi[slot];
+          kl[w] = key_lo[slot];
+        }
+        multiply<2>(kh, kl, [&](int x) -> const half8_t& { return q_hi[x][st]; },
+                    [&](int x) -> const half8_t& { return q_lo[x][st]; },
+                    [&](int x, int w) -> acc_t& { return s[x][i + w]; });
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4_t factor = *reinterpret_cast<const float4_t*>(&key_factor[16 * i + 4 * g]);
+      const float4_t add = *reinterpret_cast<const float4_t*>(&value_exp[16 * i + 4 * g]);
+#pragma unroll
+      for (int x = 0; x < kQ; ++x)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s[x][i][v] = fmaf(s[x][i][v], row_factor[x] * factor[v], add[v]);
+    }
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          // The oldest key in the window of key p is p - window + 1; sinks are in every one.
+          const int key = key_of(16 * i + 4 * g + v);
+          const int until = a.window == 0 || key < a.sinks ? 0x7fffffff : key + a.window;
+#pragma unroll
+          for (int x = 0; x < kQ; ++x) s[x][i][v] = key <= p_row[x] && until > p_row[x] ? s[x][i][v] : neg_inf;
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < kQ; ++x) {
+      float top = m[x];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) top = fmaxf(top, s[x][i][v]);
+      top = fmaxf(top, __shfl_xor(top, 16, kWave));
+      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      // Rescaled only where some row's maximum moved.
+      if (__any(top > m[x])) {
+        const float f = __builtin_amdgcn_exp2f(m[x] - (top == neg_inf ? 0.F : top));
+        l[x] *= f;
+#pragma unroll
+        for (int i = 0; i < kT; ++i) o[x][i] *= f;
+        m[x] = top;
+      }
+      const float at = m[x] == neg_inf ? 0.F : m[x] - 15.F;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4_t unit = *reinterpret_cast<const float4_t*>(&value_unit[16 * i + 4 * g]);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          s[x][i][v] = __builtin_amdgcn_exp2f(s[x][i][v] - at);
+          l[x] = fmaf(s[x][i][v], unit[v], l[x]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float w[8] = {s[x][2 * k][0],     s[x][2 * k][1],     s[x][2 * k][2],     s[x][2 * k][3],
+                            s[x][2 * k + 1][0], s[x][2 * k + 1][1], s[x][2 * k + 1][2], s[x][2 * k + 1][3]};
+        split_halves<8>(w, p_hi[x][k], p_lo[x][k]);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void outputs(const half8_t* value_hi, const half8_t* value_lo, const half8_t (&p_hi)[kQ][2],
+                                          const half8_t (&p_lo)[kQ][2]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < kT; i += 2) {
+        half8_t vh[2], vl[2];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const int slot = value_slot(16 * (i + w) + n16, 4 * k + g);
+          vh[w] = value_hi[slot];
+          vl[w] = value_lo[slot];
+        }
+        multiply<2>(vh, vl, [&](int x) -> const half8_t& { return p_hi[x][k]; },
+                    [&](int x) -> const half8_t& { return p_lo[x][k]; },
+                    [&](int x, int w) -> acc_t& { return o[x][i + w]; });
+      }
+  }
+
+  // sum(x, w) += (hi + lo)[w] (hi + lo)(x) without lo lo, term by term.
+  template <int kN, typename H, typename L, typename S>
+  __device__ __forceinline__ static void multiply(const half8_t (&hi)[kN], const half8_t (&lo)[kN], H&& b_hi, L&& b_lo,
+                                                  S&& sum) {
+#pragma unroll
+    for (int term = 0; term < 3; ++term)
+#pragma unroll
+      for (int w = 0; w < kN; ++w)
+#pragma unroll
+        for (int x = 0; x < kQ; ++x)
+          sum(x, w) = __builtin_amdgcn_mfma_f32_16x16x32_f16(term == 0 ? lo[w] : hi[w], term == 1 ? b_lo(x) : b_hi(x),
+                                                             sum(x, w), 0, 0, 0);
+  }
+
+  // The values that were taken out of a tile of `count` keys, for the rows that see them.
+  template <typename F>
+  __device__ __forceinline__ void add_bad(const DecodeArgs& a, const float* vb, int count, F&& key_of) {
+    for (int k = 0; k < count; ++k) {
+      const int key = key_of(k);
+      const float* row = vb + key * a.v_stride[2];
+#pragma unroll
+      for (int i = 0; i < kT; ++i)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int at = 16 * i + 4 * g + v, f = 4 * (at % kQuads) + at / kQuads;
+          const float value = f < a.features ? row[f] : 0.F;
+          if (magnitude(value) < 0x7f800000U) continue;
+#pragma unroll
+          for (int x = 0; x < kQ; ++x)
+            if (sees(p_row[x], key, a.window, a.sinks)) o[x][i][v] += value;
+        }
+    }
+  }
+
+  __device__ __forceinline__ void finish(const DecodeArgs& a, int b, int kv, int head, int split, int r1) {
+    const int total = a.rows * a.share;
+#pragma unroll
+    for (int x = 0; x < kQ; ++x) {
+      l[x] += __shfl_xor(l[x], 16, kWave);
+      l[x] += __shfl_xor(l[x], 32, kWave);
+      const int r = row0 + 16 * x + n16;
+      if (r > r1) continue;
+      const RowPlace place = row_place(a, kv, r);
+      const std::int64_t row = (static_cast<std::int64_t>(split) * a.batch * a.kv_heads + head) * total + r;
+      float* out = a.splits == 1
+                       ? a.out + b * a.out_stride[0] + place.head * a.out_stride[1] + place.query * a.out_stride[2]
+                       : a.part + row * a.features;
+      // 2^-13: the offset of value_exp.
+      const float by = a.splits > 1 ? 1.F / 8192.F : l[x] == 0.F ? 0.F : 1.F / 8192.F / l[x];
+      if constexpr (kQuads % 16 == 0) {
+        // Rows e D / 4 + c for e = 0..3 are features 4 c + e: one store of four.
+#pragma unroll
+        for (int i = 0; i < kT / 4; ++i)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int f = 4 * (16 * i + 4 * g + v);
+            if (f < a.features)
+              *reinterpret_cast<float4_t*>(out + f) = float4_t{o[x][i][v] * by, o[x][i + kT / 4][v] * by,
+                                                               o[x][i + kT / 2][v] * by, o[x][i + 3 * kT / 4][v] * by};
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kT; ++i)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int at = 16 * i + 4 * g + v, f = 4 * (at % kQuads) + at / kQuads;
+            if (f < a.features) out[f] = o[x][i][v] * by;
+          }
+      }
+      if (a.splits > 1 && g == 0) {
+        a.part_ml[2 * row] = m[x];
+        a.part_ml[2 * row + 1] = l[x];
+      }
+    }
+  }
+};
+
+template <int D, int kWaves, int kQ>
+__global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(DecodeArgs a, std::int64_t items, int row_tiles) {
+  constexpr int kThreads = 64 * kWaves, kRows = 16 * kQ * kWaves, kTile = 64;
+  constexpr int kKeyChunks = D / 8;  // of 8 features a key
+  constexpr int kKeyTasks = (kTile * kKeyChunks + kThreads - 1) / kThreads;
+  constexpr int kQuads = D / 4;      // of 4 features of a key's values
+  constexpr int kValueTasks = (kTile / 4 * kQuads + kThreads - 1) / kThreads;
+  __shared__ half8_t key_hi[8 * D], key_lo[8 * D], value_hi[8 * D], value_lo[8 * D];
+  __shared__ alignas(16) float key_factor[kTile];    // 2^-scale of a key
+  __shared__ alignas(16) float value_exp[2][kTile];  // e_j + 13, and 2 to the minus that
+  __shared__ alignas(16) float value_unit[2][kTile];
+  __shared__ int value_bad[2];                       // some value is not finite
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int total = a.rows * a.share;
+  for (std::int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int split = static_cast<int>(item % a.splits);
+    const std::int64_t rest = item / a.splits;
+    // The last tiles of a prompt see the most keys: they start first.
+    const int tile_of = row_tiles - 1 - static_cast<int>(rest % row_tiles), head = static_cast<int>(rest / row_tiles);
+    const int b = head / a.kv_heads, kv = head % a.kv_heads;
+    const int r0 = tile_of * kRows, r1 = min(r0 + kRows, total) - 1;
+    const int n = checked_length(a, b);
+    const SeenKeys seen = seen_keys(n, a.rows, r0 / a.share, r1 / a.share, a.window, a.sinks);
+    const int u0 = static_cast<int>(static_cast<std::int64_t>(seen.count()) * split / a.splits);
+    const int u1 = static_cast<int>(static_cast<std::int64_t>(seen.count()) * (split + 1) / a.splits);
+    const float* kb = static_cast<const float*>(a.k) + b * a.k_stride[0] + kv * a.k_stride[1];
+    const float* vb = static_cast<const float*>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
+
+    // Keys and values by turns.
+    constexpr int kStage = 2 * kKeyTasks > 4 * kValueTasks ? 2 * kKeyTasks : 4 * kValueTasks;
+    float4_t stage[kStage];
+    auto& key = reinterpret_cast<float4_t(&)[kKeyTasks][2]>(stage);
+    auto& value = reinterpret_cast<float4_t(&)[kValueTasks][4]>(stage);
+    int field[kValueTasks][4];
+    auto load_keys = [&](int u) {
+#pragma unroll
+      for (int i = 0; i < kKeyTasks; ++i) {
+        const int task = t + i * kThreads, j = task / kKeyChunks, f = 8 * (task % kKeyChunks);
+        const bool in = j < kTile && u + j < u1 && f < a.features;
+        const float* row = kb + seen.key(min(u + j, u1 - 1)) * a.k_stride[2] + (in ? f : 0);
+        key[i][0] = *reinterpret_cast<const float4_t*>(row);
+        key[i][1] = *reinterpret_cast<const float4_t*>(row + 4);
+        if (!in) key[i][0] = key[i][1] = float4_t{0.F, 0.F, 0.F, 0.F};
+      }
+    };
+    auto store_keys = [&] {
+#pragma unroll
+      for (int i = 0; i < kKeyTasks; ++i) {
+        const int task = t + i * kThreads;
+        pack_keys<D>(key[i], task / kKeyChunks, task % kKeyChunks, key_hi, key_lo, key_factor);
+      }
+    };
+    auto load_values = [&](int u) {
+#pragma unroll
+      for (int i = 0; i < kValueTasks; ++i) {
+        const int task = t + i * kThreads, f = 4 * (task % kQuads), h = task / kQuads;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int j = u + 4 * h + v;
+          const bool in = h < kTile / 4 && j < u1 && f < a.features;
+          const float* row = vb + seen.key(min(j, u1 - 1)) * a.v_stride[2] + (in ? f : 0);
+          value[i][v] = *reinterpret_cast<const float4_t*>(row);
+          if (!in) value[i][v] = float4_t{0.F, 0.F, 0.F, 0.F};
+        }
+      }
+    };
+    auto measure = [&](int buffer) {
+#pragma unroll
+      for (int i = 0; i < kValueTasks; ++i) {
+        const int task = t + i * kThreads;
+        measure_values<D>(value[i], task / kQuads, task % kQuads, field[i], value_exp[buffer], value_unit[buffer],
+                          &value_bad[buffer]);
+      }
+    };
+    auto store_values = [&] {
+#pragma unroll
+      for (int i = 0; i < kValueTasks; ++i) {
+        const int task = t + i * kThreads;
+        pack_values<D>(value[i], task / kQuads, task % kQuads, field[i], reinterpret_cast<half4_t*>(value_hi),
+                       reinterpret_cast<half4_t*>(value_lo));
+      }
+    };
+
+    PromptRows<D, kQ> rows;
+    if (t < 2) value_bad[t] = 0;
+    __syncthreads();
+    if (u0 < u1) load_keys(u0);
+    rows.start(a, b, kv, n, r0 + wave * kQ * 16, r1, lane);
+    if (u0 < u1) {
+      store_keys();
+      load_values(u0);
+      measure(0);
+    }
+    int buffer = 0;
+    for (int u = u0; u < u1; u += kTile, buffer ^= 1) {
+      const bool more = u + kTile < u1;
+      __syncthreads();  // A: this tile's keys and value powers are in LDS, the last tile's values are free
+      if (t == 0) value_bad[buffer ^ 1] = 0;  // the last tile's mark has been read
+      store_values();
+      if (more) load_keys(u + kTile);
+      // Which of the tile's keys the wave's rows see: the sinks in it by all; its
+      // part of the window runs from `from` to `last`.
+      const int last = seen.key(min(u + kTile, u1) - 1), from = u >= seen.sinks ? seen.key(u) : seen.first;
+      const bool with_window = last >= seen.first;
+      const bool any_seen = u < seen.sinks || (from <= rows.last_row && (a.window == 0 || last > rows.first_row - a.window ||
+                                                                         from < a.sinks));
+      const bool all_seen = u + kTile <= u1 &&
+                            (!with_window || (last <= rows.first_row && (a.window == 0 || from > rows.last_row - a.window)));
+      auto key_of = [&](int k) { return u + k < u1 ? seen.key(u + k) : 1 << 30; };
+      half8_t p_hi[kQ][2], p_lo[kQ][2];
+      if (any_seen)
+        rows.scores(a, key_hi, key_lo, key_factor, value_exp[buffer], value_unit[buffer], all_seen, key_of, p_hi, p_lo);
+      __syncthreads();  // B: this tile's values are in LDS, its keys are free
+      if (more) {
+        store_keys();
+        load_values(u + kTile);
+      }
+      if (any_seen) {
+        rows.outputs(value_hi, value_lo, p_hi, p_lo);
+        if (value_bad[buffer]) rows.add_bad(a, vb, min(kTile, u1 - u), key_of);
+      }
+      if (more) measure(buffer ^ 1);
+    }
+    rows.finish(a, b, kv, head, split, r1);
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ long prompts
+// Where many blocks see the same keys, splitting them into halves anew in each
+// costs more than the products (790 vector instructions a wave and tile, half of
+// them for that). A first kernel then writes each tile of 64 keys once, as the
+// block's buffers hold it, to the workspace, and prompt_tile_kernel takes the
+// tiles from there straight into LDS, two buffers and one barrier a tile.
+
+// A tile as it lies in the workspace and in LDS.
+template <int D>
+struct PromptTile {
+  half8_t key_hi[8 * D], key_lo[8 * D];
+  half8_t value_hi[8 * D], value_lo[8 * D];
+  float key_factor[64], value_exp[64], value_unit[64];
+  int bad;  // some value is not finite
+  int pad[15];
+};
+
+// The tiles that a call sees: those of its sinks, then the window's; tile i is
+// keys 64 i .. 64 i + 63.
+struct SeenTiles {
+  int sinks, first, end;  // tiles [0, sinks) and [first, end)
+  __host__ __device__ int count() const { return sinks + end - first; }
+  __device__ int tile(int i) const { return i < sinks ? i : i - sinks + first; }
+  __device__ int place(int tile) const { return tile < sinks ? tile : tile - first + sinks; }
+};
+__host__ __device__ inline SeenTiles seen_tiles(const SeenKeys& s) {
+  SeenTiles t;
+  t.sinks = (s.sinks + 63) / 64;
+  t.end = (s.end + 63) / 64;
+  t.first = s.first / 64 > t.sinks ? s.first / 64 : t.sinks;
+  if (t.first > t.end) t.first = t.end;
+  return t;
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void prompt_pack_kernel(DecodeArgs a, PromptTile<D>* tiles, int places) {
+  constexpr int kTile = 64, kThreads = 256;
+  constexpr int kKeyChunks = D / 8, kKeyTasks = (kTile * kKeyChunks + kThreads - 1) / kThreads;
+  constexpr int kQuads = D / 4, kValueTasks = (kTile / 4 * kQuads + kThreads - 1) / kThreads;
+  __shared__ PromptTile<D> out;
+  const int t = threadIdx.x, place = blockIdx.x;
+  const int heads = a.batch * a.kv_heads;
+  for (int head = blockIdx.y; head < heads; head += gridDim.y) {
+    const int b = head / a.kv_heads, kv = head % a.kv_heads;
+    const int n = checked_length(a, b);
+    const SeenTiles seen = seen_tiles(seen_keys(n, a.rows, 0, a.rows - 1, a.window, a.sinks));
+    if (place >= seen.count()) continue;  // the same for the whole block
+    const int j0 = 64 * seen.tile(place);
+    const float* kb = static_cast<const float*>(a.k) + b * a.k_stride[0] + kv * a.k_stride[1];
+    const float* vb = static_cast<const float*>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
+    if (t == 0) out.bad = 0;
+    float4_t key[kKeyTasks][2], value[kValueTasks][4];
+#pragma unroll
+    for (int i = 0; i < kKeyTasks; ++i) {
+      const int task = t + i * kThreads, j = task / kKeyChunks, f = 8 * (task % kKeyChunks);
+      const bool in = j0 + j < n && f < a.features;
+      const float* row = kb + (in ? j0 + j : 0) * a.k_stride[2] + (in ? f : 0);
+      key[i][0] = *reinterpret_cast<const float4_t*>(row);
+      key[i][1] = *reinterpret_cast<const float4_t*>(row + 4);
+      if (!in) key[i][0] = key[i][1] = float4_t{0.F, 0.F, 0.F, 0.F};
+    }
+#pragma unroll
+    for (int i = 0; i < kValueTasks; ++i) {
+      const int task = t + i * kThreads, f = 4 * (task % kQuads), h = task / kQuads;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int j = j0 + 4 * h + v;
+        const bool in = h < kTile / 4 && j < n && f < a.features;
+        const float* row = vb + (in ? j : 0) * a.v_stride[2] + (in ? f : 0);
+        value[i][v] = *reinterpret_cast<const float4_t*>(row);
+        if (!in) value[i][v] = float4_t{0.F, 0.F, 0.F, 0.F};
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kKeyTasks; ++i) {
+      const int task = t + i * kThreads;
+      pack_keys<D>(key[i], task / kKeyChunks, task % kKeyChunks, out.key_hi, out.key_lo, out.key_factor);
+    }
+#pragma unroll
+    for (int i = 0; i < kValueTasks; ++i) {
+      const int task = t + i * kThreads, h = task / kQuads;
+      int field[4];
+      measure_values<D>(value[i], h, task % kQuads, field, out.value_exp, out.value_unit, &out.bad);
+      pack_values<D>(value[i], h, task % kQuads, field, reinterpret_cast<half4_t*>(out.value_hi),
+                     reinterpret_cast<half4_t*>(out.value_lo));
+    }
+    __syncthreads();
+    auto* to = reinterpret_cast<float4_t*>(tiles + static_cast<std::int64_t>(head) * places + place);
+    const auto* from = reinterpret_cast<const float4_t*>(&out);
+    for (int i = t; i < static_cast<int>(sizeof(out) / 16); i += kThreads) to[i] = from[i];
+    __syncthreads();
+  }
+}
+
+// Copies `bytes` (a multiple of 16) from global memory into LDS, straight, 16 bytes a
+// lane: instruction p of wave w fills 1024 bytes from (p waves + w) 1024 on.
+template <int kWaves, int kBytes>
+__device__ __forceinline__ void copy_to_lds(const void* from, void* to, int wave, int lane) {
+  using int4v = int __attribute__((ext_vector_type(4)));
+  const auto address = reinterpret_cast<std::uint64_t>(from);
+  // The resource's size: reads past it give zeros.
+  const int4v rsrc{static_cast<int>(address), static_cast<int>(address >> 32), kBytes, 0x00020000};
+  const auto lds = static_cast<unsigned>(
+      reinterpret_cast<std::uintptr_t>((__attribute__((address_space(3))) void*)to));
+  constexpr int kInst = (kBytes + 1024 * kWaves - 1) / (1024 * kWaves);
+#pragma unroll
+  for (int p = 0; p < kInst; ++p) {
+    const int at = (p * kWaves + wave) * 1024;
+    if (at >= kBytes) continue;
+    // The last lanes of the last piece would write past the tile in LDS.
+    if (at + 1024 > kBytes && at + 16 * lane >= kBytes) continue;
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds + at),
+                 "v"(at + 16 * lane), "s"(rsrc)
+                 : "memory", "m0");
+#pragma clang diagnostic pop
+  }
+}
+
+template <int D, int kWaves, int kQ>
+__global__ __launch_bounds__(64 * kWaves, 2) void prompt_tile_kernel(DecodeArgs a, const PromptTile<D>* tiles, int places,
+                                                                     std::int64_t items, std::int64_t per_xcd,
+                                                                     int row_tiles) {
+  constexpr int kRows = 16 * kQ * kWaves;
+  extern __shared__ __align__(16) char shared[];
+  auto* stage = reinterpret_cast<PromptTile<D>*>(shared);  // two
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int total = a.rows * a.share;
+  for (std::int64_t block = blockIdx.x; block < 8 * per_xcd; block += gridDim.x) {
+    const std::int64_t item = block % 8 * per_xcd + block / 8;
+    if (item >= items) continue;
+    const int split = static_cast<int>(item % a.splits);
+    const std::int64_t rest = item / a.splits;
+    // The last tiles of a prompt see the most keys: they start first.
+    const int tile_of = row_tiles - 1 - static_cast<int>(rest % row_tiles), head = static_cast<int>(rest / row_tiles);
+    const int b = head / a.kv_heads, kv = head % a.kv_heads;
+    const int r0 = tile_of * kRows, r1 = min(r0 + kRows, total) - 1;
+    const int n = checked_length(a, b);
+    const SeenTiles all = seen_tiles(seen_keys(n, a.rows, 0, a.rows - 1, a.window, a.sinks));
+    const SeenTiles seen = seen_tiles(seen_keys(n, a.rows, r0 / a.share, r1 / a.share, a.window, a.sinks));
+    const PromptTile<D>* from = tiles + static_cast<std::int64_t>(head) * places;
+    const float* vb = static_cast<const float*>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
+    PromptRows<D, kQ> rows;
+    const int t0 = static_cast<int>(static_cast<std::int64_t>(seen.count()) * split / a.splits);
+    const int t1 = static_cast<int>(static_cast<std::int64_t>(seen.count()) * (split + 1) / a.splits);
+    auto copy = [&](int i) {
+      copy_to_lds<kWaves, static_cast<int>(sizeof(PromptTile<D>))>(from + all.place(seen.tile(i)), &stage[i & 1], wave, lane);
+    };
+    if (t0 < t1) copy(t0);
+    rows.start(a, b, kv, n, r0 + wave * kQ * 16, r1, lane);
+    for (int i = t0; i < t1; ++i) {
+      // This tile has landed, for every wave, and the other buffer is free.
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (i + 1 < t1) copy(i + 1);
+      const PromptTile<D>& now = stage[i & 1];
+      const int j0 = 64 * seen.tile(i);
+      if (!rows.any_seen(a, j0)) continue;
+      half8_t p_hi[kQ][2], p_lo[kQ][2];
+      rows.scores(a, now.key_hi, now.key_lo, now.key_factor, now.value_exp, now.value_unit, rows.all_seen(a, j0),
+                  [&](int k) { return j0 + k; }, p_hi, p_lo);
+      rows.outputs(now.value_hi, now.value_lo, p_hi, p_lo);
+      if (now.bad) rows.add_bad(a, vb, min(64, n - j0), [&](int k) { return j0 + k; });
+    }
+    rows.finish(a, b, kv, head, split, r1);
+    __syncthreads();  // both buffers are free again
+  }
+}
+
+}  // namespace tcx

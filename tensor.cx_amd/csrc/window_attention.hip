@@ -1,12 +1,13 @@
-// Attention with a sliding window and sinks over float32 keys and values, and
-// what the attentions of a decoding loop share on the host: checked arguments,
-// key splits and their join.
+// Attention with a sliding window and sinks over float32 keys and values, the
+// choice of its kernels, and what the attentions of a decoding loop share on
+// the host: checked arguments, key splits and their join.
 
 #include <algorithm>
 #include <cmath>
 #include <limits>
 
 #include "decode_stream.hpp"
+#include "prompt_attention.hpp"
 
 namespace tcx {
 namespace {
@@ -181,10 +182,113 @@ int join_splits(const DecodeArgs& a, hipStream_t s) {
 
 namespace {
 
-int window_splits(const DecodeArgs& a, std::size_t workspace_bytes) {
-  const int rows = stream_rows(a);
-  const std::int64_t blocks = static_cast<std::int64_t>(a.batch) * a.kv_heads * ((a.rows * a.share + rows - 1) / rows);
-  return plan_splits(a, blocks, 128, workspace_bytes);
+// How a call runs.
+struct WindowForm {
+  bool prompt;      // on matrix instructions: `waves` waves of 16 `each` rows
+  bool packed;      // from tiles that a first kernel writes to the workspace
+  int waves, each, rows;
+  int splits;
+  std::size_t tiles, bytes;  // of the packed tiles, and of the whole workspace
+};
+
+// Tiles of 64 keys that the rows of a head see, at most.
+std::int64_t most_tiles(const DecodeArgs& a) {
+  const std::int64_t all = (std::int64_t{a.cols} + 63) / 64;
+  if (a.window == 0) return all;
+  return std::min(all, (std::int64_t{a.sinks} + 63) / 64 + (std::int64_t{a.window} + a.rows + 62) / 64 + 1);
+}
+
+std::size_t tile_bytes(const DecodeArgs& a) {
+  return a.features <= 32 ? sizeof(PromptTile<32>) : a.features <= 64 ? sizeof(PromptTile<64>) : sizeof(PromptTile<128>);
+}
+
+// Which kernel, for `total` rows of `heads` key heads:
+// * fewer than 16 rows stream the keys past them;
+// * from 16 rows on, matrix instructions, in blocks of 64 rows that pack what
+//   they see for themselves (prompt_attention_kernel);
+// * where a tile of keys would be packed by four blocks and more of a full GPU, or
+//   by sixteen, it is packed once instead (prompt_pack_kernel and
+//   prompt_tile_kernel): 8 sequences of 64 rows, 32 heads on 8 of 64 features and
+//   512 keys 35.5 -> 27.3 us, a prompt of 2048 86 -> 59; 2 sequences of 64 rows,
+//   16 heads on 4 of 128 features and 8192 keys 90 -> 98 the other way;
+// * in blocks of 128 rows where those are at least 256, one a CU (2048 rows, 16
+//   heads on 4 of 128 features: 137 -> 107 us; 8 heads of their own, 128 blocks:
+//   90 -> 103 the other way), and of 256 where those are, heads have more than 64
+//   features and a window leaves the blocks alike (4096 rows, window 1024: 139 ->
+//   119 us; a causal prompt without a window 163 -> 173 the other way).
+WindowForm window_form(const DecodeArgs& a, std::size_t workspace_bytes) {
+  const int total = a.rows * a.share;
+  const std::int64_t heads = static_cast<std::int64_t>(a.batch) * a.kv_heads;
+  const auto blocks = [&](int rows) { return heads * ((total + rows - 1) / rows); };
+  WindowForm f{};
+  f.splits = 1;
+  if (total < 16) {
+    f.rows = stream_rows(a);
+  } else {
+    f.prompt = true;
+    f.waves = 4;
+    f.each = 1;
+    const std::size_t tiles = static_cast<std::size_t>(heads * most_tiles(a)) * tile_bytes(a);
+    if ((total >= 1024 || (total >= 256 && blocks(64) >= 256)) && tiles <= workspace_bytes) {
+      f.packed = true;
+      f.tiles = tiles;
+      if (blocks(128) >= 256) f.waves = 8;
+      if (a.features > 64 && a.window > 0 && blocks(256) >= 256) f.each = 2;
+    }
+    f.rows = 16 * f.waves * f.each;
+  }
+  // A CU holds four blocks that stream, two of four waves with tiles in LDS and
+  // one of eight. Packed tiles are split only where a part keeps 512 keys (512
+  // rows, 16 heads on 4, 512 keys: 34 us whole, 40 in four parts).
+  f.splits = plan_splits(a, (f.prompt ? f.waves / 2 : 1) * blocks(f.rows), f.packed ? 512 : 128, workspace_bytes - f.tiles);
+  f.bytes = f.tiles + split_bytes(a, f.splits);
+  return f;
+}
+
+template <int D>
+int launch_packed(const DecodeArgs& a, const WindowForm& form, void* workspace, hipStream_t s) {
+  auto* tiles = static_cast<PromptTile<D>*>(workspace);
+  const int places = static_cast<int>(most_tiles(a)), row_tiles = (a.rows * a.share + form.rows - 1) / form.rows;
+  const std::int64_t heads = static_cast<std::int64_t>(a.batch) * a.kv_heads, items = heads * row_tiles * a.splits;
+  if (places > 0) {
+    const unsigned y = static_cast<unsigned>(std::min<std::int64_t>(heads, 65535));
+    hipLaunchKernelGGL(prompt_pack_kernel<D>, dim3(places, y), dim3(256), 0, s, a, tiles, places);
+    if (int rc = check(hipGetLastError(), "attention pack launch"); rc != TCX_OK) return rc;
+  }
+  auto go = [&](auto kernel) -> int {
+    constexpr std::size_t kShared = 2 * sizeof(PromptTile<D>);
+    if constexpr (kShared > 65536) {
+      if (int rc = check(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, kShared),
+                         "attention shared memory");
+          rc != TCX_OK)
+        return rc;
+    }
+    const std::int64_t per_xcd = (items + 7) / 8;
+    hipLaunchKernelGGL(kernel, dim3(grid_for(8 * per_xcd, 1, 1 << 22)), dim3(64 * form.waves), kShared, s, a, tiles, places,
+                       items, per_xcd, row_tiles);
+    return check(hipGetLastError(), "attention launch");
+  };
+  if constexpr (D == 128)
+    if (form.each == 2) return go(prompt_tile_kernel<D, 8, 2>);
+  return form.waves == 8 ? go(prompt_tile_kernel<D, 8, 1>) : go(prompt_tile_kernel<D, 4, 1>);
+}
+
+template <int D>
+int launch_prompt(const DecodeArgs& a, const WindowForm& form, hipStream_t s) {
+  const int tiles = (a.rows * a.share + form.rows - 1) / form.rows;
+  const std::int64_t items = static_cast<std::int64_t>(a.batch) * a.kv_heads * tiles * a.splits;
+  hipLaunchKernelGGL((prompt_attention_kernel<D, 4, 1>), dim3(grid_for(items, 1, 1 << 22)), dim3(256), 0, s, a, items, tiles);
+  return check(hipGetLastError(), "attention launch");
+}
+
+template <int D>
+int launch_window(DecodeArgs& a, const WindowForm& form, void* workspace, hipStream_t s) {
+  place_split(a, form.splits, static_cast<char*>(workspace) + form.tiles);
+  const int rc = form.packed   ? launch_packed<D>(a, form, workspace, s)
+                 : form.prompt ? launch_prompt<D>(a, form, s)
+                               : launch_stream<FloatRows<D>>(a, s);
+  return rc == TCX_OK && a.splits > 1 ? join_splits(a, s) : rc;
 }
 
 }  // namespace
@@ -203,7 +307,7 @@ size_t tcx_hip_window_attention_workspace_bytes(const tcx_hip_window_attention_d
   // Any aligned address passes for the buffers, which are not touched.
   alignas(16) static float any[4];
   if (decode_args(any, any, any, any, desc, false, a, done) != TCX_OK || done) return 0;
-  return split_bytes(a, window_splits(a, SIZE_MAX));
+  return window_form(a, SIZE_MAX).bytes;
 }
 
 int tcx_hip_window_attention_f32(const float* q, const float* k, const float* v, float* out,
@@ -217,12 +321,10 @@ int tcx_hip_window_attention_f32(const float* q, const float* k, const float* v,
     return fail(TCX_INVALID_ARGUMENT, "attention workspace must be 16-byte aligned");
   if (int rc = ready(); rc != TCX_OK) return rc;
   const auto s = static_cast<hipStream_t>(stream);
-  place_split(a, window_splits(a, workspace != nullptr ? workspace_bytes : 0), workspace);
-  int rc = a.features <= 32 ? launch_stream<FloatRows<32>>(a, s)
-           : a.features <= 64 ? launch_stream<FloatRows<64>>(a, s)
-                              : launch_stream<FloatRows<128>>(a, s);
-  if (rc == TCX_OK && a.splits > 1) rc = join_splits(a, s);
-  return rc;
+  const WindowForm form = window_form(a, workspace != nullptr ? workspace_bytes : 0);
+  if (a.features <= 32) return launch_window<32>(a, form, workspace, s);
+  if (a.features <= 64) return launch_window<64>(a, form, workspace, s);
+  return launch_window<128>(a, form, workspace, s);
 }
 
 }  // extern "C"

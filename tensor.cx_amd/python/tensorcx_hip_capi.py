@@ -425,10 +425,15 @@ def window_attention_desc(batch, heads, kv_heads, rows, cols, features, *, windo
     return d
 
 
-def window_attention_workspace(desc: WindowAttentionDesc, cache: bool = False) -> DeviceBuffer | None:
-    """The workspace that window_attention (cache4_attention with `cache`) can use (None when it needs none)."""
+def window_attention_workspace_bytes(desc: WindowAttentionDesc, cache: bool = False) -> int:
+    """Bytes of workspace that window_attention (cache4_attention with `cache`) can use."""
     query = lib().tcx_hip_cache4_attention_workspace_bytes if cache else lib().tcx_hip_window_attention_workspace_bytes
-    nbytes = query(ctypes.byref(desc))
+    return query(ctypes.byref(desc))
+
+
+def window_attention_workspace(desc: WindowAttentionDesc, cache: bool = False) -> DeviceBuffer | None:
+    """A workspace of that size (None when none is of use)."""
+    nbytes = window_attention_workspace_bytes(desc, cache)
     return DeviceBuffer(nbytes) if nbytes else None
 
 
@@ -465,8 +470,12 @@ def cache4_attention(q: int, key_cache: int, value_cache: int, out: int, desc: W
                                              _on(s)), "cache4_attention")
 
 
+def beam_select_workspace_bytes(batch: int, beams: int, vocabulary: int, count: int) -> int:
+    return lib().tcx_hip_beam_select_workspace_bytes(batch, beams, vocabulary, count)
+
+
 def beam_select_workspace(batch: int, beams: int, vocabulary: int, count: int) -> DeviceBuffer | None:
-    nbytes = lib().tcx_hip_beam_select_workspace_bytes(batch, beams, vocabulary, count)
+    nbytes = beam_select_workspace_bytes(batch, beams, vocabulary, count)
     return DeviceBuffer(nbytes) if nbytes else None
 
 
