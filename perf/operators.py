@@ -322,9 +322,15 @@ def _own(state):
     kind, stream = case["kind"], torch.cuda.current_stream().cuda_stream
     if not plan:  # what the program keeps from call to call
         capi = plan["capi"] = _capi()
-        plan["workspace"] = capi.Workspace(state["scratch"].data_ptr(), state["scratch"].numel())
+        wanted = 0  # the scratch buffer, or one of the size that the library asks for where that is more
         if kind in ("window", "cache", "step"):
             plan["desc"] = _attention_plan(capi, case, t, state)
+            wanted = capi.window_attention_workspace_bytes(plan["desc"], cache=kind != "window")
+        elif kind == "select":
+            wanted = capi.beam_select_workspace_bytes(case["batch"], case["beams"], case["vocabulary"], case["count"])
+        plan["scratch"] = state["scratch"] if wanted <= state["scratch"].numel() else torch.empty(
+            wanted, dtype=torch.uint8, device="cuda")
+        plan["workspace"] = capi.Workspace(plan["scratch"].data_ptr(), plan["scratch"].numel())
         if kind in ("store", "step"):
             plan["store"] = _store_plan(capi, case)
         if kind == "reorder":
