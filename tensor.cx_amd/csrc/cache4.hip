@@ -13,7 +13,7 @@
 
 #include <algorithm>
 
-#include "decode_stream.hpp"
+#include "cache4_attention.hpp"
 
 namespace tcx {
 namespace {
@@ -52,35 +52,6 @@ template <typename V>
 __device__ __forceinline__ std::uint32_t scale_word(const V& v, int g) {
   return v[g];
 }
-
-template <int D>
-struct CacheRows {
-  using Row = CacheRow<D>;
-  static constexpr int kFeatures = D / 16;
-  struct Raw {
-    std::uint32_t codes;
-    typename Row::Scales scales;
-  };
-  static __device__ __forceinline__ int feature(int li, int e) { return 16 * e + li; }
-  std::int64_t k_base, v_base;
-  int li;
-  __device__ CacheRows(const DecodeArgs& a, int b, int kv, int lane)
-      : k_base(b * a.k_stride[0] + kv * a.k_stride[1]), v_base(b * a.v_stride[0] + kv * a.v_stride[1]), li(lane) {}
-  __device__ __forceinline__ void load(const void* p, std::int64_t base, std::int64_t stride, std::int64_t key,
-                                       Raw& raw) const {
-    const std::int32_t* row = static_cast<const std::int32_t*>(p) + base + key * stride;
-    raw.codes = reinterpret_cast<const typename Row::Codes*>(row)[li];
-    raw.scales = *reinterpret_cast<const typename Row::Scales*>(row + D / 8);
-  }
-  __device__ __forceinline__ void values(const Raw& raw, float (&x)[kFeatures]) const {
-#pragma unroll
-    for (int e = 0; e < kFeatures; ++e) {
-      const std::uint32_t word = scale_word(raw.scales, e / 2);
-      const float low = __uint_as_float(word & 0xffff0000U), step = __uint_as_float(word << 16);
-      x[e] = fmaf(step, static_cast<float>((raw.codes >> (4 * e)) & 15U), low);
-    }
-  }
-};
 
 // The largest (or smallest) of sixteen lanes' values, in all of them.
 template <bool kLargest>
@@ -180,10 +151,30 @@ __global__ __launch_bounds__(256) void cache_load_kernel(const std::int32_t* __r
 
 bool aligned16(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15U) == 0; }
 
+// Rows of a block: 4 where a head has no more, else 16 (cache_attention_kernel:
+// 16 sequences of 4096 to 8192 tokens, 8 heads of 128 features, one row each 45.4
+// -> 37.5 us, four 46.3 -> 39.9).
+int cache_rows(const DecodeArgs& a) { return a.rows * a.share <= 4 ? 4 : 16; }
+
+// 768 blocks fill the GPU three to a CU (512 and 1024: 39.9 and 42.1 us against
+// 37.9), and a split of fewer than 256 keys costs more than it spares.
 int cache_splits(const DecodeArgs& a, std::size_t workspace_bytes) {
-  const int rows = stream_rows(a);
+  const int rows = cache_rows(a);
   const std::int64_t blocks = static_cast<std::int64_t>(a.batch) * a.kv_heads * ((a.rows * a.share + rows - 1) / rows);
-  return plan_splits(a, blocks, 128, workspace_bytes);
+  return plan_splits(a, blocks, 768, 256, workspace_bytes);
+}
+
+template <int D, int kRows>
+int launch_cache(const DecodeArgs& a, hipStream_t s) {
+  const int tiles = (a.rows * a.share + kRows - 1) / kRows;
+  std::uint32_t items;
+  if (int rc = count_items(a, tiles, items); rc != TCX_OK) return rc;
+  hipLaunchKernelGGL((cache_attention_kernel<D, kRows>), dim3(grid_for(items, 1, 1 << 22)), dim3(256), 0, s, a, items, tiles);
+  return check(hipGetLastError(), "cache attention launch");
+}
+template <int D>
+int launch_cache(const DecodeArgs& a, hipStream_t s) {
+  return cache_rows(a) == 4 ? launch_cache<D, 4>(a, s) : launch_cache<D, 16>(a, s);
 }
 
 }  // namespace
@@ -287,9 +278,7 @@ int tcx_hip_cache4_attention_f32(const float* q, const int32_t* key_cache, const
   if (int rc = ready(); rc != TCX_OK) return rc;
   const auto s = static_cast<hipStream_t>(stream);
   place_split(a, cache_splits(a, workspace != nullptr ? workspace_bytes : 0), workspace);
-  int rc = a.features == 32 ? launch_stream<CacheRows<32>>(a, s)
-           : a.features == 64 ? launch_stream<CacheRows<64>>(a, s)
-                              : launch_stream<CacheRows<128>>(a, s);
+  int rc = a.features == 32 ? launch_cache<32>(a, s) : a.features == 64 ? launch_cache<64>(a, s) : launch_cache<128>(a, s);
   if (rc == TCX_OK && a.splits > 1) rc = join_splits(a, s);
   return rc;
 }

@@ -14,7 +14,7 @@
 namespace tcx {
 
 template <class Source, int kRows, int kEach>
-__global__ __launch_bounds__(256) void stream_attention_kernel(DecodeArgs a, std::int64_t items, int row_tiles) {
+__global__ __launch_bounds__(256) void stream_attention_kernel(DecodeArgs a, std::uint32_t items, int row_tiles) {
   constexpr int kF = Source::kFeatures, D = 16 * kF;
   constexpr float kLog2e = 1.44269502F;
   __shared__ float part_o[4][kRows][D];
@@ -22,17 +22,13 @@ __global__ __launch_bounds__(256) void stream_attention_kernel(DecodeArgs a, std
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, li = lane & 15, group = t >> 4;
   const float neg_inf = -__builtin_inff();
   const int total = a.rows * a.share;
-  for (std::int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int split = static_cast<int>(item % a.splits);
-    const std::int64_t rest = item / a.splits;
-    const int tile = static_cast<int>(rest % row_tiles), head = static_cast<int>(rest / row_tiles);
-    const int b = head / a.kv_heads, kv = head % a.kv_heads;
+  for (std::uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const auto [split, tile, head, b, kv] = block_work(a, item, row_tiles);
     const int r0 = tile * kRows, r1 = min(r0 + kRows, total) - 1;
     const int n = checked_length(a, b);
-    const int i0 = r0 / a.share, i1 = r1 / a.share;
+    const int i0 = row_query(a, r0), i1 = row_query(a, r1);
     const SeenKeys seen = seen_keys(n, a.rows, i0, i1, a.window, a.sinks);
-    const int u0 = static_cast<int>(static_cast<std::int64_t>(seen.count()) * split / a.splits);
-    const int u1 = static_cast<int>(static_cast<std::int64_t>(seen.count()) * (split + 1) / a.splits);
+    const int u0 = split_start(a, seen.count(), split), u1 = split_start(a, seen.count(), split + 1);
 
     float q[kRows][kF], o[kRows][kF], m[kRows], l[kRows];
     int p_row[kRows];
@@ -177,7 +173,8 @@ inline int stream_rows(const DecodeArgs& a) {
 template <class Source>
 int launch_stream(const DecodeArgs& a, hipStream_t s) {
   const int rows = stream_rows(a), tiles = (a.rows * a.share + rows - 1) / rows;
-  const std::int64_t items = static_cast<std::int64_t>(a.batch) * a.kv_heads * tiles * a.splits;
+  std::uint32_t items;
+  if (int rc = count_items(a, tiles, items); rc != TCX_OK) return rc;
   const unsigned grid = grid_for(items, 1, 1 << 22);
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, a, items, tiles); };
   if (rows == 1) go(stream_attention_kernel<Source, 1, 4>);

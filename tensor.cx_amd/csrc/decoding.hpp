@@ -63,20 +63,54 @@ int decode_args(const float* q, const void* k, const void* v, float* out, const 
 std::size_t split_bytes(const DecodeArgs& a, int splits);
 // Places part and part_ml in the workspace.
 void place_split(DecodeArgs& a, int splits, void* workspace);
-// How many splits a call of `blocks` blocks takes, of at least split_keys keys
-// each and with no more bytes than the workspace has.
-int plan_splits(const DecodeArgs& a, std::int64_t blocks, int split_keys, std::size_t workspace_bytes);
+// How many splits a call of `blocks` blocks takes to come to `wanted` of them, with
+// at least split_keys keys in each and no more bytes than the workspace has.
+int plan_splits(const DecodeArgs& a, std::int64_t blocks, int wanted, int split_keys, std::size_t workspace_bytes);
+// The blocks' work items of a call of `row_tiles` row tiles a head, as a 32-bit
+// count; TCX_INVALID_ARGUMENT where there are more.
+int count_items(const DecodeArgs& a, std::int64_t row_tiles, std::uint32_t& items);
 // Joins the splits into out.
 int join_splits(const DecodeArgs& a, hipStream_t s);
 
-// The keys of sequence b, its length checked.
+// The keys of sequence b (the same for the whole wave), its length checked; in a
+// scalar register, and what follows from it too.
 __device__ __forceinline__ int checked_length(const DecodeArgs& a, int b) {
   if (a.lengths == nullptr) return a.cols;
-  const int n = a.lengths[b];
+  const int n = __builtin_amdgcn_readfirstlane(a.lengths[b]);
   if (n >= 0 && n <= a.cols) return n;
   if (a.flag != nullptr) __hip_atomic_store(a.flag, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
   return n < 0 ? 0 : a.cols;
 }
+
+// What a block does: a split of the keys of row tile `tile` of key head `head` of
+// all. Divisions run on vector registers even where their operands are the same
+// for the whole wave; the results go back to scalar ones, and with them whatever
+// is computed from them (buffer resources most of all, which take a loop over
+// the lanes otherwise).
+struct BlockWork {
+  int split, tile, head, b, kv;
+};
+__device__ __forceinline__ BlockWork block_work(const DecodeArgs& a, std::uint32_t item, int row_tiles) {
+  const std::uint32_t rest = item / static_cast<std::uint32_t>(a.splits), head = rest / static_cast<std::uint32_t>(row_tiles);
+  BlockWork w;
+  w.split = __builtin_amdgcn_readfirstlane(static_cast<int>(item - rest * a.splits));
+  w.tile = __builtin_amdgcn_readfirstlane(static_cast<int>(rest - head * row_tiles));
+  w.head = __builtin_amdgcn_readfirstlane(static_cast<int>(head));
+  w.b = __builtin_amdgcn_readfirstlane(w.head / a.kv_heads);
+  w.kv = w.head - w.b * a.kv_heads;
+  return w;
+}
+// The first of the `count` keys (or tiles of them) that falls to split s: equal
+// shares (a fixed number of keys to each split, which leaves the last ones of
+// short sequences empty, was slower: 44 us against 38 for 16 sequences of 4096 to
+// 8192 tokens).
+__device__ __forceinline__ int split_start(const DecodeArgs& a, int count, int s) {
+  if (a.splits == 1) return s == 0 ? 0 : count;
+  const int each = __builtin_amdgcn_readfirstlane(count / a.splits);
+  return each * s + min(s, count - each * a.splits);
+}
+// The query of row r.
+__device__ __forceinline__ int row_query(const DecodeArgs& a, int r) { return __builtin_amdgcn_readfirstlane(r / a.share); }
 
 // Row r of a head's rows: query r / share of query head kv * share + r % share,
 // so that neighbouring rows see the same keys.

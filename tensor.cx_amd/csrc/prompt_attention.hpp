@@ -36,53 +36,10 @@
 #pragma once
 
 #include "decoding.hpp"
+#include "halves.hpp"
 
 namespace tcx {
 
-using half2_t = _Float16 __attribute__((ext_vector_type(2)));
-using half4_t = _Float16 __attribute__((ext_vector_type(4)));
-using half8_t = _Float16 __attribute__((ext_vector_type(8)));
-using float2v_t = float __attribute__((ext_vector_type(2)));
-using acc_t = float __attribute__((ext_vector_type(4)));
-
-// hi and lo halves of N scaled numbers.
-template <int N, typename H>
-__device__ __forceinline__ void split_halves(const float (&x)[N], H& hi, H& lo) {
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const half2_t h = __builtin_convertvector((float2v_t{x[i], x[i + 1]}), half2_t);
-    const half2_t l = __builtin_convertvector(
-        (float2v_t{x[i] - static_cast<float>(h[0]), x[i + 1] - static_cast<float>(h[1])}), half2_t);
-    hi[i] = h[0];
-    hi[i + 1] = h[1];
-    lo[i] = l[0];
-    lo[i + 1] = l[1];
-  }
-}
-
-__device__ __forceinline__ std::uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffU; }
-
-// The largest of kLanes neighbouring lanes' words, in all of them.
-template <int kLanes>
-__device__ __forceinline__ std::uint32_t lanes_most(std::uint32_t x) {
-  auto with = [&]<int kControl>() {
-    x = max(x, static_cast<std::uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), kControl, 0xf, 0xf, true)));
-  };
-  with.template operator()<0xb1>();
-  with.template operator()<0x4e>();
-  if constexpr (kLanes >= 8) with.template operator()<0x141>();
-  if constexpr (kLanes >= 16) with.template operator()<0x140>();
-  if constexpr (kLanes >= 32)
-    x = max(x, static_cast<std::uint32_t>(__builtin_amdgcn_ds_swizzle(static_cast<int>(x), 0x401f)));
-  return x;
-}
-
-// The exponent field of the power of two that brings a magnitude into [2^14,
-// 2^15), at most `most`.
-__device__ __forceinline__ int scale_field(std::uint32_t magnitude_bits, int most) {
-  return min(268 - static_cast<int>(magnitude_bits >> 23), most);
-}
-__device__ __forceinline__ float power_field(int field) { return __int_as_float(field << 23); }
 constexpr int kMostKeyField = 253;   // its inverse is a normal number
 constexpr int kMostValueField = 217; // 2^90: a sum of 2^20 weights stays finite
 
@@ -186,8 +143,8 @@ struct PromptRows {
     row0 = r0;
     n16 = lane & 15;
     g = lane >> 4;
-    first_row = n - a.rows + min(r0, r1) / a.share;
-    last_row = n - a.rows + min(r0 + kQ * 16 - 1, r1) / a.share;
+    first_row = n - a.rows + row_query(a, min(r0, r1));
+    last_row = n - a.rows + row_query(a, min(r0 + kQ * 16 - 1, r1));
 #pragma unroll
     for (int x = 0; x < kQ; ++x) {
       const RowPlace at = row_place(a, kv, min(r0 + 16 * x + n16, r1));
@@ -207,8 +164,7 @@ struct PromptRows {
             most = max(most, magnitude(w[e]));
           }
         }
-      most = max(most, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(most), 16, kWave)));
-      most = max(most, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(most), 32, kWave)));
+      most = across_max(most);
       const int field = scale_field(most, kMostKeyField);
       row_factor[x] = power_field(254 - field) * (a.scale * kLog2e);
 #pragma unroll
@@ -288,8 +244,7 @@ struct PromptRows {
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int v = 0; v < 4; ++v) top = fmaxf(top, s[x][i][v]);
-      top = fmaxf(top, __shfl_xor(top, 16, kWave));
-      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      top = across_max(top);
       // Rescaled only where some row's maximum moved.
       if (__any(top > m[x])) {
         const float f = __builtin_amdgcn_exp2f(m[x] - (top == neg_inf ? 0.F : top));
@@ -374,8 +329,7 @@ struct PromptRows {
     const int total = a.rows * a.share;
 #pragma unroll
     for (int x = 0; x < kQ; ++x) {
-      l[x] += __shfl_xor(l[x], 16, kWave);
-      l[x] += __shfl_xor(l[x], 32, kWave);
+      l[x] = across_sum(l[x]);
       const int r = row0 + 16 * x + n16;
       if (r > r1) continue;
       const RowPlace place = row_place(a, kv, r);
@@ -414,7 +368,7 @@ struct PromptRows {
 };
 
 template <int D, int kWaves, int kQ>
-__global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(DecodeArgs a, std::int64_t items, int row_tiles) {
+__global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(DecodeArgs a, std::uint32_t items, int row_tiles) {
   constexpr int kThreads = 64 * kWaves, kRows = 16 * kQ * kWaves, kTile = 64;
   constexpr int kKeyChunks = D / 8;  // of 8 features a key
   constexpr int kKeyTasks = (kTile * kKeyChunks + kThreads - 1) / kThreads;
@@ -427,17 +381,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Decode
   __shared__ int value_bad[2];                       // some value is not finite
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int total = a.rows * a.share;
-  for (std::int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int split = static_cast<int>(item % a.splits);
-    const std::int64_t rest = item / a.splits;
+  for (std::uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const auto [split, from_end, head, b, kv] = block_work(a, item, row_tiles);
     // The last tiles of a prompt see the most keys: they start first.
-    const int tile_of = row_tiles - 1 - static_cast<int>(rest % row_tiles), head = static_cast<int>(rest / row_tiles);
-    const int b = head / a.kv_heads, kv = head % a.kv_heads;
-    const int r0 = tile_of * kRows, r1 = min(r0 + kRows, total) - 1;
+    const int r0 = (row_tiles - 1 - from_end) * kRows, r1 = min(r0 + kRows, total) - 1;
     const int n = checked_length(a, b);
-    const SeenKeys seen = seen_keys(n, a.rows, r0 / a.share, r1 / a.share, a.window, a.sinks);
-    const int u0 = static_cast<int>(static_cast<std::int64_t>(seen.count()) * split / a.splits);
-    const int u1 = static_cast<int>(static_cast<std::int64_t>(seen.count()) * (split + 1) / a.splits);
+    const SeenKeys seen = seen_keys(n, a.rows, row_query(a, r0), row_query(a, r1), a.window, a.sinks);
+    const int u0 = split_start(a, seen.count(), split), u1 = split_start(a, seen.count(), split + 1);
     const float* kb = static_cast<const float*>(a.k) + b * a.k_stride[0] + kv * a.k_stride[1];
     const float* vb = static_cast<const float*>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
 
@@ -584,7 +534,7 @@ __global__ __launch_bounds__(256) void prompt_pack_kernel(DecodeArgs a, PromptTi
   const int t = threadIdx.x, place = blockIdx.x;
   const int heads = a.batch * a.kv_heads;
   for (int head = blockIdx.y; head < heads; head += gridDim.y) {
-    const int b = head / a.kv_heads, kv = head % a.kv_heads;
+    const int b = __builtin_amdgcn_readfirstlane(head / a.kv_heads), kv = head - b * a.kv_heads;
     const int n = checked_length(a, b);
     const SeenTiles seen = seen_tiles(seen_keys(n, a.rows, 0, a.rows - 1, a.window, a.sinks));
     if (place >= seen.count()) continue;  // the same for the whole block
@@ -664,30 +614,26 @@ __device__ __forceinline__ void copy_to_lds(const void* from, void* to, int wave
 
 template <int D, int kWaves, int kQ>
 __global__ __launch_bounds__(64 * kWaves, 2) void prompt_tile_kernel(DecodeArgs a, const PromptTile<D>* tiles, int places,
-                                                                     std::int64_t items, std::int64_t per_xcd,
+                                                                     std::uint32_t items, std::uint32_t per_xcd,
                                                                      int row_tiles) {
   constexpr int kRows = 16 * kQ * kWaves;
   extern __shared__ __align__(16) char shared[];
   auto* stage = reinterpret_cast<PromptTile<D>*>(shared);  // two
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int total = a.rows * a.share;
-  for (std::int64_t block = blockIdx.x; block < 8 * per_xcd; block += gridDim.x) {
-    const std::int64_t item = block % 8 * per_xcd + block / 8;
+  for (std::uint32_t block = blockIdx.x; block < 8 * per_xcd; block += gridDim.x) {
+    const std::uint32_t item = block % 8 * per_xcd + block / 8;
     if (item >= items) continue;
-    const int split = static_cast<int>(item % a.splits);
-    const std::int64_t rest = item / a.splits;
+    const auto [split, from_end, head, b, kv] = block_work(a, item, row_tiles);
     // The last tiles of a prompt see the most keys: they start first.
-    const int tile_of = row_tiles - 1 - static_cast<int>(rest % row_tiles), head = static_cast<int>(rest / row_tiles);
-    const int b = head / a.kv_heads, kv = head % a.kv_heads;
-    const int r0 = tile_of * kRows, r1 = min(r0 + kRows, total) - 1;
+    const int r0 = (row_tiles - 1 - from_end) * kRows, r1 = min(r0 + kRows, total) - 1;
     const int n = checked_length(a, b);
     const SeenTiles all = seen_tiles(seen_keys(n, a.rows, 0, a.rows - 1, a.window, a.sinks));
-    const SeenTiles seen = seen_tiles(seen_keys(n, a.rows, r0 / a.share, r1 / a.share, a.window, a.sinks));
+    const SeenTiles seen = seen_tiles(seen_keys(n, a.rows, row_query(a, r0), row_query(a, r1), a.window, a.sinks));
     const PromptTile<D>* from = tiles + static_cast<std::int64_t>(head) * places;
     const float* vb = static_cast<const float*>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
     PromptRows<D, kQ> rows;
-    const int t0 = static_cast<int>(static_cast<std::int64_t>(seen.count()) * split / a.splits);
-    const int t1 = static_cast<int>(static_cast<std::int64_t>(seen.count()) * (split + 1) / a.splits);
+    const int t0 = split_start(a, seen.count(), split), t1 = split_start(a, seen.count(), split + 1);
     auto copy = [&](int i) {
       copy_to_lds<kWaves, static_cast<int>(sizeof(PromptTile<D>))>(from + all.place(seen.tile(i)), &stage[i & 1], wave, lane);
     };

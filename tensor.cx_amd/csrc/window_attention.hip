@@ -63,11 +63,24 @@ __global__ __launch_bounds__(256) void join_splits_kernel(DecodeArgs a, std::int
     float* out = a.out + b * a.out_stride[0] + place.head * a.out_stride[1] + place.query * a.out_stride[2];
     const bool low = lane < a.features, high = lane + 64 < a.features;
     float x = 0.F, y = 0.F;
-    for (int s = 0; s < a.splits; ++s) {
-      const float w = __shfl(weight, s, kWave);
-      const float* part = a.part + (s * rows + row) * a.features;
-      if (low) x = fmaf(part[lane], w, x);
-      if (high) y = fmaf(part[lane + 64], w, y);
+    // Eight splits' loads at a time, so that their latencies pass together.
+    for (int first = 0; first < a.splits; first += 8) {
+      float px[8], py[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float* part = a.part + (min(first + u, a.splits - 1) * rows + row) * a.features;
+        px[u] = low ? part[lane] : 0.F;
+        py[u] = high ? part[lane + 64] : 0.F;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        // A split past the last has weight 0; it is left out, in case the last holds NaN.
+        const float w = __shfl(weight, first + u, kWave);
+        if (first + u < a.splits) {
+          x = fmaf(px[u], w, x);
+          y = fmaf(py[u], w, y);
+        }
+      }
     }
     if (low) out[lane] = sum == 0.F ? 0.F : x / sum;
     if (high) out[lane + 64] = sum == 0.F ? 0.F : y / sum;
@@ -96,8 +109,6 @@ bool fill_strides(const std::int64_t (&in)[3], std::int64_t heads, std::int64_t 
 
 bool aligned(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15U) == 0; }
 
-// Splits of the keys: enough blocks to fill the CUs several times, with at
-// least kSplitKeys keys in each.
 constexpr int kMostSplits = 64;  // join_splits_kernel: a lane each
 
 }  // namespace
@@ -166,12 +177,19 @@ void place_split(DecodeArgs& a, int splits, void* workspace) {
   a.part_ml = a.part + static_cast<std::size_t>(splits) * a.batch * a.kv_heads * a.rows * a.share * a.features;
 }
 
-int plan_splits(const DecodeArgs& a, std::int64_t blocks, int split_keys, std::size_t workspace_bytes) {
+int plan_splits(const DecodeArgs& a, std::int64_t blocks, int wanted, int split_keys, std::size_t workspace_bytes) {
   std::int64_t keys = a.cols;  // a block's rows see at most this many
   if (a.window > 0) keys = std::min<std::int64_t>(keys, std::int64_t{a.window} + a.sinks + a.rows - 1);
-  std::int64_t splits = std::min<std::int64_t>({kMostSplits, 1024 / std::max<std::int64_t>(1, blocks), keys / split_keys});
+  std::int64_t splits = std::min<std::int64_t>({kMostSplits, wanted / std::max<std::int64_t>(1, blocks), keys / split_keys});
   while (splits > 1 && split_bytes(a, static_cast<int>(splits)) > workspace_bytes) --splits;
   return static_cast<int>(std::max<std::int64_t>(1, splits));
+}
+
+int count_items(const DecodeArgs& a, std::int64_t row_tiles, std::uint32_t& items) {
+  const std::int64_t heads = static_cast<std::int64_t>(a.batch) * a.kv_heads;
+  if (row_tiles * a.splits > (kMostIndex * 2) / heads) return fail(TCX_INVALID_ARGUMENT, "attention is too large for one call");
+  items = static_cast<std::uint32_t>(heads * row_tiles * a.splits);
+  return TCX_OK;
 }
 
 int join_splits(const DecodeArgs& a, hipStream_t s) {
@@ -240,7 +258,7 @@ WindowForm window_form(const DecodeArgs& a, std::size_t workspace_bytes) {
   // A CU holds four blocks that stream, two of four waves with tiles in LDS and
   // one of eight. Packed tiles are split only where a part keeps 512 keys (512
   // rows, 16 heads on 4, 512 keys: 34 us whole, 40 in four parts).
-  f.splits = plan_splits(a, (f.prompt ? f.waves / 2 : 1) * blocks(f.rows), f.packed ? 512 : 128, workspace_bytes - f.tiles);
+  f.splits = plan_splits(a, blocks(f.rows), f.prompt ? 2048 / f.waves : 1024, f.packed ? 512 : 128, workspace_bytes - f.tiles);
   f.bytes = f.tiles + split_bytes(a, f.splits);
   return f;
 }
@@ -249,7 +267,9 @@ template <int D>
 int launch_packed(const DecodeArgs& a, const WindowForm& form, void* workspace, hipStream_t s) {
   auto* tiles = static_cast<PromptTile<D>*>(workspace);
   const int places = static_cast<int>(most_tiles(a)), row_tiles = (a.rows * a.share + form.rows - 1) / form.rows;
-  const std::int64_t heads = static_cast<std::int64_t>(a.batch) * a.kv_heads, items = heads * row_tiles * a.splits;
+  const std::int64_t heads = static_cast<std::int64_t>(a.batch) * a.kv_heads;
+  std::uint32_t items;
+  if (int rc = count_items(a, row_tiles, items); rc != TCX_OK) return rc;
   if (places > 0) {
     const unsigned y = static_cast<unsigned>(std::min<std::int64_t>(heads, 65535));
     hipLaunchKernelGGL(prompt_pack_kernel<D>, dim3(places, y), dim3(256), 0, s, a, tiles, places);
@@ -264,8 +284,8 @@ int launch_packed(const DecodeArgs& a, const WindowForm& form, void* workspace, 
           rc != TCX_OK)
         return rc;
     }
-    const std::int64_t per_xcd = (items + 7) / 8;
-    hipLaunchKernelGGL(kernel, dim3(grid_for(8 * per_xcd, 1, 1 << 22)), dim3(64 * form.waves), kShared, s, a, tiles, places,
+    const std::uint32_t per_xcd = (items + 7) / 8;
+    hipLaunchKernelGGL(kernel, dim3(grid_for(8 * std::int64_t{per_xcd}, 1, 1 << 22)), dim3(64 * form.waves), kShared, s, a, tiles, places,
                        items, per_xcd, row_tiles);
     return check(hipGetLastError(), "attention launch");
   };
@@ -277,7 +297,8 @@ int launch_packed(const DecodeArgs& a, const WindowForm& form, void* workspace, 
 template <int D>
 int launch_prompt(const DecodeArgs& a, const WindowForm& form, hipStream_t s) {
   const int tiles = (a.rows * a.share + form.rows - 1) / form.rows;
-  const std::int64_t items = static_cast<std::int64_t>(a.batch) * a.kv_heads * tiles * a.splits;
+  std::uint32_t items;
+  if (int rc = count_items(a, tiles, items); rc != TCX_OK) return rc;
   hipLaunchKernelGGL((prompt_attention_kernel<D, 4, 1>), dim3(grid_for(items, 1, 1 << 22)), dim3(256), 0, s, a, items, tiles);
   return check(hipGetLastError(), "attention launch");
 }
