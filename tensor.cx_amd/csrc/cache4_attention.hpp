@@ -1,17 +1,20 @@
 // Attention over a 4-bit cache on matrix instructions.
 //
-// Products. A code n of 0..15 is the float16 with the bits n, the subnormal n
-// 2^-24: taking a byte of a row apart yields operands without a conversion, and
-// matrix instructions multiply them exactly. Their other factor is float32 held
-// as two float16 halves of 22 bits together (queries times a power of two of
-// their row), so a score is
-//   s_j = sum over groups G of step_jG (sum over G of q c_j) + low_jG (sum over G of q).
-// The second term is one product on the scale words as they are: a word is the
-// bfloat16 pair (step, low), and meets (0, sum of q) in three bfloat16 parts of
-// 24 bits.
+// Products. A code c of 0..15 enters as (c - 7.5) 2^-9, which float16 holds: the
+// bits c are the float16 c 2^-24, and one packed fused multiply-add of those yields
+// it. (Matrix instructions would take the subnormals themselves, but keep five bits
+// less of a sum; and codes around zero, with the middle of a group in the place of
+// its low end, do not cancel against it in sums over many tokens. Both together: an
+// error of 3.6e-5 of the outputs' size over 512 tokens, where this form's is 3e-7.) Their other factor
+// is float32 held as two float16 halves of 22 bits together (queries times a power
+// of two of their row), so a score is
+//   s_j = sum over groups G of step_jG (sum over G of q (c_j - 7.5)) + mid_jG (sum over G of q),
+// mid = low + 7.5 step. The second term is one product on the scale words as they
+// are: a word is the bfloat16 pair (step, low), and meets 7.5 times the sum of q and
+// the sum, in three bfloat16 parts of 24 bits.
 //
-// Weights. The outputs are sums of (p_j step_jG) c_j and, apart from the codes, of
-// p_j low_jG. With e_j the exponent of token j's largest low or step, the running
+// Weights. The outputs are sums of (p_j step_jG) (c_j - 7.5) and, apart from the
+// codes, of p_j mid_jG. With e_j the exponent of token j's largest low or step, the running
 // maximum M is that of x_j + e_j (x the score in units of log2): p_j = 2^(x_j - M
 // + 14) makes p_j step_jG at most 2^15, which two halves hold to 22 bits, and of a
 // row only what it sees decides M.
@@ -22,7 +25,7 @@
 // n's scores of tokens 16 b + 4 g + v, just the k indices it supplies to O^T =
 // V^T P^T. A lane's 16 bytes of key codes are four columns of a token, of which
 // byte G of each makes group G's operand; its eight values of a V operand are
-// the bytes of column n of eight tokens. Steps and lows go through LDS (for each
+// the bytes of column n of eight tokens. Steps and middles go through LDS (for each
 // group a row of the tile's tokens), where every lane finds its tokens'.
 //
 // With 16 rows a column is a row. With 4, which is what most models ask of a
@@ -34,8 +37,8 @@
 // not four times.
 //
 // Measured: 16 sequences of up to 8192 tokens, 32 heads on 8 of 128 features, 129
-// MB in 36 us and 4 more for the join (a vector kernel of a key at a time: 98 us);
-// 131072 tokens of 16 heads of 64, 168 MB, in 45 us. A copy would take 23 and 31.
+// MB in 38 us and 4 more for the join (a vector kernel of a key at a time: 98 us);
+// 131072 tokens of 16 heads of 64, 168 MB, in 46 and 7. A copy would take 23 and 31.
 // What bounds it is the waves' issue: a tile of 32 tokens is some 500 instructions
 // on 5 KB. Tiles brought by asynchronous copies into an LDS ring, and splits of a
 // fixed length, were no faster.
@@ -57,8 +60,16 @@ __device__ __forceinline__ std::uint32_t byte_pair(std::uint32_t a, std::uint32_
   // Selectors 0..3 are b's bytes, 4..7 a's, 12 is zero.
   return __builtin_amdgcn_perm(a, b, 0x0c000c00U | (kByteB << 16) | (4 + kByteA));
 }
-__device__ __forceinline__ std::uint32_t low_nibbles(std::uint32_t pair) { return pair & 0x000f000fU; }
-__device__ __forceinline__ std::uint32_t high_nibbles(std::uint32_t pair) { return (pair >> 4) & 0x000f000fU; }
+// The codes of a pair's low or high half bytes as operands, (c - 7.5) / 512.
+template <int kBits>
+__device__ __forceinline__ std::uint32_t centred(std::uint32_t bits) {
+  const half2_t c = __builtin_bit_cast(half2_t, bits);
+  constexpr _Float16 kBy = static_cast<_Float16>(32768.F / (1 << kBits)), kMiddle = static_cast<_Float16>(-7.5F / 512.F);
+  return __builtin_bit_cast(std::uint32_t, __builtin_elementwise_fma(c, half2_t{kBy, kBy}, half2_t{kMiddle, kMiddle}));
+}
+__device__ __forceinline__ std::uint32_t low_codes(std::uint32_t pair) { return centred<0>(pair & 0x000f000fU); }
+__device__ __forceinline__ std::uint32_t high_codes(std::uint32_t pair) { return centred<4>(pair & 0x00f000f0U); }
+constexpr float kCodeUnit = 512.F;
 
 // Rows of the cache as a lane takes them.
 template <int D>
@@ -112,7 +123,7 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
   constexpr float kLog2e = 1.44269502F;
   static_assert(kRows == 16 || kRows == 4);
   struct Wave {  // of a group, a token each
-    float key_step[kGroups][32], value_step[kGroups][32], value_low[kGroups][32];
+    float key_step[kGroups][32], value_step[kGroups][32], value_mid[kGroups][32];
     float value_exp[32];
   };
   constexpr int kPitch = D + 4;
@@ -208,15 +219,19 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
         }
         sum = across_sum(sum);
         // Three bfloat16 parts, lanes g = 0, 1 and 2 one each.
-        const __bf16 first = static_cast<__bf16>(sum);
-        const float rest1 = sum - static_cast<float>(first);
-        const __bf16 second = static_cast<__bf16>(rest1);
-        const __bf16 third = static_cast<__bf16>(rest1 - static_cast<float>(second));
-        q_sums[2 * y + 1] = g == 3 ? short{0} : __builtin_bit_cast(short, g == 0 ? first : g == 1 ? second : third);
+        auto part = [&](float value) {
+          const __bf16 first = static_cast<__bf16>(value);
+          const float rest1 = value - static_cast<float>(first);
+          const __bf16 second = static_cast<__bf16>(rest1);
+          const __bf16 third = static_cast<__bf16>(rest1 - static_cast<float>(second));
+          return g == 3 ? short{0} : __builtin_bit_cast(short, g == 0 ? first : g == 1 ? second : third);
+        };
+        q_sums[2 * y] = part(7.5F * sum);
+        q_sums[2 * y + 1] = part(sum);
       }
       most = across_max(most);
       const int field = scale_field(most, 253);
-      row_factor = power_field(254 - field) * 16777216.F;  // 2^24: of the codes
+      row_factor = power_field(254 - field) * kCodeUnit;
 #pragma unroll
       for (int y = 0; y < kGroups; ++y) {
         const bool mine_y = kRows == 16 || q == y;
@@ -228,18 +243,18 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
     __syncthreads();
 
     acc_t o[kT];
-    float low[kGroups], m = neg_inf, l = 0.F;
+    float mid[kGroups], m = neg_inf, l = 0.F;
 #pragma unroll
     for (int y = 0; y < kT; ++y) o[y] = acc_t{0.F, 0.F, 0.F, 0.F};
 #pragma unroll
-    for (int y = 0; y < kGroups; ++y) low[y] = 0.F;
+    for (int y = 0; y < kGroups; ++y) mid[y] = 0.F;
 
     for (int i = wave; i < tiles; i += 4) {
       int j0, count;
       place(i, j0, count);
       const bool whole = count == 32 && j0 + 31 <= p_first && (a.window == 0 || j0 > p_last - a.window || j0 + 31 < a.sinks);
 
-      // Steps and lows into LDS, a token's by a lane that loaded it.
+      // Steps and middles into LDS, a token's by a lane that loaded it.
       {
         std::uint32_t finite = 0;
 #pragma unroll
@@ -253,8 +268,9 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
           for (int y = 0; y < kGroups; ++y) {
             const std::uint32_t even = key_scale[0][y], odd = key_scale[1][y];
             mine.key_step[y][k] = __uint_as_float((g == 0 ? even : odd) << 16);
-            mine.value_step[y][k] = __uint_as_float(value_scale[y] << 16);
-            mine.value_low[y][k] = __uint_as_float(value_scale[y] & 0xffff0000U);
+            const float step = __uint_as_float(value_scale[y] << 16);
+            mine.value_step[y][k] = step;
+            mine.value_mid[y][k] = fmaf(7.5F, step, __uint_as_float(value_scale[y] & 0xffff0000U));
           }
           // Not below 2^-90, so that the sum of the weights stays finite.
           mine.value_exp[k] = static_cast<float>(max(static_cast<int>(finite >> 23), 37) - 127);
@@ -279,7 +295,7 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
         for_groups<kGroups>([&]<int kG>() {
           const std::uint32_t c01 = Lanes::template columns<kG, 0>(key[w]), c23 = Lanes::template columns<kG, 2>(key[w]);
           const half8_t codes = __builtin_bit_cast(
-              half8_t, (word4_t{low_nibbles(c01), high_nibbles(c01), low_nibbles(c23), high_nibbles(c23)}));
+              half8_t, (word4_t{low_codes(c01), high_codes(c01), low_codes(c23), high_codes(c23)}));
           if (kRows == 16) sum = acc_t{0.F, 0.F, 0.F, 0.F};
           sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q_halves[kG][1][lane], sum, 0, 0, 0);
           sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q_halves[kG][0][lane], sum, 0, 0, 0);
@@ -331,7 +347,7 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
 #pragma unroll
         for (int y = 0; y < kT; ++y) o[y] *= f;
 #pragma unroll
-        for (int y = 0; y < kGroups; ++y) low[y] *= f;
+        for (int y = 0; y < kGroups; ++y) mid[y] *= f;
         m = top;
       }
       const float shift = m == neg_inf ? 0.F : m - 14.F;
@@ -343,29 +359,29 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
 
       // A group's weights and its part of the outputs.
       for_groups<kGroups>([&]<int kG>() {
-        float step[kTokens], lows[kTokens];
+        float step[kTokens], mids[kTokens];
 #pragma unroll
         for (int k = 0; k < kTokens; k += 2) {
           const float2v_t u = *reinterpret_cast<const float2v_t*>(&mine.value_step[kG][token(k)]);
-          const float2v_t v = *reinterpret_cast<const float2v_t*>(&mine.value_low[kG][token(k)]);
+          const float2v_t v = *reinterpret_cast<const float2v_t*>(&mine.value_mid[kG][token(k)]);
           step[k] = u[0];
           step[k + 1] = u[1];
-          lows[k] = v[0];
-          lows[k + 1] = v[1];
+          mids[k] = v[0];
+          mids[k + 1] = v[1];
         }
         if (!whole) {  // a token that is not seen may hold NaN
 #pragma unroll
           for (int k = 0; k < kTokens; ++k) {
             const bool out = hidden >> k & 1U;
             step[k] = out ? 0.F : step[k];
-            lows[k] = out ? 0.F : lows[k];
+            mids[k] = out ? 0.F : mids[k];
           }
         }
         float weight[kTokens];
 #pragma unroll
         for (int k = 0; k < kTokens; ++k) {
           weight[k] = x[k] * step[k];
-          low[kG] = fmaf(x[k], lows[k], low[kG]);
+          mid[kG] = fmaf(x[k], mids[k], mid[kG]);
         }
         word4_t w_hi, w_lo;
         if constexpr (kRows == 16) {
@@ -387,8 +403,8 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const std::uint32_t p = byte_pair<kG, kG>(value[2 * k], value[2 * k + 1]);
-          even[k] = low_nibbles(p);
-          odd[k] = high_nibbles(p);
+          even[k] = low_codes(p);
+          odd[k] = high_codes(p);
         }
         const half8_t c0 = __builtin_bit_cast(half8_t, even), c1 = __builtin_bit_cast(half8_t, odd);
         const half8_t hi = __builtin_bit_cast(half8_t, w_hi), lo = __builtin_bit_cast(half8_t, w_lo);
@@ -404,11 +420,11 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
     // A row's columns, then the waves' states, joined in LDS.
     l = across_sum(l);
 #pragma unroll
-    for (int y = 0; y < kGroups; ++y) low[y] = across_sum(low[y]);
+    for (int y = 0; y < kGroups; ++y) mid[y] = across_sum(mid[y]);
     if constexpr (kRows == 4) {
       l = shares_sum(l);
 #pragma unroll
-      for (int y = 0; y < kGroups; ++y) low[y] = shares_sum(low[y]);
+      for (int y = 0; y < kGroups; ++y) mid[y] = shares_sum(mid[y]);
 #pragma unroll
       for (int y = 0; y < kT; ++y)
 #pragma unroll
@@ -420,7 +436,7 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
       for (int y = 0; y < kT; ++y) {
         float4_t part;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) part[v] = fmaf(o[y][v], 16777216.F, low[y / 2]);
+        for (int v = 0; v < 4; ++v) part[v] = fmaf(o[y][v], kCodeUnit, mid[y / 2]);
         *reinterpret_cast<float4_t*>(&shared.part[wave][column][16 * y + 4 * g]) = part;
       }
       if (g == 0) {

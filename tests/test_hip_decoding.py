@@ -346,6 +346,23 @@ def test_cache_attention_of_far_scales(cx):
     assert (np.abs(out - expected)[..., 32:64] <= bound * group * 1.01).all()
 
 
+@pytest.mark.parametrize("heads,rows", [(2, 1), (8, 1), (2, 16)])
+@pytest.mark.parametrize("features", [32, 64, 128])
+def test_cache_attention_of_many_alike(cx, features, heads, rows):
+    """Outputs that are means of many values are exact to their own size.
+
+    Such sums cancel as the exact ones do: a term's error is a weight's (two halves of 22
+    bits, exp2 and the score, some 2^-22 together) times a value, so the root mean
+    square over the outputs is some 2^-21 of theirs; eight times that is allowed."""
+    rng = np.random.default_rng(25)
+    q, k, v = f32(rng, 1, heads, rows, features), f32(rng, 1, 2, 512, features), f32(rng, 1, 2, 512, features)
+    keys, values = cases.cache_rows(k), cases.cache_rows(v)
+    expected, _ = cases.attention(q, cases.cache_values(keys, features), cases.cache_values(values, features), [512], None,
+                                  0, features ** -0.5)
+    out = cx.hip.cache_attention(hip(cx, q), hip(cx, keys), hip(cx, values), hip(cx, np.array([512], np.int32))).numpy()
+    assert np.sqrt(((out - expected) ** 2).mean()) <= 2.0 ** -18 * np.sqrt((expected ** 2).mean())
+
+
 def test_a_lost_group_makes_its_readers_nan(cx):
     rng = np.random.default_rng(24)
     q, k, v, lengths = attention_inputs(rng, (1, 4, 2, 1, 100, 64, None, 0, None))
