@@ -10,6 +10,7 @@
 #pragma once
 
 #include "decoding.hpp"
+#include "halves.hpp"
 
 namespace tcx {
 
@@ -30,41 +31,41 @@ __global__ __launch_bounds__(256) void stream_attention_kernel(DecodeArgs a, std
     const SeenKeys seen = seen_keys(n, a.rows, i0, i1, a.window, a.sinks);
     const int u0 = split_start(a, seen.count(), split), u1 = split_start(a, seen.count(), split + 1);
 
+    const Source source(a, b, kv, li);
     float q[kRows][kF], o[kRows][kF], m[kRows], l[kRows];
+    typename Source::Raw q_raw[kRows];
     int p_row[kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const RowPlace at = row_place(a, kv, min(r0 + r, r1));
       const float* row = a.q + b * a.q_stride[0] + at.head * a.q_stride[1] + at.query * a.q_stride[2];
-#pragma unroll
-      for (int e = 0; e < kF; ++e) {
-        const int f = Source::feature(li, e);
-        // The scale and log2 e go into the query: scores come out in units of log2.
-        q[r][e] = f < a.features ? row[f] * (a.scale * kLog2e) : 0.F;
-        o[r][e] = 0.F;
-      }
+      source.load(row, 0, 0, 0, q_raw[r]);
       p_row[r] = n - a.rows + at.query;
       m[r] = neg_inf;
       l[r] = 0.F;
     }
-    const Source source(a, b, kv, li);
 
-    // Keys of [u0, u1) from `base` on. kMasked: some key is not seen by all of
-    // the rows, or lies past the end; its value is left out, not weighted with 0,
-    // which would let a NaN through.
+    // Keys of [u0, u1) from `base` on, whose loads are under way; each is followed
+    // by the load of the next pass as soon as it has been used. (Past the end they
+    // read the last key again.)
+    typename Source::Raw kr[kEach], vr[kEach];
+    auto place = [&](int base, int u) { return seen.key(min(base + 16 * u + group, u1 - 1)); };
+    auto load_keys = [&](int base) {
+#pragma unroll
+      for (int u = 0; u < kEach; ++u) source.load(a.k, source.k_base, a.k_stride[2], place(base, u), kr[u]);
+    };
+    auto load_values = [&](int base) {
+#pragma unroll
+      for (int u = 0; u < kEach; ++u) source.load(a.v, source.v_base, a.v_stride[2], place(base, u), vr[u]);
+    };
+    // kMasked: some key is not seen by all of the rows, or lies past the end; its
+    // value is left out, not weighted with 0, which would let a NaN through.
     auto pass = [&]<bool kMasked>(int base) {
-      typename Source::Raw kr[kEach], vr[kEach];
-      int key[kEach];
-#pragma unroll
-      for (int u = 0; u < kEach; ++u) {
-        key[u] = seen.key(min(base + 16 * u + group, u1 - 1));
-        source.load(a.k, source.k_base, a.k_stride[2], key[u], kr[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < kEach; ++u) source.load(a.v, source.v_base, a.v_stride[2], key[u], vr[u]);
       float s[kRows][kEach];
+      bool in[kRows][kEach];
 #pragma unroll
       for (int u = 0; u < kEach; ++u) {
+        const int j = place(base, u);
         float x[kF];
         source.values(kr[u], x);
 #pragma unroll
@@ -73,9 +74,11 @@ __global__ __launch_bounds__(256) void stream_attention_kernel(DecodeArgs a, std
 #pragma unroll
           for (int e = 0; e < kF; ++e) dot = fmaf(q[r][e], x[e], dot);
           s[r][u] = lanes16_sum(dot);
-          if (kMasked && !(base + 16 * u + group < u1 && sees(p_row[r], key[u], a.window, a.sinks))) s[r][u] = neg_inf;
+          in[r][u] = !kMasked || ((base + 16 * u + group < u1) & sees(p_row[r], j, a.window, a.sinks));
+          s[r][u] = in[r][u] ? s[r][u] : neg_inf;
         }
       }
+      load_keys(base + 16 * kEach);
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         float top = m[r];
@@ -95,18 +98,30 @@ __global__ __launch_bounds__(256) void stream_attention_kernel(DecodeArgs a, std
       }
 #pragma unroll
       for (int u = 0; u < kEach; ++u) {
-        float x[kF];
-        source.values(vr[u], x);
+        float x[kF];  // past the last feature anything: such outputs are not written
+        source.values_all(vr[u], x);
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-          const bool in =
-              !kMasked || (base + 16 * u + group < u1 && sees(p_row[r], key[u], a.window, a.sinks));
+        for (int r = 0; r < kRows; ++r)
 #pragma unroll
-          for (int e = 0; e < kF; ++e) o[r][e] = in ? fmaf(s[r][u], x[e], o[r][e]) : o[r][e];
-        }
+          for (int e = 0; e < kF; ++e) o[r][e] = in[r][u] ? fmaf(s[r][u], x[e], o[r][e]) : o[r][e];
       }
+      load_values(base + 16 * kEach);
     };
     int base = u0;
+    if (base < u1) {
+      load_keys(base);
+      load_values(base);
+    }
+    // The scale and log2 e go into the query: scores come out in units of log2.
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      source.values(q_raw[r], q[r]);
+#pragma unroll
+      for (int e = 0; e < kF; ++e) {
+        q[r][e] *= a.scale * kLog2e;
+        o[r][e] = 0.F;
+      }
+    }
     if (i0 == i1)
       for (; base + 16 * kEach <= u1; base += 16 * kEach) pass.template operator()<false>(base);
     for (; base < u1; base += 16 * kEach) pass.template operator()<true>(base);
@@ -114,17 +129,12 @@ __global__ __launch_bounds__(256) void stream_attention_kernel(DecodeArgs a, std
     // The wave's four groups, then the block's four waves.
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      float top = fmaxf(m[r], __shfl_xor(m[r], 16, kWave));
-      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      const float top = across_max(m[r]);
       const float f = __builtin_amdgcn_exp2f(m[r] - (top == neg_inf ? 0.F : top));
-      l[r] *= f;
-      l[r] += __shfl_xor(l[r], 16, kWave);
-      l[r] += __shfl_xor(l[r], 32, kWave);
+      l[r] = across_sum(l[r] * f);
 #pragma unroll
       for (int e = 0; e < kF; ++e) {
-        float v = o[r][e] * f;
-        v += __shfl_xor(v, 16, kWave);
-        v += __shfl_xor(v, 32, kWave);
+        const float v = across_sum(o[r][e] * f);
         if (lane < 16) part_o[wave][r][Source::feature(li, e)] = v;
       }
       if (lane == 0) {

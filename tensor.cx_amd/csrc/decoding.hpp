@@ -31,7 +31,7 @@ __host__ __device__ inline SeenKeys seen_keys(int n, int rows, int i0, int i1, i
 
 // Whether the query at key p sees key j.
 __device__ __forceinline__ bool sees(int p, int j, int window, int sinks) {
-  return j <= p && (window == 0 || j > p - window || j < sinks);
+  return (j <= p) & ((window == 0) | (j > p - window) | (j < sinks));
 }
 
 // A call with its arguments checked: strides filled in, window and sinks cut to cols.

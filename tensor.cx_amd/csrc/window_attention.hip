@@ -34,12 +34,18 @@ struct FloatRows {
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       const int f = feature(li, c * kChunk);
-      // Chunks past the last feature read chunk 0 and count as zero.
       raw.c[c] = stream_load(reinterpret_cast<const Chunk*>(row + (f < features ? f : 0)));
-      if (f >= features) raw.c[c] = Chunk{};
     }
   }
+  // Chunks past the last feature hold chunk 0 and count as zeros. (Not set to zeros
+  // where they are loaded: that would wait for the load.)
   __device__ __forceinline__ void values(const Raw& raw, float (&x)[kFeatures]) const {
+    values_all(raw, x);
+#pragma unroll
+    for (int e = 0; e < kFeatures; ++e)
+      if (e >= kChunk || kChunks == 1) x[e] = feature(li, e) < features ? x[e] : 0.F;
+  }
+  __device__ __forceinline__ void values_all(const Raw& raw, float (&x)[kFeatures]) const {
 #pragma unroll
     for (int e = 0; e < kFeatures; ++e) x[e] = raw.c[e / kChunk][e % kChunk];
   }
@@ -50,9 +56,10 @@ __global__ __launch_bounds__(256) void join_splits_kernel(DecodeArgs a, std::int
   const int lane = threadIdx.x & 63, total = a.rows * a.share;
   const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * 4;
   for (std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); row < rows; row += step) {
-    const std::int64_t at = lane < a.splits ? lane * rows + row : row;
-    const float m = lane < a.splits ? a.part_ml[2 * at] : -__builtin_inff();
-    const float l = lane < a.splits ? a.part_ml[2 * at + 1] : 0.F;
+    // Lanes past the last split or feature read the last one: loads without branches
+    // pass together.
+    const auto ml = reinterpret_cast<const float2v_t*>(a.part_ml)[min(lane, a.splits - 1) * rows + row];
+    const float m = lane < a.splits ? ml[0] : -__builtin_inff(), l = lane < a.splits ? ml[1] : 0.F;
     float top = m;
 #pragma unroll
     for (int offset = 32; offset > 0; offset >>= 1) top = fmaxf(top, __shfl_xor(top, offset, kWave));
@@ -69,8 +76,8 @@ __global__ __launch_bounds__(256) void join_splits_kernel(DecodeArgs a, std::int
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const float* part = a.part + (min(first + u, a.splits - 1) * rows + row) * a.features;
-        px[u] = low ? part[lane] : 0.F;
-        py[u] = high ? part[lane + 64] : 0.F;
+        px[u] = part[min(lane, a.features - 1)];
+        py[u] = part[min(lane + 64, a.features - 1)];
       }
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
