@@ -229,11 +229,13 @@ bool aligned16(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15
 int cache_rows(const DecodeArgs& a) { return a.rows * a.share <= 4 ? 4 : 16; }
 
 // 768 blocks fill the GPU three to a CU (512 and 1024: 39.9 and 42.1 us against
-// 37.9), and a split of fewer than 256 keys costs more than it spares.
+// 37.9), and a split of fewer than 256 keys costs more than it spares; nor do two or
+// three pay for the join (8 heads of 64 features, one sequence: 512 keys 8.1 us
+// whole, 9.2 in two; 1024 keys 11.7 whole, 9.5 in four).
 int cache_splits(const DecodeArgs& a, std::size_t workspace_bytes) {
   const int rows = cache_rows(a);
   const std::int64_t blocks = static_cast<std::int64_t>(a.batch) * a.kv_heads * ((a.rows * a.share + rows - 1) / rows);
-  return plan_splits(a, blocks, 768, 256, workspace_bytes);
+  return plan_splits(a, blocks, 768, 256, 1024, workspace_bytes);
 }
 
 template <int D, int kRows>

@@ -64,8 +64,9 @@ std::size_t split_bytes(const DecodeArgs& a, int splits);
 // Places part and part_ml in the workspace.
 void place_split(DecodeArgs& a, int splits, void* workspace);
 // How many splits a call of `blocks` blocks takes to come to `wanted` of them, with
-// at least split_keys keys in each and no more bytes than the workspace has.
-int plan_splits(const DecodeArgs& a, std::int64_t blocks, int wanted, int split_keys, std::size_t workspace_bytes);
+// at least split_keys keys in each and no more bytes than the workspace has; one
+// where its rows see fewer than least_keys, which would not pay for the join.
+int plan_splits(const DecodeArgs& a, std::int64_t blocks, int wanted, int split_keys, int least_keys, std::size_t workspace_bytes);
 // The blocks' work items of a call of `row_tiles` row tiles a head, as a 32-bit
 // count; TCX_INVALID_ARGUMENT where there are more.
 int count_items(const DecodeArgs& a, std::int64_t row_tiles, std::uint32_t& items);

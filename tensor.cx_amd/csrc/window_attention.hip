@@ -184,9 +184,11 @@ void place_split(DecodeArgs& a, int splits, void* workspace) {
   a.part_ml = a.part + static_cast<std::size_t>(splits) * a.batch * a.kv_heads * a.rows * a.share * a.features;
 }
 
-int plan_splits(const DecodeArgs& a, std::int64_t blocks, int wanted, int split_keys, std::size_t workspace_bytes) {
+int plan_splits(const DecodeArgs& a, std::int64_t blocks, int wanted, int split_keys, int least_keys,
+                std::size_t workspace_bytes) {
   std::int64_t keys = a.cols;  // a block's rows see at most this many
   if (a.window > 0) keys = std::min<std::int64_t>(keys, std::int64_t{a.window} + a.sinks + a.rows - 1);
+  if (keys < least_keys) return 1;
   std::int64_t splits = std::min<std::int64_t>({kMostSplits, wanted / std::max<std::int64_t>(1, blocks), keys / split_keys});
   while (splits > 1 && split_bytes(a, static_cast<int>(splits)) > workspace_bytes) --splits;
   return static_cast<int>(std::max<std::int64_t>(1, splits));
@@ -264,8 +266,11 @@ WindowForm window_form(const DecodeArgs& a, std::size_t workspace_bytes) {
   }
   // A CU holds four blocks that stream, two of four waves with tiles in LDS and
   // one of eight. Packed tiles are split only where a part keeps 512 keys (512
-  // rows, 16 heads on 4, 512 keys: 34 us whole, 40 in four parts).
-  f.splits = plan_splits(a, blocks(f.rows), f.prompt ? 2048 / f.waves : 1024, f.packed ? 512 : 128, workspace_bytes - f.tiles);
+  // rows, 16 heads on 4, 512 keys: 34 us whole, 40 in four parts). Others from 512
+  // keys on, of 128 (8 heads of 64 features, one row: 256 keys 4.9 us whole, 7.8 in
+  // two; of 128 features 512 keys 11.8 whole, 9.8 in four).
+  f.splits = plan_splits(a, blocks(f.rows), f.prompt ? 2048 / f.waves : 1024, f.packed ? 512 : 128, f.packed ? 1024 : 512,
+                         workspace_bytes - f.tiles);
   f.bytes = f.tiles + split_bytes(a, f.splits);
   return f;
 }
