@@ -54,15 +54,16 @@ __device__ __forceinline__ int key_slot(int j, int c) {
 __device__ __forceinline__ int value_slot(int row, int chunk) { return row * 8 + (chunk ^ ((row >> 1) & 7)); }
 
 // Chunk c of key j, from registers into the tile's buffers; D / 8 neighbouring
-// lanes hold a key.
+// lanes hold a key. Chunks past the last feature become zeros here: set where they are
+// loaded, the program would wait there for each load.
 template <int D>
-__device__ __forceinline__ void pack_keys(const float4_t (&in)[2], int j, int c, half8_t* key_hi, half8_t* key_lo,
+__device__ __forceinline__ void pack_keys(const float4_t (&in)[2], int j, int c, int features, half8_t* key_hi, half8_t* key_lo,
                                           float* key_factor) {
   float x[8];
   std::uint32_t most = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    x[e] = in[e / 4][e % 4];
+    x[e] = 8 * c < features ? in[e / 4][e % 4] : 0.F;
     most = max(most, magnitude(x[e]));
   }
   const int field = scale_field(lanes_most<D / 8>(most), kMostKeyField);
@@ -81,13 +82,16 @@ __device__ __forceinline__ void pack_keys(const float4_t (&in)[2], int j, int c,
 // D / 4 neighbouring lanes hold a key. Values that are not finite are taken out
 // and marked: a product with them would reach rows that do not see them.
 template <int D>
-__device__ __forceinline__ void measure_values(float4_t (&in)[4], int h, int c, int (&field)[4], float* value_exp,
+__device__ __forceinline__ void measure_values(float4_t (&in)[4], int h, int c, int features, int (&field)[4], float* value_exp,
                                                float* value_unit, int* bad) {
 #pragma unroll
   for (int v = 0; v < 4; ++v) {
     std::uint32_t most = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) most = max(most, magnitude(in[v][e]));
+    for (int e = 0; e < 4; ++e) {
+      in[v][e] = 4 * c < features ? in[v][e] : 0.F;
+      most = max(most, magnitude(in[v][e]));
+    }
     if (__any(most >= 0x7f800000U)) {
       if (most >= 0x7f800000U) {
         most = 0;
@@ -401,18 +405,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Decode
 #pragma unroll
       for (int i = 0; i < kKeyTasks; ++i) {
         const int task = t + i * kThreads, j = task / kKeyChunks, f = 8 * (task % kKeyChunks);
-        const bool in = j < kTile && u + j < u1 && f < a.features;
-        const float* row = kb + seen.key(min(u + j, u1 - 1)) * a.k_stride[2] + (in ? f : 0);
+        // Keys past the end are the last one again, which no row sees there.
+        const float* row = kb + seen.key(min(u + j, u1 - 1)) * a.k_stride[2] + (f < a.features ? f : 0);
         key[i][0] = *reinterpret_cast<const float4_t*>(row);
         key[i][1] = *reinterpret_cast<const float4_t*>(row + 4);
-        if (!in) key[i][0] = key[i][1] = float4_t{0.F, 0.F, 0.F, 0.F};
       }
     };
     auto store_keys = [&] {
 #pragma unroll
       for (int i = 0; i < kKeyTasks; ++i) {
         const int task = t + i * kThreads;
-        pack_keys<D>(key[i], task / kKeyChunks, task % kKeyChunks, key_hi, key_lo, key_factor);
+        pack_keys<D>(key[i], task / kKeyChunks, task % kKeyChunks, a.features, key_hi, key_lo, key_factor);
       }
     };
     auto load_values = [&](int u) {
@@ -421,11 +424,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Decode
         const int task = t + i * kThreads, f = 4 * (task % kQuads), h = task / kQuads;
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const int j = u + 4 * h + v;
-          const bool in = h < kTile / 4 && j < u1 && f < a.features;
-          const float* row = vb + seen.key(min(j, u1 - 1)) * a.v_stride[2] + (in ? f : 0);
+          const float* row = vb + seen.key(min(u + 4 * h + v, u1 - 1)) * a.v_stride[2] + (f < a.features ? f : 0);
           value[i][v] = *reinterpret_cast<const float4_t*>(row);
-          if (!in) value[i][v] = float4_t{0.F, 0.F, 0.F, 0.F};
         }
       }
     };
@@ -433,7 +433,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Decode
 #pragma unroll
       for (int i = 0; i < kValueTasks; ++i) {
         const int task = t + i * kThreads;
-        measure_values<D>(value[i], task / kQuads, task % kQuads, field[i], value_exp[buffer], value_unit[buffer],
+        measure_values<D>(value[i], task / kQuads, task % kQuads, a.features, field[i], value_exp[buffer], value_unit[buffer],
                           &value_bad[buffer]);
       }
     };
@@ -546,35 +546,30 @@ __global__ __launch_bounds__(256) void prompt_pack_kernel(DecodeArgs a, PromptTi
 #pragma unroll
     for (int i = 0; i < kKeyTasks; ++i) {
       const int task = t + i * kThreads, j = task / kKeyChunks, f = 8 * (task % kKeyChunks);
-      const bool in = j0 + j < n && f < a.features;
-      const float* row = kb + (in ? j0 + j : 0) * a.k_stride[2] + (in ? f : 0);
+      const float* row = kb + min(j0 + j, n - 1) * a.k_stride[2] + (f < a.features ? f : 0);
       key[i][0] = *reinterpret_cast<const float4_t*>(row);
       key[i][1] = *reinterpret_cast<const float4_t*>(row + 4);
-      if (!in) key[i][0] = key[i][1] = float4_t{0.F, 0.F, 0.F, 0.F};
     }
 #pragma unroll
     for (int i = 0; i < kValueTasks; ++i) {
       const int task = t + i * kThreads, f = 4 * (task % kQuads), h = task / kQuads;
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        const int j = j0 + 4 * h + v;
-        const bool in = h < kTile / 4 && j < n && f < a.features;
-        const float* row = vb + (in ? j : 0) * a.v_stride[2] + (in ? f : 0);
+        const float* row = vb + min(j0 + 4 * h + v, n - 1) * a.v_stride[2] + (f < a.features ? f : 0);
         value[i][v] = *reinterpret_cast<const float4_t*>(row);
-        if (!in) value[i][v] = float4_t{0.F, 0.F, 0.F, 0.F};
       }
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kKeyTasks; ++i) {
       const int task = t + i * kThreads;
-      pack_keys<D>(key[i], task / kKeyChunks, task % kKeyChunks, out.key_hi, out.key_lo, out.key_factor);
+      pack_keys<D>(key[i], task / kKeyChunks, task % kKeyChunks, a.features, out.key_hi, out.key_lo, out.key_factor);
     }
 #pragma unroll
     for (int i = 0; i < kValueTasks; ++i) {
       const int task = t + i * kThreads, h = task / kQuads;
       int field[4];
-      measure_values<D>(value[i], h, task % kQuads, field, out.value_exp, out.value_unit, &out.bad);
+      measure_values<D>(value[i], h, task % kQuads, a.features, field, out.value_exp, out.value_unit, &out.bad);
       pack_values<D>(value[i], h, task % kQuads, field, reinterpret_cast<half4_t*>(out.value_hi),
                      reinterpret_cast<half4_t*>(out.value_lo));
     }
