@@ -230,14 +230,16 @@ std::size_t tile_bytes(const DecodeArgs& a) {
 }
 
 // Which kernel, for `total` rows of `heads` key heads:
-// * fewer than 16 rows stream the keys past them;
-// * from 16 rows on, matrix instructions, in blocks of 64 rows that pack what
-//   they see for themselves (prompt_attention_kernel);
-// * where a tile of keys would be packed by four blocks and more of a full GPU, or
-//   by sixteen, it is packed once instead (prompt_pack_kernel and
-//   prompt_tile_kernel): 8 sequences of 64 rows, 32 heads on 8 of 64 features and
-//   512 keys 35.5 -> 27.3 us, a prompt of 2048 86 -> 59; 2 sequences of 64 rows,
-//   16 heads on 4 of 128 features and 8192 keys 90 -> 98 the other way;
+// * up to 8 rows stream the keys past them (4 sequences of 12 rows, 8 heads of 128
+//   features, 2000 keys: 47 -> 32 us on matrix instructions; of 8 rows 28 -> 32);
+// * more take matrix instructions, in blocks of 64 rows that pack what they see for
+//   themselves (prompt_attention_kernel);
+// * where a tile of keys would be packed by four blocks and more of a GPU that is
+//   nearly full, or by sixteen, it is packed once instead (prompt_pack_kernel and
+//   prompt_tile_kernel): 4 sequences of 200 rows, 16 heads on 8 of 128 features and
+//   1000 keys 71 -> 57 us, a prompt of 2048, 16 heads on 4 of 64, 107 -> 63; 2
+//   sequences of 64 rows, 16 heads on 4 of 128 features and 8192 keys, 32 blocks, 65
+//   -> 80 the other way, one of 512, 8 heads of 64 features, 64 blocks, 17 -> 20;
 // * in blocks of 128 rows where those are at least 256, one a CU (2048 rows, 16
 //   heads on 4 of 128 features: 137 -> 107 us; 8 heads of their own, 128 blocks:
 //   90 -> 103 the other way), and of 256 where those are, heads have more than 64
@@ -249,14 +251,14 @@ WindowForm window_form(const DecodeArgs& a, std::size_t workspace_bytes) {
   const auto blocks = [&](int rows) { return heads * ((total + rows - 1) / rows); };
   WindowForm f{};
   f.splits = 1;
-  if (total < 16) {
+  if (total <= 8) {
     f.rows = stream_rows(a);
   } else {
     f.prompt = true;
     f.waves = 4;
     f.each = 1;
     const std::size_t tiles = static_cast<std::size_t>(heads * most_tiles(a)) * tile_bytes(a);
-    if ((total >= 1024 || (total >= 256 && blocks(64) >= 256)) && tiles <= workspace_bytes) {
+    if ((total >= 1024 || (total >= 256 && blocks(64) >= 192)) && tiles <= workspace_bytes) {
       f.packed = true;
       f.tiles = tiles;
       if (blocks(128) >= 256) f.waves = 8;

@@ -209,10 +209,12 @@ def test_two_threads(capi, runtime):
         same(loop.results(), want)
 
 
-# (batch, heads, kv_heads, rows, cols, features, window, sinks): sixteen rows and more of a
+# (batch, heads, kv_heads, rows, cols, features, window, sinks): more than eight rows of a
 # head take matrix instructions; those with many blocks pack the keys once, in
 # blocks of 64, 128 or 256 rows.
 PROMPTS = [
+    (2, 3, 1, 3, 700, 64, None, 0),
+    (1, 1, 1, 15, 900, 128, None, 2),
     (1, 1, 1, 1030, 1030, 64, 100, 3),
     (1, 2, 1, 600, 1500, 128, None, 0),
     (43, 2, 2, 257, 300, 32, 70, 5),
