@@ -539,7 +539,8 @@ int tcx_hip_window_attention_supported(int64_t features);
  * that sees no key gets zeros. Hidden keys have no influence, whatever they
  * hold; a row that sees a NaN is NaN, and what infinities that it sees make of
  * it is not specified. Pointers are 16-byte aligned, strides multiples of 4, rows *
- * heads / kv_heads, cols and batch * kv_heads below 2^30. The workspace (16-byte
+ * heads / kv_heads, cols and batch * kv_heads below 2^30, and no more than 2^31
+ * blocks (of at least a row of a key head each) may be asked for. The workspace (16-byte
  * aligned, may be NULL) takes the states of keys split over blocks, as far as
  * it has room; the query says how much such a call can use, and it must stay
  * allocated until the stream has run the call. */
@@ -583,9 +584,10 @@ int tcx_hip_cache4_attention_f32(const float* q, const int32_t* key_cache, const
 /* Beam search's choice: of the candidates (beam k, token v) of each sequence, at
  * scores[b, k] + logits[b, k, v] - log(sum over the beam of exp(logits)), the
  * `count` best in descending order: their scores, beams and tokens, [batch,
- * count] each. Candidates are compared in 64 bits; of one beam the larger logit
- * comes first, then the lower token, and of equal scores the lower beam. NaN
- * comes before every number; a beam whose logits are all -inf offers -inf. A
+ * count] each. Candidates are compared in 64 bits; of equal scores the lower
+ * beam comes first, and of one beam the larger logit, then the lower token. NaN
+ * comes before every number, and a beam with a NaN or +inf among its logits offers
+ * NaN alone; a beam whose logits are all -inf offers -inf. A
  * beam with finished[b, k] != 0 (may be NULL) offers token `eos` at its own
  * score and -inf for the others. beams * vocabulary is below 2^31, count at most
  * TCX_HIP_BEAM_MAX_COUNT and beams * vocabulary. The workspace (16-byte aligned,

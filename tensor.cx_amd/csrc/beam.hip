@@ -208,14 +208,16 @@ __device__ __forceinline__ double key_double(std::uint64_t key) {
   return __longlong_as_double(static_cast<long long>(word));
 }
 
-// A candidate of a sequence: its score's key (0: none), and its flat index
-// beam * vocabulary + token inverted.
+// A candidate of a sequence: its score's key (0: none), then what orders equal
+// scores, the lower beam, of one beam the larger logit, then the lower token.
+// (Scores of different logits are equal where a beam's own score is far larger.)
 struct Candidate {
-  std::uint64_t key;
-  std::uint32_t order;
+  std::uint64_t key, logit;  // logit: its key under the beam, inverted
+  std::uint32_t token;       // inverted
 };
 __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
-  return a.key > b.key || (a.key == b.key && a.order > b.order);
+  if (a.key != b.key) return a.key > b.key;
+  return a.logit > b.logit || (a.logit == b.logit && a.token > b.token);
 }
 
 // A block a sequence.
@@ -223,8 +225,8 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
   constexpr int kHeld = 8;  // candidates of a thread that stay in registers
   constexpr float kLog2e = 1.44269502F;
   __shared__ double shift[kBeams];
-  __shared__ std::uint64_t listed_key[kMerged];
-  __shared__ std::uint32_t listed_order[kMerged];
+  __shared__ std::uint64_t listed_key[kMerged], listed_logit[kMerged];
+  __shared__ std::uint32_t listed_token[kMerged];
   __shared__ std::uint32_t wave_key[4];
   __shared__ Candidate wave_best[4];
   __shared__ int listed_count;
@@ -272,20 +274,21 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
     auto make = [&](int c, std::uint64_t place, double score) -> Candidate {
       const int beam = c / each, at = c - beam * each;
       double value;
-      std::uint32_t token;
+      std::uint32_t token, logit = 0;
       if (done(beam)) {
         // The end token at the beam's score, then the others at -inf by index; a
         // score of -inf leaves nothing but the index to go by.
-        if (at >= min(a.count, a.vocabulary)) return {0, 0};
+        if (at >= min(a.count, a.vocabulary)) return {0, 0, 0};
         const bool plain = score == -__builtin_inf();
         token = plain ? at : at == 0 ? a.eos : at - 1 < a.eos ? at - 1 : at;
         value = plain || at > 0 ? -__builtin_inf() : score;
       } else {
-        if (place == 0) return {0, 0};
+        if (place == 0) return {0, 0, 0};
         token = ~static_cast<std::uint32_t>(place);
-        value = (static_cast<double>(key_logit(static_cast<std::uint32_t>(place >> 32))) - shift[beam]) + score;
+        logit = static_cast<std::uint32_t>(place >> 32);
+        value = (static_cast<double>(key_logit(logit)) - shift[beam]) + score;
       }
-      return {double_key(value), ~(static_cast<std::uint32_t>(beam) * static_cast<std::uint32_t>(a.vocabulary) + token)};
+      return {double_key(value), (static_cast<std::uint64_t>(~static_cast<std::uint32_t>(beam)) << 32) | logit, ~token};
     };
     auto candidate = [&](int c) {
       return make(c, a.places[b * candidates + c], a.scores[b * a.beams + c / each]);
@@ -295,7 +298,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
       const int c = t + 256 * h;
-      held[h] = c < candidates ? make(c, place[h], score[h]) : Candidate{0, 0};
+      held[h] = c < candidates ? make(c, place[h], score[h]) : Candidate{0, 0, 0};
       most = max(most, static_cast<std::uint32_t>(held[h].key >> 32));
     }
     for (int c = t + 256 * kHeld; c < candidates; c += 256) most = max(most, static_cast<std::uint32_t>(candidate(c).key >> 32));
@@ -305,30 +308,35 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
       const int place = atomicAdd(&listed_count, 1);
       if (place >= kMerged) return;
       listed_key[place] = mine.key;
-      listed_order[place] = mine.order;
+      listed_logit[place] = mine.logit;
+      listed_token[place] = mine.token;
     };
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) list(held[h]);
     for (int c = t + 256 * kHeld; c < candidates; c += 256) list(candidate(c));
     __syncthreads();
     auto write = [&](int n, const Candidate& c) {
-      const std::uint32_t flat = ~c.order, beam = flat / static_cast<std::uint32_t>(a.vocabulary);
       a.out_scores[b * a.count + n] = static_cast<float>(key_double(c.key));
-      a.out_beams[b * a.count + n] = static_cast<std::int32_t>(beam);
-      a.out_tokens[b * a.count + n] = static_cast<std::int32_t>(flat - beam * static_cast<std::uint32_t>(a.vocabulary));
+      a.out_beams[b * a.count + n] = static_cast<std::int32_t>(~static_cast<std::uint32_t>(c.logit >> 32));
+      a.out_tokens[b * a.count + n] = static_cast<std::int32_t>(~c.token);
     };
     const int found = listed_count;
     if (found <= kMerged) {
       for (int i = t; i < found; i += 256) {
-        const Candidate mine{listed_key[i], listed_order[i]};
-        const int rank = count_before(found, [&](int j) { return before({listed_key[j], listed_order[j]}, mine); });
+        const std::uint64_t key = listed_key[i];
+        int rank = count_before(found, [&](int j) { return listed_key[j] > key; });
+        if (rank >= a.count) continue;
+        const Candidate mine{key, listed_logit[i], listed_token[i]};
+        // Among equal scores; most have none, and the first pass is over the keys alone.
+        if (count_before(found, [&](int j) { return listed_key[j] == key; }) > 1)
+          for (int j = 0; j < found; ++j) rank += listed_key[j] == key && before({key, listed_logit[j], listed_token[j]}, mine);
         if (rank < a.count) write(rank, mine);
       }
     } else {
-      Candidate last{~std::uint64_t{0}, ~std::uint32_t{0}};
-      bool first = true;  // the first may be the very last key and order
+      Candidate last{0, 0, 0};
+      bool first = true;
       for (int n = 0; n < a.count; ++n) {
-        Candidate best{0, 0};
+        Candidate best{0, 0, 0};
         for (int c = t; c < candidates; c += 256) {
           const Candidate mine = candidate(c);
           if ((first || before(last, mine)) && before(mine, best)) best = mine;
@@ -336,7 +344,8 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
 #pragma unroll
         for (int offset = 32; offset > 0; offset >>= 1) {
           const Candidate other{__shfl_xor(static_cast<unsigned long long>(best.key), offset, kWave),
-                                static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(best.order), offset, kWave))};
+                                __shfl_xor(static_cast<unsigned long long>(best.logit), offset, kWave),
+                                static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(best.token), offset, kWave))};
           if (before(other, best)) best = other;
         }
         __syncthreads();

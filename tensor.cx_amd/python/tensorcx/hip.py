@@ -152,9 +152,9 @@ def beam_select(logits, scores, count: int, *, finished=None, eos: int | None = 
     token v) of every sequence the best ``count`` (at most 256) by scores[b, k] +
     log_softmax(logits[b, k])[v], in descending order, for logits (batch, beams,
     vocabulary) and scores (batch, beams) of up to 64 beams. Candidates are
-    compared in 64 bits; of one beam the larger logit comes first, then the lower
-    token, and of equal scores the lower beam; NaN comes before every number. A
-    beam that is finished (bool (batch, beams)) offers the token ``eos`` at its own
+    compared in 64 bits; of equal scores the lower beam comes first, and of one beam
+    the larger logit, then the lower token. NaN comes before every number, and a beam
+    with a NaN or +inf among its logits offers NaN alone. A beam that is finished (bool (batch, beams)) offers the token ``eos`` at its own
     score and nothing (-inf) besides."""
     from . import Tensor, _core, _inference
     if (finished is None) != (eos is None):

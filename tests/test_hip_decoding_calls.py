@@ -355,3 +355,47 @@ def test_select_of_ties_alone(capi, beams, vocabulary, count, value):
         assert np.isneginf(got[0]).all()
     else:
         assert (np.abs(got[0] + np.log(vocabulary)) <= np.log(vocabulary) * cases.EPS + 120 * cases.EPS).all()
+
+
+def test_select_behind_a_far_score(capi):
+    """A beam at -1e30 whose scores all round to the same: the larger logits first, after
+    every token of the other beam."""
+    rng = np.random.default_rng(51)
+    logits = f32(rng, 1, 2, 9000)
+    logits[0, 0, 20:] = -np.inf
+    got = select(capi, logits, np.array([[0, -1e30]], np.float32), 40)
+    assert got[1][0].tolist() == [0] * 20 + [1] * 20
+    np.testing.assert_array_equal(got[2][0, :20], np.argsort(-logits[0, 0, :20], kind="stable"))
+    np.testing.assert_array_equal(got[2][0, 20:], np.argsort(-logits[0, 1], kind="stable")[:20])
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+@pytest.mark.parametrize("vocabulary", [50, 40000])
+def test_select_of_a_lost_beam(capi, vocabulary, value):
+    """NaN or +inf makes its beam's candidates NaN, which come first, by their logits."""
+    rng = np.random.default_rng(52)
+    logits = f32(rng, 1, 3, vocabulary)
+    logits[0, 1, 37] = value
+    got = select(capi, logits, np.zeros((1, 3), np.float32), 5)
+    assert np.isnan(got[0]).all() and got[1][0].tolist() == [1] * 5
+    rest = np.where(np.arange(vocabulary) == 37, -np.inf, logits[0, 1])
+    np.testing.assert_array_equal(got[2][0], [37, *np.argsort(-rest, kind="stable")[:4]])
+
+
+@pytest.mark.parametrize("batch,heads,kv,rows", [(1, 2, 1, 20), (2, 4, 4, 300), (3, 8, 2, 1), (64, 8, 8, 130)])
+def test_no_keys(capi, batch, heads, kv, rows):
+    """Without keys every row is zeros, in each form, with the workspace that the query asks for."""
+    q = capi.DeviceArray.from_numpy(np.ones((batch, heads, rows, 64), np.float32))
+    out = capi.DeviceArray.from_numpy(np.full((batch, heads, rows, 64), 7, np.float32))
+    desc = capi.window_attention_desc(batch, heads, kv, rows, 0, 64)
+    capi.window_attention(q.ptr, None, None, out.ptr, desc, workspace=capi.window_attention_workspace(desc))
+    capi.synchronize()
+    assert (out.numpy() == 0).all()
+    n = capi.DeviceArray.from_numpy(np.zeros(batch, np.int32))
+    cache = capi.DeviceArray.from_numpy(np.full((batch, kv, 700, 10), 0x7fc07fc0, np.int32))
+    out = capi.DeviceArray.from_numpy(np.full((batch, heads, rows, 64), 7, np.float32))
+    desc = capi.window_attention_desc(batch, heads, kv, rows, 700, 64, lengths=n.ptr)
+    ws = capi.window_attention_workspace(desc, cache=True)
+    capi.cache4_attention(q.ptr, cache.ptr, cache.ptr, out.ptr, desc, workspace=ws)
+    capi.synchronize()
+    assert (out.numpy() == 0).all()
