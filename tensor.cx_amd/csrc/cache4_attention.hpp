@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
     const int n = checked_length(a, b);
     const int i0 = row_query(a, r0), i1 = row_query(a, r1);
     const SeenKeys seen = seen_keys(n, a.rows, i0, i1, a.window, a.sinks);
-    const int u0 = split_start(a, seen.count(), split), u1 = split_start(a, seen.count(), split + 1);
+    const int u0 = split_start<128>(a, seen.count(), split), u1 = split_start<128>(a, seen.count(), split + 1);
     // The split's keys as two runs, of the sinks and of the window, in tiles of 32.
     const int sink_end = min(u1, seen.sinks);
     const int from = seen.key(max(u0, seen.sinks)), to = from + max(u1 - max(u0, seen.sinks), 0);

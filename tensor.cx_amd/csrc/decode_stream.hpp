@@ -29,7 +29,7 @@ __global__ __launch_bounds__(256) void stream_attention_kernel(DecodeArgs a, std
     const int n = checked_length(a, b);
     const int i0 = row_query(a, r0), i1 = row_query(a, r1);
     const SeenKeys seen = seen_keys(n, a.rows, i0, i1, a.window, a.sinks);
-    const int u0 = split_start(a, seen.count(), split), u1 = split_start(a, seen.count(), split + 1);
+    const int u0 = split_start<16 * kEach>(a, seen.count(), split), u1 = split_start<16 * kEach>(a, seen.count(), split + 1);
 
     const Source source(a, b, kv, li);
     float q[kRows][kF], o[kRows][kF], m[kRows], l[kRows];

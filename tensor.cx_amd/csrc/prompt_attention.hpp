@@ -391,7 +391,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Decode
     const int r0 = (row_tiles - 1 - from_end) * kRows, r1 = min(r0 + kRows, total) - 1;
     const int n = checked_length(a, b);
     const SeenKeys seen = seen_keys(n, a.rows, row_query(a, r0), row_query(a, r1), a.window, a.sinks);
-    const int u0 = split_start(a, seen.count(), split), u1 = split_start(a, seen.count(), split + 1);
+    const int u0 = split_start<kTile>(a, seen.count(), split), u1 = split_start<kTile>(a, seen.count(), split + 1);
     const float* kb = static_cast<const float*>(a.k) + b * a.k_stride[0] + kv * a.k_stride[1];
     const float* vb = static_cast<const float*>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
 
@@ -628,7 +628,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_tile_kernel(DecodeArgs 
     const PromptTile<D>* from = tiles + static_cast<std::int64_t>(head) * places;
     const float* vb = static_cast<const float*>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
     PromptRows<D, kQ> rows;
-    const int t0 = split_start(a, seen.count(), split), t1 = split_start(a, seen.count(), split + 1);
+    const int t0 = split_start<1>(a, seen.count(), split), t1 = split_start<1>(a, seen.count(), split + 1);
     auto copy = [&](int i) {
       copy_to_lds<kWaves, static_cast<int>(sizeof(PromptTile<D>))>(from + all.place(seen.tile(i)), &stage[i & 1], wave, lane);
     };

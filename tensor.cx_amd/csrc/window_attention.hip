@@ -189,7 +189,9 @@ int plan_splits(const DecodeArgs& a, std::int64_t blocks, int wanted, int split_
   std::int64_t keys = a.cols;  // a block's rows see at most this many
   if (a.window > 0) keys = std::min<std::int64_t>(keys, std::int64_t{a.window} + a.sinks + a.rows - 1);
   if (keys < least_keys) return 1;
-  std::int64_t splits = std::min<std::int64_t>({kMostSplits, wanted / std::max<std::int64_t>(1, blocks), keys / split_keys});
+  // The nearest number of parts (2000 keys in parts of 128: 16 of two rounds of 64, not
+  // 15 of up to three: 4 sequences of 12 rows, 8 heads of 128 features 32 -> 25 us).
+  std::int64_t splits = std::min<std::int64_t>({kMostSplits, wanted / std::max<std::int64_t>(1, blocks), (keys + split_keys / 2) / split_keys});
   while (splits > 1 && split_bytes(a, static_cast<int>(splits)) > workspace_bytes) --splits;
   return static_cast<int>(std::max<std::int64_t>(1, splits));
 }
@@ -231,7 +233,8 @@ std::size_t tile_bytes(const DecodeArgs& a) {
 
 // Which kernel, for `total` rows of `heads` key heads:
 // * up to 8 rows stream the keys past them (4 sequences of 12 rows, 8 heads of 128
-//   features, 2000 keys: 47 -> 32 us on matrix instructions; of 8 rows 28 -> 32);
+//   features, 2000 keys: 47 -> 32 us on matrix instructions; of 8 rows 28 -> 32, in
+//   15 parts of the keys);
 // * more take matrix instructions, in blocks of 64 rows that pack what they see for
 //   themselves (prompt_attention_kernel);
 // * where a tile of keys would be packed by four blocks and more of a GPU that is
