@@ -112,8 +112,9 @@ struct StoreArgs {
 //
 // Measured: 2 sequences of 4096 tokens, 8 heads of 128 features, 67 MB in and 10 MB
 // out, in 17.2 us (28.6 with sixteen lanes' extremes of each group in all lanes, the
-// compiler's quotient, a token's place by divisions and loads that stay in the caches; two and
-// four tokens of a lane were no faster); 10 us of it are its vector instructions.
+// compiler's quotient, a token's place by divisions and loads that stay in the
+// caches; two and four tokens of a lane were no faster); 10 us of it are its vector
+// instructions.
 template <int D>
 __global__ __launch_bounds__(256) void cache_store_kernel(StoreArgs a) {
   using Row = CacheRow<D>;

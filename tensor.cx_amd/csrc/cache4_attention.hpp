@@ -38,9 +38,9 @@
 //
 // Measured: 16 sequences of up to 8192 tokens, 32 heads on 8 of 128 features, 129
 // MB in 38 us and 4 more for the join (a vector kernel of a key at a time: 98 us);
-// 131072 tokens of 16 heads of 64, 168 MB, in 46 and 7. A copy would take 23 and 31.
+// 131072 tokens of 16 heads of 64, 168 MB, in 45 and 7. A copy would take 23 and 31.
 // What bounds it is the waves' issue: a tile of 32 tokens is some 500 instructions
-// on 5 KB. Tiles brought by asynchronous copies into an LDS ring, and splits of a
+// on 5 KB (four query rows that share a key head, and one, take the same time). Tiles brought by asynchronous copies into an LDS ring, and splits of a
 // fixed length, were no faster.
 #pragma once
 

@@ -6,7 +6,12 @@
 // block sixteen; each group of lanes keeps an online softmax of its own (the
 // running maximum m in units of log2, the sum l, the outputs o) and the sixteen
 // states are joined at the end, in registers across a wave's groups and in LDS
-// across the waves.
+// across the waves. Matrix instructions would have their rows idle: a step has as
+// many rows as heads share a key head, up to 8.
+//
+// Measured: 8 sequences of 1028 keys seen, 32 heads on 8 of 128 features, 67 MB in 17.4
+// us and 3.9 for the join; a plain read takes 10.5. The rest is a block's start (its
+// length, then its queries and first keys) and end around four passes.
 #pragma once
 
 #include "decoding.hpp"

@@ -105,8 +105,8 @@ __device__ __forceinline__ BlockWork block_work(const DecodeArgs& a, std::uint32
 // differ by one quantum at most, the keys that a block takes in one round, so that no
 // round is left to a few keys (8 sequences of 1028 keys, 32 heads on 8 of 128
 // features: 18.6 -> 17.4 us; the 4-bit cache of 16 sequences of 4096 to 8192 tokens:
-// 38.1 -> 37.6). A fixed number of keys to each split, which leaves the last ones of short sequences empty, was
-// slower: 44 us against 38 for 16 sequences of 4096 to 8192 tokens.
+// 38.1 -> 37.6). A fixed number of keys to each split, which leaves the last ones of
+// short sequences empty, was slower: 44 us against 38 for the latter.
 template <int kQuantum>
 __device__ __forceinline__ int split_start(const DecodeArgs& a, int count, int s) {
   if (a.splits == 1) return s == 0 ? 0 : count;
