@@ -11,8 +11,9 @@
 // of its candidates; T is the least, over the four waves, of a wave's ceil(count /
 // 4)-th largest thread maximum, so that at least count candidates are >= T. Those,
 // a few times count of them where values are in no special order, go to a list
-// in LDS and are put in order by counting those before each. Where the list is
-// too short for them (long runs of equal values) the first are taken one by one.
+// in LDS and are put in order by counting those before each. Where they are too many
+// for that (long runs of equal values, such as masked tokens) the first are taken one
+// by one.
 //
 // The parts read the logits once, and hold them in registers. Measured: 128 beams of
 // 128256 logits, 65.7 MB, in 20.5 us with count 16 (a plain read takes 10.5), and
@@ -70,6 +71,14 @@ __device__ __forceinline__ std::uint32_t block_bound(std::uint32_t most, int cou
   if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = bound;
   __syncthreads();
   return min(min(shared[0], shared[1]), min(shared[2], shared[3]));
+}
+
+// Whether `found` of a list are put in order by counting: that takes a thread some 35
+// cycles for each pair, where taking `wanted` one by one costs some 2400 each and
+// more for `more` candidates of a thread (four beams of 32000 logits, one in a
+// hundred not masked: 245 us by counting alone, 16 so).
+__device__ __forceinline__ bool counted(int found, int listed, int wanted, int more) {
+  return found <= listed && (found + 255) / 256 * found <= wanted * (70 + 4 * more);
 }
 
 // How many of a list come before one of them.
@@ -164,7 +173,7 @@ __global__ __launch_bounds__(256, kEach == 32 ? 3 : 4) void beam_part_kernel(Bea
     }
     std::uint64_t* out = a.places + static_cast<std::int64_t>(item) * a.count;
     const int found = listed_count, wanted = min(a.count, n);
-    if (found <= kListed) {
+    if (counted(found, kListed, wanted, 0)) {
       for (int i = t; i < found; i += 256) {
         const std::uint64_t mine = listed[i];
         const int rank = count_before(found, [&](int j) { return listed[j] > mine; });
@@ -321,7 +330,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
       a.out_tokens[b * a.count + n] = static_cast<std::int32_t>(~c.token);
     };
     const int found = listed_count;
-    if (found <= kMerged) {
+    if (counted(found, kMerged, a.count, candidates / 256)) {
       for (int i = t; i < found; i += 256) {
         const std::uint64_t key = listed_key[i];
         int rank = count_before(found, [&](int j) { return listed_key[j] > key; });

@@ -357,6 +357,22 @@ def test_select_of_ties_alone(capi, beams, vocabulary, count, value):
         assert (np.abs(got[0] + np.log(vocabulary)) <= np.log(vocabulary) * cases.EPS + 120 * cases.EPS).all()
 
 
+@pytest.mark.parametrize("shape", [(1, 4, 32000, 8), (16, 8, 40000, 16), (1, 2, 2048, 3)], ids=str)
+@pytest.mark.parametrize("kept", [0.3, 0.01, 0.0005])
+def test_select_of_masked_logits(capi, shape, kept):
+    """Most tokens at -inf, in some parts of a row all of them."""
+    batch, beams, vocabulary, count = shape
+    rng = np.random.default_rng(vocabulary)
+    logits, scores = f32(rng, batch, beams, vocabulary), f32(rng, batch, beams)
+    logits[rng.random(logits.shape) >= kept] = -np.inf
+    want, got = cases.beam_best(logits, scores, count), select(capi, logits, scores, count)
+    np.testing.assert_array_equal(got[1], want[1])
+    np.testing.assert_array_equal(got[2], want[2])
+    seen = np.isfinite(want[0])
+    assert np.isneginf(got[0][~seen]).all()
+    assert (np.abs(got[0][seen] - want[0][seen]) <= np.abs(want[0][seen]) * cases.EPS + 120 * cases.EPS).all()
+
+
 def test_select_behind_a_far_score(capi):
     """A beam at -1e30 whose scores all round to the same: the larger logits first, after
     every token of the other beam."""
