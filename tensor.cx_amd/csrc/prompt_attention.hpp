@@ -12,11 +12,15 @@
 // in its row still keeps its 22 bits, and below that an absolute error of 2^-40
 // of the largest.
 //
-// Weights. With s the score in units of log2 and V_j = 2^e_j V'_j, the sum over
-// keys of 2^s_j V_j is one of 2^(s_j + e_j) V'_j: the running maximum M is that
-// of x_j = s_j + e_j, which is each row's own, so that no row's precision depends
-// on values that it does not see. P = 2^(x - M + 15) is at most 2^15, split as
-// above; the softmax's sum takes 2^-e_j P.
+// Weights. With s the score in units of log2, p_j = 2^(s_j - base) for a whole number
+// `base` of each row, near its largest score, and the softmax's sum is that of p_j,
+// whatever the values are. With V_j = 2^e_j V'_j, the outputs are sums of p_j 2^e_j times
+// V'_j: `base` is also such that those products stay below 2^16, which are split as
+// above, and where a row's values are too large or small for both, a power of two
+// 2^rest goes into the products alone. Only what a row sees moves its base and rest,
+// so that nothing else has an influence, and by whole numbers, which is exact. What
+// the halves cost: a weight is off by 2^-22 of itself and by 2^-35 of the row's largest
+// p_j 2^e_j, which shows where one key's values are 2^13 times another's and more.
 //
 // Layout. A block takes 16 kQ rows a wave of one key head (row r: query r / share,
 // head r % share, so that neighbours see the same keys) and walks the keys that
@@ -47,7 +51,15 @@
 namespace tcx {
 
 constexpr int kMostKeyField = 253;   // its inverse is a normal number
-constexpr int kMostValueField = 217; // 2^90: a sum of 2^20 weights stays finite
+constexpr int kMostValueField = 245; // 2^118
+constexpr int kLeastExp = 141 - kMostValueField;  // of e_j
+// A row's base is such that its largest product of a weight and 2^e_j is 2^kAim when it
+// is set, as far as that leaves its largest weight between 2^-kNear and 2^kNear. The
+// five powers of two up to 2^kMost, which float16 still holds, are what scores can rise
+// before it is set anew (with three 241 us in place of 230 for 8192 rows, 16 heads of 64
+// features, window 2048).
+constexpr float kAim = 11.F, kMost = 15.99F, kNear = 60.F, kFar = 64.F;
+constexpr float kWhole = 8388608.F;  // from here on float32 has no fractions
 
 // The slot of chunk c of 8 features of key row j, and of the 16 bytes of 8 keys at
 // chunk c of value row f: xored so that the lanes of a fragment meet different
@@ -111,11 +123,24 @@ __device__ __forceinline__ void measure_values(float4_t (&in)[4], int h, int c, 
     }
     field[v] = scale_field(lanes_most<D / 4>(most), kMostValueField);
     if (c == 0 && h < 16) {
-      value_exp[4 * h + v] = static_cast<float>(140 - field[v]);
-      value_unit[4 * h + v] = power_field(field[v] - 13);
+      value_exp[4 * h + v] = static_cast<float>(141 - field[v]);
+      value_unit[4 * h + v] = power_field(268 - field[v]);
     }
   }
 }
+
+// The largest e_j of a wave's values: of all lanes' fields.
+template <int D, int kTasks>
+__device__ __forceinline__ int most_exponent(const int (&field)[kTasks][4]) {
+  int least = kMostValueField;
+#pragma unroll
+  for (int i = 0; i < kTasks; ++i) least = min(least, min(min(field[i][0], field[i][1]), min(field[i][2], field[i][3])));
+  auto most = static_cast<std::uint32_t>(kMostValueField - least);
+  if constexpr (D < 64) most = lanes_most<16>(most);
+  return static_cast<int>(across_max(most)) + kLeastExp;
+}
+
+__device__ __forceinline__ float largest(const float (&x)[4]) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); }
 
 template <int D>
 __device__ __forceinline__ void pack_values(const float4_t (&in)[4], int h, int c, const int (&field)[4],
@@ -136,6 +161,9 @@ __device__ __forceinline__ void pack_values(const float4_t (&in)[4], int h, int 
   }
 }
 
+// A whole number as an exponent (past those of float32 it makes no difference).
+__device__ __forceinline__ int exponent(float x) { return static_cast<int>(fminf(fmaxf(x, -400.F), 400.F)); }
+
 // A wave's 16 kQ rows: queries as B operands, the running maxima, sums and outputs.
 template <int D, int kQ>
 struct PromptRows {
@@ -144,7 +172,8 @@ struct PromptRows {
   float row_factor[kQ];
   int p_row[kQ];
   acc_t o[kQ][kT];  // feature 4 (r % (D / 4)) + r / (D / 4) of query n at r = 16 i + 4 g + v
-  float m[kQ], l[kQ];
+  float base[kQ], rest[kQ];
+  float top[kQ], l[kQ];  // the largest score from base on, and the sum of this lane's weights
   int first_row, last_row;  // the keys of the wave's first and last queries
   int row0, n16, g;
 
@@ -185,8 +214,9 @@ struct PromptRows {
       }
 #pragma unroll
       for (int i = 0; i < kT; ++i) o[x][i] = acc_t{0.F, 0.F, 0.F, 0.F};
-      m[x] = -__builtin_inff();
-      l[x] = 0.F;
+      base[x] = l[x] = 0.F;
+      top[x] = -__builtin_inff();
+      rest[x] = 0.F;
     }
   }
 
@@ -198,11 +228,65 @@ struct PromptRows {
     return j0 + 63 <= first_row && (a.window == 0 || j0 > last_row - a.window || j0 + 63 < a.sinks);
   }
 
+  // The largest of a tile's s + exponent.
+  __device__ __forceinline__ float most_product(const acc_t (&s)[4], const float* value_exp) const {
+    float most = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4_t add = *reinterpret_cast<const float4_t*>(&value_exp[16 * i + 4 * g]);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) most = fmaxf(most, s[i][v] + add[v]);
+    }
+    return across_max(most);
+  }
+  // Moves the base of the rows x that need it. Rows that do not stay as they are to the
+  // bit: another row's keys, and hidden ones, may be why this is called.
+  __device__ __forceinline__ void move(acc_t (&s)[4], int x, bool first, float most, const float* value_exp) {
+    const float high = most_product(s, value_exp) + rest[x];
+    const bool past = first || high > kMost, need = most > -__builtin_inff() && (past || most > kFar);
+    float to = base[x], aim = rest[x], gone = 0.F;
+    bool plain = true, far = false;
+    if (need) {
+      const float all = past ? ceilf(high) - kAim : 0.F, peak = ceilf(top[x]);
+      const float by = fminf(fmaxf(all, peak - kNear), peak + kNear);
+      to += by;
+      far = fabsf(to) >= kWhole;
+      if (far) to = base[x] + top[x];  // the largest score itself, which the others are then rounded like
+      plain = by == all && !far;
+      gone = to - base[x];
+    }
+    if (__any(!plain)) [[unlikely]] {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s[i][v] = far ? (s[i][v] + base[x]) - to : s[i][v] - gone;
+      top[x] = far ? 0.F : top[x] - gone;
+      gone = 0.F;
+      const float product = most_product(s, value_exp);
+      if (!plain && (first || product + rest[x] > kMost)) aim = kAim - ceilf(product);
+    }
+    top[x] -= gone;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) s[i][v] -= gone;
+    l[x] = ldexpf(l[x], exponent(base[x] - to));
+    const int scale = first ? 0 : exponent((base[x] - to) + (aim - rest[x]));
+    if (__any(scale != 0)) {
+#pragma unroll
+      for (int i = 0; i < kT; ++i)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) o[x][i][v] = ldexpf(o[x][i][v], scale);
+    }
+    base[x] = to;
+    rest[x] = aim;
+  }
+
   // A tile's weights, as B operands of the P V products. key_of(k): the key at
   // place k of the tile, or one past every query.
   template <typename F>
   __device__ __forceinline__ void scores(const DecodeArgs& a, const half8_t* key_hi, const half8_t* key_lo,
-                                         const float* key_factor, const float* value_exp, const float* value_unit,
+                                         const float* key_factor, const float* value_exp, const float* value_unit, float most_exp,
                                          bool whole, F&& key_of, half8_t (&p_hi)[kQ][2], half8_t (&p_lo)[kQ][2]) {
     const float neg_inf = -__builtin_inff();
     acc_t s[kQ][4];
@@ -229,11 +313,10 @@ struct PromptRows {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float4_t factor = *reinterpret_cast<const float4_t*>(&key_factor[16 * i + 4 * g]);
-      const float4_t add = *reinterpret_cast<const float4_t*>(&value_exp[16 * i + 4 * g]);
 #pragma unroll
       for (int x = 0; x < kQ; ++x)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) s[x][i][v] = fmaf(s[x][i][v], row_factor[x] * factor[v], add[v]);
+        for (int v = 0; v < 4; ++v) s[x][i][v] = fmaf(s[x][i][v], row_factor[x] * factor[v], -base[x]);
     }
     if (!whole) {
 #pragma unroll
@@ -249,29 +332,32 @@ struct PromptRows {
     }
 #pragma unroll
     for (int x = 0; x < kQ; ++x) {
-      float top = m[x];
+      float most = s[x][0][0];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) top = fmaxf(top, s[x][i][v]);
-      top = across_max(top);
-      // Rescaled only where some row's maximum moved.
-      if (__any(top > m[x])) {
-        const float f = __builtin_amdgcn_exp2f(m[x] - (top == neg_inf ? 0.F : top));
-        l[x] *= f;
-#pragma unroll
-        for (int i = 0; i < kT; ++i) o[x][i] *= f;
-        m[x] = top;
-      }
-      const float at = m[x] == neg_inf ? 0.F : m[x] - 15.F;
+        for (int v = 0; v < 4; ++v) most = fmaxf(most, s[x][i][v]);
+      most = across_max(most);
+      const bool first = top[x] == neg_inf;
+      top[x] = fmaxf(top[x], most);
+      // By the tile's largest exponent no row's product passes 2^15: mostly.
+      if (__any(first | (most > kFar) | (most + most_exp + rest[x] > kMost))) [[unlikely]]
+        move(s[x], x, first, most, value_exp);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float4_t unit = *reinterpret_cast<const float4_t*>(&value_unit[16 * i + 4 * g]);
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          s[x][i][v] = __builtin_amdgcn_exp2f(s[x][i][v] - at);
-          l[x] = fmaf(s[x][i][v], unit[v], l[x]);
+          s[x][i][v] = __builtin_amdgcn_exp2f(s[x][i][v]);
+          l[x] += s[x][i][v];
+          s[x][i][v] *= unit[v];
         }
+      }
+      if (__any(rest[x] != 0.F)) [[unlikely]] {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) s[x][i][v] = ldexpf(s[x][i][v], exponent(rest[x]));
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -347,8 +433,11 @@ struct PromptRows {
       float* out = a.splits == 1
                        ? a.out + b * a.out_stride[0] + place.head * a.out_stride[1] + place.query * a.out_stride[2]
                        : a.part + row * a.features;
-      // 2^-13: the offset of value_exp.
-      const float by = a.splits > 1 ? 1.F / 8192.F : l[x] == 0.F ? 0.F : 1.F / 8192.F / l[x];
+      // Outputs are held times 2^rest, and 2^14 of V'.
+      const int whole = top[x] > -__builtin_inff() ? exponent(ceilf(top[x])) : 0;
+      const int back = -14 - exponent(rest[x]) - (a.splits > 1 ? whole : 0);
+      const float by = a.splits > 1 ? 1.F : l[x] == 0.F ? 0.F : 1.F / l[x];
+      auto result = [&](float y) { return ldexpf(y * by, back); };
       if constexpr (kQuads % 16 == 0) {
         // Rows e D / 4 + c for e = 0..3 are features 4 c + e: one store of four.
 #pragma unroll
@@ -357,8 +446,8 @@ struct PromptRows {
           for (int v = 0; v < 4; ++v) {
             const int f = 4 * (16 * i + 4 * g + v);
             if (f < a.features)
-              *reinterpret_cast<float4_t*>(out + f) = float4_t{o[x][i][v] * by, o[x][i + kT / 4][v] * by,
-                                                               o[x][i + kT / 2][v] * by, o[x][i + 3 * kT / 4][v] * by};
+              *reinterpret_cast<float4_t*>(out + f) = float4_t{result(o[x][i][v]), result(o[x][i + kT / 4][v]),
+                                                               result(o[x][i + kT / 2][v]), result(o[x][i + 3 * kT / 4][v])};
           }
       } else {
 #pragma unroll
@@ -366,12 +455,12 @@ struct PromptRows {
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const int at = 16 * i + 4 * g + v, f = 4 * (at % kQuads) + at / kQuads;
-            if (f < a.features) out[f] = o[x][i][v] * by;
+            if (f < a.features) out[f] = result(o[x][i][v]);
           }
       }
       if (a.splits > 1 && g == 0) {
-        a.part_ml[2 * row] = m[x];
-        a.part_ml[2 * row + 1] = l[x];
+        a.part_ml[2 * row] = top[x] > -__builtin_inff() ? base[x] + static_cast<float>(whole) : top[x];
+        a.part_ml[2 * row + 1] = ldexpf(l[x], -whole);
       }
     }
   }
@@ -386,8 +475,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Decode
   constexpr int kValueTasks = (kTile / 4 * kQuads + kThreads - 1) / kThreads;
   __shared__ half8_t key_hi[8 * D], key_lo[8 * D], value_hi[8 * D], value_lo[8 * D];
   __shared__ alignas(16) float key_factor[kTile];    // 2^-scale of a key
-  __shared__ alignas(16) float value_exp[2][kTile];  // e_j + 13, and 2 to the minus that
+  __shared__ alignas(16) float value_exp[2][kTile];  // e_j of a key
   __shared__ alignas(16) float value_unit[2][kTile];
+  __shared__ alignas(16) float value_most[2][4];     // the largest e_j that each wave found
   __shared__ int value_bad[2];                       // some value is not finite
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int total = a.rows * a.share;
@@ -442,6 +532,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Decode
         measure_values<D>(value[i], task / kQuads, task % kQuads, a.features, field[i], value_exp[buffer], value_unit[buffer],
                           &value_bad[buffer]);
       }
+      const int most = most_exponent<D>(field);
+      if (lane == 0) value_most[buffer][wave] = static_cast<float>(most);
     };
     auto store_values = [&] {
 #pragma unroll
@@ -480,7 +572,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Decode
       auto key_of = [&](int k) { return u + k < u1 ? seen.key(u + k) : 1 << 30; };
       half8_t p_hi[kQ][2], p_lo[kQ][2];
       if (any_seen)
-        rows.scores(a, key_hi, key_lo, key_factor, value_exp[buffer], value_unit[buffer], all_seen, key_of, p_hi, p_lo);
+        rows.scores(a, key_hi, key_lo, key_factor, value_exp[buffer], value_unit[buffer],
+                    largest(value_most[buffer]), all_seen, key_of, p_hi, p_lo);
       __syncthreads();  // B: this tile's values are in LDS, its keys are free
       if (more) {
         store_keys();
@@ -518,9 +611,11 @@ template <int D>
 struct PromptTile {
   half8_t key_hi[8 * D], key_lo[8 * D];
   half8_t value_hi[8 * D], value_lo[8 * D];
-  float key_factor[64], value_exp[64], value_unit[64];
-  int bad;  // some value is not finite
-  int pad[15];
+  float key_factor[64], value_exp[64];
+  float value_unit[64];
+  int most;  // the largest e_j
+  int bad;   // some value is not finite
+  int pad[14];
 };
 
 // The tiles that a call sees: those of its sinks, then the window's; tile i is
@@ -556,8 +651,12 @@ __global__ __launch_bounds__(256) void prompt_pack_kernel(DecodeArgs a, PromptTi
     const int j0 = 64 * seen.tile(place);
     const float* kb = static_cast<const float*>(a.k) + b * a.k_stride[0] + kv * a.k_stride[1];
     const float* vb = static_cast<const float*>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
-    if (t == 0) out.bad = 0;
+    if (t == 0) {
+      out.most = kLeastExp;
+      out.bad = 0;
+    }
     float4_t key[kKeyTasks][2], value[kValueTasks][4];
+    int field[kValueTasks][4];
 #pragma unroll
     for (int i = 0; i < kKeyTasks; ++i) {
       const int task = t + i * kThreads, j = task / kKeyChunks, f = 8 * (task % kKeyChunks);
@@ -583,11 +682,12 @@ __global__ __launch_bounds__(256) void prompt_pack_kernel(DecodeArgs a, PromptTi
 #pragma unroll
     for (int i = 0; i < kValueTasks; ++i) {
       const int task = t + i * kThreads, h = task / kQuads;
-      int field[4];
-      measure_values<D>(value[i], h, task % kQuads, a.features, field, out.value_exp, out.value_unit, &out.bad);
-      pack_values<D>(value[i], h, task % kQuads, field, reinterpret_cast<half4_t*>(out.value_hi),
+      measure_values<D>(value[i], h, task % kQuads, a.features, field[i], out.value_exp, out.value_unit, &out.bad);
+      pack_values<D>(value[i], h, task % kQuads, field[i], reinterpret_cast<half4_t*>(out.value_hi),
                      reinterpret_cast<half4_t*>(out.value_lo));
     }
+    const int most = most_exponent<D>(field);
+    if ((t & 63) == 0) atomicMax(&out.most, most);
     __syncthreads();
     auto* to = reinterpret_cast<float4_t*>(tiles + static_cast<std::int64_t>(head) * places + place);
     const auto* from = reinterpret_cast<const float4_t*>(&out);
@@ -658,8 +758,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_tile_kernel(DecodeArgs 
       const int j0 = 64 * seen.tile(i);
       if (!rows.any_seen(a, j0)) continue;
       half8_t p_hi[kQ][2], p_lo[kQ][2];
-      rows.scores(a, now.key_hi, now.key_lo, now.key_factor, now.value_exp, now.value_unit, rows.all_seen(a, j0),
-                  [&](int k) { return j0 + k; }, p_hi, p_lo);
+      rows.scores(a, now.key_hi, now.key_lo, now.key_factor, now.value_exp, now.value_unit,
+                  static_cast<float>(now.most), rows.all_seen(a, j0), [&](int k) { return j0 + k; }, p_hi, p_lo);
       rows.outputs(now.value_hi, now.value_lo, p_hi, p_lo);
       if (now.bad) rows.add_bad(a, vb, min(64, n - j0), [&](int k) { return j0 + k; });
     }

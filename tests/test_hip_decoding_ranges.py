@@ -1,0 +1,161 @@
+"""GPU tests of the decoding operators over the ranges of their numbers: values of
+keys side by side that are zero, tiny, far apart or near float32's largest.
+
+Each call of more than eight rows of a key head runs in all of its forms: without a
+workspace, with its keys split over blocks, and from packed tiles."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import decoding_cases as cases
+from conftest import require_gpu
+
+pytestmark = pytest.mark.gpu
+
+EPS = cases.EPS
+
+
+@pytest.fixture(scope="module")
+def capi():
+    require_gpu()
+    import tensorcx_hip_capi
+    assert tensorcx_hip_capi.available()
+    return tensorcx_hip_capi
+
+
+def f32(rng, *shape):
+    return rng.normal(size=shape).astype(np.float32)
+
+
+def window(capi, q, k, v, *, window=0, sinks=0, scale=None, lengths=None, workspace=True):
+    """Outputs of (batch, heads, rows, features) arrays, with the workspace that is asked for or none."""
+    dq, dk, dv = (capi.DeviceArray.from_numpy(x) for x in (q, k, v))
+    out = capi.DeviceArray.from_numpy(np.full_like(q, 7))
+    dn = None if lengths is None else capi.DeviceArray.from_numpy(np.asarray(lengths, np.int32))
+    desc = capi.window_attention_desc(*q.shape[:2], k.shape[1], q.shape[2], k.shape[2], q.shape[3], window=window, sinks=sinks,
+                                      scale=scale, lengths=None if dn is None else dn.ptr)
+    ws = capi.window_attention_workspace(desc) if workspace else None
+    capi.window_attention(dq.ptr, dk.ptr, dv.ptr, out.ptr, desc, workspace=ws)
+    capi.synchronize()
+    return out.numpy()
+
+
+def check(out, q, k, v, lengths, window, sinks, scale, heads=None):
+    """Against the plain form and its bound; of many heads those named."""
+    share = q.shape[1] // k.shape[1]
+    for b, h in heads or [(b, h) for b in range(q.shape[0]) for h in range(q.shape[1])]:
+        key = np.s_[b:b + 1, h // share:h // share + 1]
+        expected, bound = cases.attention(q[b:b + 1, h:h + 1], k[key], v[key], lengths[b:b + 1], window or None, sinks, scale)
+        off = np.abs(out[b:b + 1, h:h + 1].astype(float) - expected)
+        assert (off <= bound).all(), f"head {b}, {h}: off by up to {np.nanmax(off / np.maximum(bound, 1e-300)):.3g} of the bound"
+
+
+# (batch, heads, kv_heads, rows, cols, features), with a workspace or not: the
+# stream, 16 rows whole and over splits, packed tiles of every block size.
+FORMS = [
+    ((1, 2, 1, 2, 700, 64), True),
+    ((1, 2, 1, 20, 200, 64), False),
+    ((1, 2, 1, 20, 200, 128), False),
+    ((1, 2, 1, 20, 900, 128), True),
+    ((1, 1, 1, 1030, 1100, 64), True),
+    ((43, 2, 2, 257, 260, 32), True),
+    ((128, 1, 1, 257, 257, 80), True),
+]
+
+
+def form_heads(shape):
+    batch, heads = shape[:2]
+    return sorted({(0, 0), (batch // 2, heads - 1), (batch - 1, 0)})
+
+
+# ------------------------------------------------------------------ values of keys
+@pytest.mark.parametrize("far", [(0, 2.0 ** 60), (0, 1e20), (0, 1e30), (2.0 ** -70, 2.0 ** 76), (1.0, 2.0 ** 126), (0, 1e-30)],
+                         ids=str)
+@pytest.mark.parametrize("shape,workspace", FORMS, ids=str)
+def test_values_far_apart(capi, shape, workspace, far):
+    """Keys of one magnitude beside keys of another: a weight counts in the softmax's sum
+    whatever its key's values are. (2^126 in one key alone, so that sums stay finite.)"""
+    batch, heads, kv, rows, cols, d = shape
+    rng = np.random.default_rng(61)
+    q, k = f32(rng, batch, heads, rows, d), f32(rng, batch, kv, cols, d)
+    v = np.sign(f32(rng, batch, kv, cols, d)) * np.float32(far[0])
+    large = slice(1, None, 2) if far[1] < 1e36 else slice(1, 2)
+    v[:, :, large] = np.abs(f32(rng, *v[:, :, large].shape)).clip(0.1, 2) * np.float32(far[1] / 2)
+    for scale in (0.0, d ** -0.5):
+        out = window(capi, q, k, v, scale=scale, workspace=workspace)
+        check(out, q, k, v, [cols] * batch, 0, 0, scale, form_heads(shape))
+
+
+@pytest.mark.parametrize("workspace", [False, True])
+def test_small_weights_beside_a_huge_value(capi, workspace):
+    """One key of values 2^126 and many of 1 whose weights are 2^-15 of its: together
+    they are a quarter of the sum."""
+    n, d = 8192, 16
+    q, k, v = (np.zeros((1, 1, r, d), np.float32) for r in (16, n, n))
+    q[..., 0], k[:, :, 0, 0], v[...] = 1, 15, 1
+    v[:, :, 0] = 2.0 ** 126
+    scale = float(np.float32(np.log(2)))
+    out = window(capi, q, k, v, scale=scale, workspace=workspace)
+    check(out, q, k, v, [n], 0, 0, scale)
+
+
+def test_a_zero_valued_keys_weight(capi):
+    """The weight of a key whose values are zero is as exact as that of any other.
+
+    Two keys, of zeros and of ones, at scores of +a and -a in units of log2, a below 1 and of
+    20 bits (held exactly): the output is w_b / (w_a + w_b). A score takes three roundings
+    (the scale, log2 e, the product) of at most EPS, of both keys together 6 ln2 EPS of the
+    quotient of the weights; the difference from the maximum, below 4, 4 ln2 EPS; two
+    exponentials 4 EPS; the halves of w_b 4 EPS; the sum, its reciprocal and two products
+    4 EPS: 19 EPS of the output."""
+    rng = np.random.default_rng(62)
+    d, scale = 16, float(np.float32(np.log(2)))
+    q, k, v = (np.zeros((1, h, r, d), np.float32) for h, r in ((4096, 1), (1, 2), (1, 2)))
+    q[..., 0] = rng.integers(1, 2 ** 20, q.shape[:3]) / 2 ** 20
+    k[:, :, 0, 0], k[:, :, 1, 0], v[:, :, 1] = 1, -1, 1
+    out = window(capi, q, k, v, scale=scale, workspace=False)
+    s = q[..., :1].astype(float) * scale
+    expected = np.exp(-s) / (np.exp(-s) + np.exp(s))
+    assert (np.abs(out - expected) <= 19 * EPS * expected).all(), np.abs(out / expected - 1).max() / EPS
+
+
+@pytest.mark.parametrize("rows", [16, 1030])
+@pytest.mark.parametrize("workspace", [False, True])
+def test_an_outlier_of_one_feature(capi, rows, workspace):
+    """One feature of one key 2^18 above everything else, judged feature by feature.
+
+    What the matrix form adds to a float32 kernel's error: weights are float16 halves of
+    numbers whose largest, the product of a weight and a key's largest value A, is above
+    2^10, so each is off by at most 2^-25, 2^-35 A over its key's own scale, and meets values
+    below twice that scale: 2^-34 A for each key that is seen."""
+    n, d = rows + 60, 64
+    rng = np.random.default_rng(63)
+    q, k, v = f32(rng, 1, 1, rows, d), f32(rng, 1, 1, n, d), f32(rng, 1, 1, n, d)
+    v[0, 0, 30, 5] = 2.0 ** 18
+    out = window(capi, q, k, v, workspace=workspace)
+    check(out, q, k, v, [n], 0, 0, d ** -0.5)
+    v[..., 5] = out[..., 5] = 0
+    expected, bound = cases.attention(q, k, v, [n], None, 0, d ** -0.5)
+    assert (np.abs(out - expected) <= bound + n * 2.0 ** -34 * 2.0 ** 18).all()
+
+
+@pytest.mark.parametrize("large", [1e4, 1e7, 1e12])
+@pytest.mark.parametrize("shape,workspace", FORMS, ids=str)
+def test_scores_without_fractions(capi, shape, workspace, large):
+    """Scores so far apart that each row takes the value of one key alone, that of the
+    largest product of small whole numbers: exact, where float32 scores have lost their
+    fractions too, and however the maxima rise along the keys."""
+    batch, heads, kv, rows, cols, d = shape
+    rng = np.random.default_rng(66)
+    q, k, v = np.zeros((batch, heads, rows, d), np.float32), np.zeros((batch, kv, cols, d), np.float32), f32(rng, batch, kv, cols, d)
+    q[..., 0] = large
+    k[..., 0] = np.arange(1, cols + 1) + 100 * (np.arange(cols) % 7 == 0)
+    out = window(capi, q, k, v, scale=1.0, workspace=workspace)
+    for b, h in form_heads(shape):
+        best = np.maximum.accumulate(k[b, h // (heads // kv), :, 0])
+        at = np.searchsorted(best, best[cols - rows:])  # the first key with it
+        expected = v[b, h // (heads // kv), at]
+        # The weight of one key alone is 1, its value held in halves.
+        assert (np.abs(out[b, h] - expected) <= 2.0 ** -21 * np.abs(v[b, h // (heads // kv), at]).max(-1, keepdims=True)).all()
