@@ -343,16 +343,19 @@ struct PromptRows {
       // By the tile's largest exponent no row's product passes 2^15: mostly.
       if (__any(first | (most > kFar) | (most + most_exp + rest[x] > kMost))) [[unlikely]]
         move(s[x], x, first, most, value_exp);
+      // A tile's weights are summed by pairs: one by one they would make a chain of a
+      // quarter of the keys, which loses small weights beside a large one.
+      float sum[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float4_t unit = *reinterpret_cast<const float4_t*>(&value_unit[16 * i + 4 * g]);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          s[x][i][v] = __builtin_amdgcn_exp2f(s[x][i][v]);
-          l[x] += s[x][i][v];
-          s[x][i][v] *= unit[v];
-        }
+        for (int v = 0; v < 4; ++v) s[x][i][v] = __builtin_amdgcn_exp2f(s[x][i][v]);
+        sum[i] = (s[x][i][0] + s[x][i][1]) + (s[x][i][2] + s[x][i][3]);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s[x][i][v] *= unit[v];
       }
+      l[x] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       if (__any(rest[x] != 0.F)) [[unlikely]] {
 #pragma unroll
         for (int i = 0; i < 4; ++i)

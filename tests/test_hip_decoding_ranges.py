@@ -1,5 +1,6 @@
 """GPU tests of the decoding operators over the ranges of their numbers: values of
-keys side by side that are zero, tiny, far apart or near float32's largest.
+keys side by side that are zero, tiny, far apart or near float32's largest, and
+weights that a long sum could lose.
 
 Each call of more than eight rows of a key head runs in all of its forms: without a
 workspace, with its keys split over blocks, and from packed tiles."""
@@ -159,3 +160,26 @@ def test_scores_without_fractions(capi, shape, workspace, large):
         expected = v[b, h // (heads // kv), at]
         # The weight of one key alone is 1, its value held in halves.
         assert (np.abs(out[b, h] - expected) <= 2.0 ** -21 * np.abs(v[b, h // (heads // kv), at]).max(-1, keepdims=True)).all()
+
+
+# ------------------------------------------------------------------ long sums
+@pytest.mark.parametrize("workspace", [False, True])
+def test_a_long_sum_of_small_weights(capi, workspace):
+    """A weight of 1 and 32767 of just under half a step of it: a lane that added them one
+    by one would lose its quarter of them, 8192 half steps, where the sums of
+    sixteen lanes and more that the bound counts lose far less."""
+    n, d = 32768, 16
+    q, k, v = (np.zeros((1, 1, r, d), np.float32) for r in (16, n, n))
+    q[..., 0], k[:, :, 0, 0], v[:, :, 0] = 1, 24.1, 1
+    scale = float(np.float32(np.log(2)))
+    out = window(capi, q, k, v, scale=scale, workspace=workspace)
+    check(out, q, k, v, [n], 0, 0, scale)
+
+
+def test_a_causal_prompt_of_thousands(capi):
+    rng = np.random.default_rng(64)
+    q, k, v = (f32(rng, 1, 1, 5000, 64) for _ in range(3))
+    out = window(capi, np.ascontiguousarray(q[:, :, -16:]), k, v, workspace=False)
+    check(out, q[:, :, -16:], k, v, [5000], 0, 0, 0.125)
+    out = window(capi, np.ascontiguousarray(q[:, :, -1100:]), k, v)
+    check(out[:, :, :20], q[:, :, -1100:-1080], k[:, :, :-1080], v[:, :, :-1080], [3920], 0, 0, 0.125)
