@@ -14,10 +14,9 @@
 // the sum, in three bfloat16 parts of 24 bits.
 //
 // Weights. The outputs are sums of (p_j step_jG) (c_j - 7.5) and, apart from the
-// codes, of p_j mid_jG. With e_j the exponent of token j's largest low or step, the running
-// maximum M is that of x_j + e_j (x the score in units of log2): p_j = 2^(x_j - M
-// + 14) makes p_j step_jG at most 2^15, which two halves hold to 22 bits, and of a
-// row only what it sees decides M.
+// codes, of p_j mid_jG. With e_j the exponent of token j's largest low or step, RowBase
+// keeps p_j 2^e_j, and so p_j step_jG, in the range of two halves, which hold it to 22
+// bits; of a row only what it sees decides, and the softmax's sum is of p_j alone.
 //
 // Layout. A wave takes 16 or 4 rows of a key head and tiles of 32 tokens, with a
 // state of its own; the four waves of a block are joined in LDS, key splits by
@@ -243,7 +242,9 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
     __syncthreads();
 
     acc_t o[kT];
-    float mid[kGroups], m = neg_inf, l = 0.F;
+    float mid[kGroups], l = 0.F;
+    RowBase weights;
+    weights.start();
 #pragma unroll
     for (int y = 0; y < kT; ++y) o[y] = acc_t{0.F, 0.F, 0.F, 0.F};
 #pragma unroll
@@ -272,8 +273,8 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
             mine.value_step[y][k] = step;
             mine.value_mid[y][k] = fmaf(7.5F, step, __uint_as_float(value_scale[y] & 0xffff0000U));
           }
-          // Not below 2^-90, so that the sum of the weights stays finite.
-          mine.value_exp[k] = static_cast<float>(max(static_cast<int>(finite >> 23), 37) - 127);
+          // Not below 2^-100, so that what makes up for it stays finite.
+          mine.value_exp[k] = static_cast<float>(max(static_cast<int>(finite >> 23) + 1, 27) - 127);
         }
       }
       load_value_scales(i + 4);
@@ -333,29 +334,46 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
           hidden |= (in ? 0U : 1U) << k;
         }
       }
-      float top = m;
+      auto row = [](float y) {
+        if constexpr (kRows == 4) y = shares_max(y);
+        return across_max(y);
+      };
+      auto product = [&] {
+        float high = neg_inf;
 #pragma unroll
-      for (int k = 0; k < kTokens; k += 2) {
-        const float2v_t add = *reinterpret_cast<const float2v_t*>(&mine.value_exp[token(k)]);
-        top = fmaxf(fmaxf(top, x[k] + add[0]), x[k + 1] + add[1]);
-      }
-      if constexpr (kRows == 4) top = shares_max(top);
-      top = across_max(top);
-      if (__any(top > m)) {
-        const float f = __builtin_amdgcn_exp2f(m - (top == neg_inf ? 0.F : top));
-        l *= f;
-#pragma unroll
-        for (int y = 0; y < kT; ++y) o[y] *= f;
-#pragma unroll
-        for (int y = 0; y < kGroups; ++y) mid[y] *= f;
-        m = top;
-      }
-      const float shift = m == neg_inf ? 0.F : m - 14.F;
+        for (int k = 0; k < kTokens; k += 2) {
+          const float2v_t add = *reinterpret_cast<const float2v_t*>(&mine.value_exp[token(k)]);
+          high = fmaxf(fmaxf(high, x[k] + add[0]), x[k + 1] + add[1]);
+        }
+        return high;
+      };
+      float most = neg_inf;
 #pragma unroll
       for (int k = 0; k < kTokens; ++k) {
-        x[k] = __builtin_amdgcn_exp2f(x[k] - shift);
+        x[k] -= weights.base;
+        most = fmaxf(most, x[k]);
+      }
+      if (__any(weights.see(most, product()))) [[unlikely]] {
+        auto each = [&](auto&& change) {
+#pragma unroll
+          for (int k = 0; k < kTokens; ++k) x[k] = change(x[k]);
+        };
+        const int scale = weights.move(l, row, each, product);
+        if (__any(scale != 0)) {
+#pragma unroll
+          for (int y = 0; y < kT; ++y)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) o[y][v] = ldexpf(o[y][v], scale);
+#pragma unroll
+          for (int y = 0; y < kGroups; ++y) mid[y] = ldexpf(mid[y], scale);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kTokens; ++k) {
+        x[k] = __builtin_amdgcn_exp2f(x[k]);
         l += x[k];
       }
+      const bool scaled = __any(weights.rest != 0.F);
 
       // A group's weights and its part of the outputs.
       for_groups<kGroups>([&]<int kG>() {
@@ -379,9 +397,16 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
         }
         float weight[kTokens];
 #pragma unroll
-        for (int k = 0; k < kTokens; ++k) {
-          weight[k] = x[k] * step[k];
-          mid[kG] = fmaf(x[k], mids[k], mid[kG]);
+        for (int k = 0; k < kTokens; ++k) weight[k] = x[k] * step[k];
+        if (scaled) [[unlikely]] {
+#pragma unroll
+          for (int k = 0; k < kTokens; ++k) {
+            weight[k] = ldexpf(weight[k], exponent(weights.rest));
+            mid[kG] += ldexpf(x[k] * mids[k], exponent(weights.rest));
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < kTokens; ++k) mid[kG] = fmaf(x[k], mids[k], mid[kG]);
         }
         word4_t w_hi, w_lo;
         if constexpr (kRows == 16) {
@@ -421,8 +446,10 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
     l = across_sum(l);
 #pragma unroll
     for (int y = 0; y < kGroups; ++y) mid[y] = across_sum(mid[y]);
+    weights.top = across_max(weights.top);
     if constexpr (kRows == 4) {
       l = shares_sum(l);
+      weights.top = shares_max(weights.top);
 #pragma unroll
       for (int y = 0; y < kGroups; ++y) mid[y] = shares_sum(mid[y]);
 #pragma unroll
@@ -432,16 +459,17 @@ __global__ __launch_bounds__(256, D == 128 && kRows == 16 ? 2 : 3) void cache_at
     }
     __syncthreads();  // every wave is done with its part of the union
     if (q == 0) {
+      const int whole = weights.whole(), back = -exponent(weights.rest) - whole;
 #pragma unroll
       for (int y = 0; y < kT; ++y) {
         float4_t part;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) part[v] = fmaf(o[y][v], kCodeUnit, mid[y / 2]);
+        for (int v = 0; v < 4; ++v) part[v] = ldexpf(fmaf(o[y][v], kCodeUnit, mid[y / 2]), back);
         *reinterpret_cast<float4_t*>(&shared.part[wave][column][16 * y + 4 * g]) = part;
       }
       if (g == 0) {
-        part_m[wave][column] = m;
-        part_l[wave][column] = l;
+        part_m[wave][column] = weights.most();
+        part_l[wave][column] = ldexpf(l, -whole);
       }
     }
     __syncthreads();

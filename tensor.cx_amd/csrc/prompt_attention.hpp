@@ -53,13 +53,6 @@ namespace tcx {
 constexpr int kMostKeyField = 253;   // its inverse is a normal number
 constexpr int kMostValueField = 245; // 2^118
 constexpr int kLeastExp = 141 - kMostValueField;  // of e_j
-// A row's base is such that its largest product of a weight and 2^e_j is 2^kAim when it
-// is set, as far as that leaves its largest weight between 2^-kNear and 2^kNear. The
-// five powers of two up to 2^kMost, which float16 still holds, are what scores can rise
-// before it is set anew (with three 241 us in place of 230 for 8192 rows, 16 heads of 64
-// features, window 2048).
-constexpr float kAim = 11.F, kMost = 15.99F, kNear = 60.F, kFar = 64.F;
-constexpr float kWhole = 8388608.F;  // from here on float32 has no fractions
 
 // The slot of chunk c of 8 features of key row j, and of the 16 bytes of 8 keys at
 // chunk c of value row f: xored so that the lanes of a fragment meet different
@@ -161,9 +154,6 @@ __device__ __forceinline__ void pack_values(const float4_t (&in)[4], int h, int 
   }
 }
 
-// A whole number as an exponent (past those of float32 it makes no difference).
-__device__ __forceinline__ int exponent(float x) { return static_cast<int>(fminf(fmaxf(x, -400.F), 400.F)); }
-
 // A wave's 16 kQ rows: queries as B operands, the running maxima, sums and outputs.
 template <int D, int kQ>
 struct PromptRows {
@@ -172,8 +162,8 @@ struct PromptRows {
   float row_factor[kQ];
   int p_row[kQ];
   acc_t o[kQ][kT];  // feature 4 (r % (D / 4)) + r / (D / 4) of query n at r = 16 i + 4 g + v
-  float base[kQ], rest[kQ];
-  float top[kQ], l[kQ];  // the largest score from base on, and the sum of this lane's weights
+  RowBase weights[kQ];
+  float l[kQ];  // the sum of this lane's weights
   int first_row, last_row;  // the keys of the wave's first and last queries
   int row0, n16, g;
 
@@ -214,9 +204,8 @@ struct PromptRows {
       }
 #pragma unroll
       for (int i = 0; i < kT; ++i) o[x][i] = acc_t{0.F, 0.F, 0.F, 0.F};
-      base[x] = l[x] = 0.F;
-      top[x] = -__builtin_inff();
-      rest[x] = 0.F;
+      weights[x].start();
+      l[x] = 0.F;
     }
   }
 
@@ -228,7 +217,7 @@ struct PromptRows {
     return j0 + 63 <= first_row && (a.window == 0 || j0 > last_row - a.window || j0 + 63 < a.sinks);
   }
 
-  // The largest of a tile's s + exponent.
+  // The largest of this lane's s + exponent of a tile.
   __device__ __forceinline__ float most_product(const acc_t (&s)[4], const float* value_exp) const {
     float most = -__builtin_inff();
 #pragma unroll
@@ -237,49 +226,24 @@ struct PromptRows {
 #pragma unroll
       for (int v = 0; v < 4; ++v) most = fmaxf(most, s[i][v] + add[v]);
     }
-    return across_max(most);
+    return most;
   }
-  // Moves the base of the rows x that need it. Rows that do not stay as they are to the
-  // bit: another row's keys, and hidden ones, may be why this is called.
-  __device__ __forceinline__ void move(acc_t (&s)[4], int x, bool first, float most, const float* value_exp) {
-    const float high = most_product(s, value_exp) + rest[x];
-    const bool past = first || high > kMost, need = most > -__builtin_inff() && (past || most > kFar);
-    float to = base[x], aim = rest[x], gone = 0.F;
-    bool plain = true, far = false;
-    if (need) {
-      const float all = past ? ceilf(high) - kAim : 0.F, peak = ceilf(top[x]);
-      const float by = fminf(fmaxf(all, peak - kNear), peak + kNear);
-      to += by;
-      far = fabsf(to) >= kWhole;
-      if (far) to = base[x] + top[x];  // the largest score itself, which the others are then rounded like
-      plain = by == all && !far;
-      gone = to - base[x];
-    }
-    if (__any(!plain)) [[unlikely]] {
+  // Moves the base of row x of the lanes that need it.
+  __device__ __forceinline__ void move(acc_t (&s)[4], int x, const float* value_exp) {
+    auto each = [&](auto&& change) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) s[i][v] = far ? (s[i][v] + base[x]) - to : s[i][v] - gone;
-      top[x] = far ? 0.F : top[x] - gone;
-      gone = 0.F;
-      const float product = most_product(s, value_exp);
-      if (!plain && (first || product + rest[x] > kMost)) aim = kAim - ceilf(product);
-    }
-    top[x] -= gone;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) s[i][v] -= gone;
-    l[x] = ldexpf(l[x], exponent(base[x] - to));
-    const int scale = first ? 0 : exponent((base[x] - to) + (aim - rest[x]));
+        for (int v = 0; v < 4; ++v) s[i][v] = change(s[i][v]);
+    };
+    const int scale = weights[x].move(l[x], [](float y) { return across_max(y); }, each,
+                                      [&] { return most_product(s, value_exp); });
     if (__any(scale != 0)) {
 #pragma unroll
       for (int i = 0; i < kT; ++i)
 #pragma unroll
         for (int v = 0; v < 4; ++v) o[x][i][v] = ldexpf(o[x][i][v], scale);
     }
-    base[x] = to;
-    rest[x] = aim;
   }
 
   // A tile's weights, as B operands of the P V products. key_of(k): the key at
@@ -316,7 +280,7 @@ struct PromptRows {
 #pragma unroll
       for (int x = 0; x < kQ; ++x)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) s[x][i][v] = fmaf(s[x][i][v], row_factor[x] * factor[v], -base[x]);
+        for (int v = 0; v < 4; ++v) s[x][i][v] = fmaf(s[x][i][v], row_factor[x] * factor[v], -weights[x].base);
     }
     if (!whole) {
 #pragma unroll
@@ -337,12 +301,9 @@ struct PromptRows {
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int v = 0; v < 4; ++v) most = fmaxf(most, s[x][i][v]);
-      most = across_max(most);
-      const bool first = top[x] == neg_inf;
-      top[x] = fmaxf(top[x], most);
-      // By the tile's largest exponent no row's product passes 2^15: mostly.
-      if (__any(first | (most > kFar) | (most + most_exp + rest[x] > kMost))) [[unlikely]]
-        move(s[x], x, first, most, value_exp);
+      // The tile's largest exponent shows of most tiles that no product passes the limit.
+      if (__any(weights[x].see(most, most + most_exp))) [[unlikely]]
+        move(s[x], x, value_exp);
       // A tile's weights are summed by pairs: one by one they would make a chain of a
       // quarter of the keys, which loses small weights beside a large one.
       float sum[4];
@@ -356,11 +317,11 @@ struct PromptRows {
         for (int v = 0; v < 4; ++v) s[x][i][v] *= unit[v];
       }
       l[x] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      if (__any(rest[x] != 0.F)) [[unlikely]] {
+      if (__any(weights[x].rest != 0.F)) [[unlikely]] {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int v = 0; v < 4; ++v) s[x][i][v] = ldexpf(s[x][i][v], exponent(rest[x]));
+          for (int v = 0; v < 4; ++v) s[x][i][v] = ldexpf(s[x][i][v], exponent(weights[x].rest));
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -429,6 +390,7 @@ struct PromptRows {
 #pragma unroll
     for (int x = 0; x < kQ; ++x) {
       l[x] = across_sum(l[x]);
+      weights[x].top = across_max(weights[x].top);
       const int r = row0 + 16 * x + n16;
       if (r > r1) continue;
       const RowPlace place = row_place(a, kv, r);
@@ -437,8 +399,7 @@ struct PromptRows {
                        ? a.out + b * a.out_stride[0] + place.head * a.out_stride[1] + place.query * a.out_stride[2]
                        : a.part + row * a.features;
       // Outputs are held times 2^rest, and 2^14 of V'.
-      const int whole = top[x] > -__builtin_inff() ? exponent(ceilf(top[x])) : 0;
-      const int back = -14 - exponent(rest[x]) - (a.splits > 1 ? whole : 0);
+      const int whole = weights[x].whole(), back = -14 - exponent(weights[x].rest) - (a.splits > 1 ? whole : 0);
       const float by = a.splits > 1 ? 1.F : l[x] == 0.F ? 0.F : 1.F / l[x];
       auto result = [&](float y) { return ldexpf(y * by, back); };
       if constexpr (kQuads % 16 == 0) {
@@ -462,7 +423,7 @@ struct PromptRows {
           }
       }
       if (a.splits > 1 && g == 0) {
-        a.part_ml[2 * row] = top[x] > -__builtin_inff() ? base[x] + static_cast<float>(whole) : top[x];
+        a.part_ml[2 * row] = weights[x].most();
         a.part_ml[2 * row + 1] = ldexpf(l[x], -whole);
       }
     }

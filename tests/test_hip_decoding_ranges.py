@@ -1,6 +1,6 @@
 """GPU tests of the decoding operators over the ranges of their numbers: values of
-keys side by side that are zero, tiny, far apart or near float32's largest, and
-weights that a long sum could lose.
+keys side by side that are zero, tiny, far apart or near float32's largest, weights
+that a long sum could lose.
 
 Each call of more than eight rows of a key head runs in all of its forms: without a
 workspace, with its keys split over blocks, and from packed tiles."""
@@ -39,6 +39,17 @@ def window(capi, q, k, v, *, window=0, sinks=0, scale=None, lengths=None, worksp
                                       scale=scale, lengths=None if dn is None else dn.ptr)
     ws = capi.window_attention_workspace(desc) if workspace else None
     capi.window_attention(dq.ptr, dk.ptr, dv.ptr, out.ptr, desc, workspace=ws)
+    capi.synchronize()
+    return out.numpy()
+
+
+def cached(capi, q, keys, values, lengths, *, window=0, sinks=0, scale=None, workspace=True):
+    dq, dk, dv, dn = (capi.DeviceArray.from_numpy(x) for x in (q, keys, values, np.asarray(lengths, np.int32)))
+    out = capi.DeviceArray.from_numpy(np.full_like(q, 7))
+    desc = capi.window_attention_desc(*q.shape[:2], keys.shape[1], q.shape[2], keys.shape[2], q.shape[3], window=window,
+                                      sinks=sinks, scale=scale, lengths=dn.ptr)
+    ws = capi.window_attention_workspace(desc, cache=True) if workspace else None
+    capi.cache4_attention(dq.ptr, dk.ptr, dv.ptr, out.ptr, desc, workspace=ws)
     capi.synchronize()
     return out.numpy()
 
@@ -142,27 +153,6 @@ def test_an_outlier_of_one_feature(capi, rows, workspace):
     assert (np.abs(out - expected) <= bound + n * 2.0 ** -34 * 2.0 ** 18).all()
 
 
-@pytest.mark.parametrize("large", [1e4, 1e7, 1e12])
-@pytest.mark.parametrize("shape,workspace", FORMS, ids=str)
-def test_scores_without_fractions(capi, shape, workspace, large):
-    """Scores so far apart that each row takes the value of one key alone, that of the
-    largest product of small whole numbers: exact, where float32 scores have lost their
-    fractions too, and however the maxima rise along the keys."""
-    batch, heads, kv, rows, cols, d = shape
-    rng = np.random.default_rng(66)
-    q, k, v = np.zeros((batch, heads, rows, d), np.float32), np.zeros((batch, kv, cols, d), np.float32), f32(rng, batch, kv, cols, d)
-    q[..., 0] = large
-    k[..., 0] = np.arange(1, cols + 1) + 100 * (np.arange(cols) % 7 == 0)
-    out = window(capi, q, k, v, scale=1.0, workspace=workspace)
-    for b, h in form_heads(shape):
-        best = np.maximum.accumulate(k[b, h // (heads // kv), :, 0])
-        at = np.searchsorted(best, best[cols - rows:])  # the first key with it
-        expected = v[b, h // (heads // kv), at]
-        # The weight of one key alone is 1, its value held in halves.
-        assert (np.abs(out[b, h] - expected) <= 2.0 ** -21 * np.abs(v[b, h // (heads // kv), at]).max(-1, keepdims=True)).all()
-
-
-# ------------------------------------------------------------------ long sums
 @pytest.mark.parametrize("workspace", [False, True])
 def test_a_long_sum_of_small_weights(capi, workspace):
     """A weight of 1 and 32767 of just under half a step of it: a lane that added them one
@@ -183,3 +173,76 @@ def test_a_causal_prompt_of_thousands(capi):
     check(out, q[:, :, -16:], k, v, [5000], 0, 0, 0.125)
     out = window(capi, np.ascontiguousarray(q[:, :, -1100:]), k, v)
     check(out[:, :, :20], q[:, :, -1100:-1080], k[:, :, :-1080], v[:, :, :-1080], [3920], 0, 0, 0.125)
+
+
+@pytest.mark.parametrize("large", [1e4, 1e7, 1e12])
+@pytest.mark.parametrize("shape,workspace", FORMS, ids=str)
+def test_scores_without_fractions(capi, shape, workspace, large):
+    """Scores so far apart that each row takes the value of one key alone, that of the
+    largest product of small whole numbers: exact, where float32 scores have lost their
+    fractions too, and however the maxima rise along the keys."""
+    batch, heads, kv, rows, cols, d = shape
+    rng = np.random.default_rng(66)
+    q, k, v = np.zeros((batch, heads, rows, d), np.float32), np.zeros((batch, kv, cols, d), np.float32), f32(rng, batch, kv, cols, d)
+    q[..., 0] = large
+    k[..., 0] = np.arange(1, cols + 1) + 100 * (np.arange(cols) % 7 == 0)
+    out = window(capi, q, k, v, scale=1.0, workspace=workspace)
+    for b, h in form_heads(shape):
+        best = np.maximum.accumulate(k[b, h // (heads // kv), :, 0])
+        at = np.searchsorted(best, best[cols - rows:])  # the first key with it
+        expected = v[b, h // (heads // kv), at]
+        # The weight of one key alone is 1, its value held in halves.
+        assert (np.abs(out[b, h] - expected) <= 2.0 ** -21 * np.abs(v[b, h // (heads // kv), at]).max(-1, keepdims=True)).all()
+
+
+@pytest.mark.parametrize("heads,rows", [(1, 1), (4, 1), (2, 16)])
+@pytest.mark.parametrize("features", [32, 64, 128])
+@pytest.mark.parametrize("workspace", [False, True])
+def test_small_cached_weights_beside_a_huge_value(capi, features, heads, rows, workspace):
+    """The same in the 4-bit cache, of values that it holds exactly."""
+    n = 8192
+    q, k = np.zeros((1, heads, rows, features), np.float32), np.zeros((1, 1, n, features), np.float32)
+    v = np.ones((1, 1, n, features), np.float32)
+    q[..., :32] = 1 / 32
+    k[:, :, 0, :32], v[:, :, 0] = 15, 2.0 ** 126
+    scale = float(np.float32(np.log(2)))
+    keys, values = cases.cache_rows(k), cases.cache_rows(v)
+    np.testing.assert_array_equal(cases.cache_values(values, features), v)
+    out = cached(capi, q, keys, values, [n], scale=scale, workspace=workspace)
+    check(out, q, k, v, [n], 0, 0, scale)
+
+
+@pytest.mark.parametrize("far", [(0, 2.0 ** 66), (0, 1e30), (2.0 ** -60, 2.0 ** 76), (0, 1e-20)], ids=str)
+@pytest.mark.parametrize("heads,rows", [(4, 1), (2, 16)])
+@pytest.mark.parametrize("features", [32, 64, 128])
+def test_cached_values_far_apart(capi, features, heads, rows, far):
+    rng = np.random.default_rng(65)
+    n = 500
+    q, k, v = f32(rng, 1, heads, rows, features), f32(rng, 1, 1, n, features), f32(rng, 1, 1, n, features)
+    v[:, :, ::2] *= np.float32(far[0])
+    v[:, :, 1::2] *= np.float32(far[1])
+    keys, values = cases.cache_rows(k), cases.cache_rows(v)
+    kk, vv = cases.cache_values(keys, features), cases.cache_values(values, features)
+    for scale in (0.0, features ** -0.5):
+        check(cached(capi, q, keys, values, [n], scale=scale), q, kk, vv, [n], 0, 0, scale)
+
+
+@pytest.mark.parametrize("large", [1e4, 1e7, 1e12])
+@pytest.mark.parametrize("heads,rows", [(1, 1), (4, 1), (2, 16)])
+@pytest.mark.parametrize("features", [32, 64, 128])
+def test_cached_scores_without_fractions(capi, features, heads, rows, large):
+    """The same: tokens of whole numbers below 256, which the cache holds exactly."""
+    n = 700
+    rng = np.random.default_rng(67)
+    q, k, v = np.zeros((1, heads, rows, features), np.float32), np.zeros((1, 1, n, features), np.float32), f32(rng, 1, 1, n, features)
+    q[..., :32] = np.float32(large) / 32
+    k[...] = (1 + np.arange(n) // 3 % 200 + 20 * (np.arange(n) % 7 == 0))[:, None]
+    keys, values = cases.cache_rows(k), cases.cache_rows(v)
+    np.testing.assert_array_equal(cases.cache_values(keys, features), k)
+    out = cached(capi, q, keys, values, [n], scale=1.0)
+    vv, best = cases.cache_values(values, features)[0, 0], k[0, 0, :, 0]
+    for i in range(rows):
+        seen = best[:n - rows + i + 1]
+        expected = vv[:len(seen)][seen == seen.max()].mean(0)
+        # Equal weights, products in halves, sums of a few.
+        assert (np.abs(out[0, :, i] - expected) <= 2.0 ** -20 * np.abs(vv).max()).all()
