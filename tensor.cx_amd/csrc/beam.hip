@@ -140,11 +140,14 @@ __global__ __launch_bounds__(256, kEach == 32 ? 3 : 4) void beam_part_kernel(Bea
     if (lane == 0) wave_top[wave] = top;
     const std::uint32_t bound = block_bound(most, a.count, wave_key);
     top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
-    const float shift = top == -__builtin_inff() ? 0.F : top * kLog2e;
+    // Differences from the maximum, which are as good as the logits, and 0 where those
+    // are equal, float32's lowest value too. (top log2 e, rounded, would be a factor of
+    // the sum: 4e-5 of the scores for logits near 1000.)
+    const float shift = top == -__builtin_inff() ? 0.F : top;
     // Four sums by turns: with the wave's and the block's a chain of at most kEach / 4 + 8.
     float part_sum[4] = {0.F, 0.F, 0.F, 0.F};
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) part_sum[e % 4] += __builtin_amdgcn_exp2f(fmaf(value[e], kLog2e, -shift));
+    for (int e = 0; e < kEach; ++e) part_sum[e % 4] += __builtin_amdgcn_exp2f((value[e] - shift) * kLog2e);
     float sum = wave_sum((part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]));
     // With a NaN in this thread's share, its largest number says nothing of the order.
     const bool lost = __any(!(part_sum[0] + part_sum[1] + part_sum[2] + part_sum[3] < __builtin_inff()));

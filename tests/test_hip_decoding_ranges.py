@@ -1,6 +1,6 @@
 """GPU tests of the decoding operators over the ranges of their numbers: values of
 keys side by side that are zero, tiny, far apart or near float32's largest, weights
-that a long sum could lose.
+that a long sum could lose, logits with offsets and at float32's lowest value.
 
 Each call of more than eight rows of a key head runs in all of its forms: without a
 workspace, with its keys split over blocks, and from packed tiles."""
@@ -246,3 +246,92 @@ def test_cached_scores_without_fractions(capi, features, heads, rows, large):
         expected = vv[:len(seen)][seen == seen.max()].mean(0)
         # Equal weights, products in halves, sums of a few.
         assert (np.abs(out[0, :, i] - expected) <= 2.0 ** -20 * np.abs(vv).max()).all()
+
+
+# ------------------------------------------------------------------ beam selection
+def select(capi, logits, scores, count):
+    batch, beams, vocabulary = logits.shape
+    dx, ds = capi.DeviceArray.from_numpy(logits), capi.DeviceArray.from_numpy(scores)
+    outs = [capi.DeviceArray((batch, count)), *(capi.DeviceArray((batch, count), np.int32) for _ in range(2))]
+    ws = capi.beam_select_workspace(batch, beams, vocabulary, count)
+    capi.beam_select(dx.ptr, ds.ptr, *(o.ptr for o in outs), batch, beams, vocabulary, count, workspace=ws)
+    capi.synchronize()
+    return [o.numpy() for o in outs]
+
+
+def check_selection(got, logits, scores, count):
+    """The plain form's candidates, and their scores to half a step and 120 EPS of a
+    float32 sum. Candidates of different beams whose scores are closer than such
+    sums are may change places: the named ones' own scores have to be in order to that."""
+    want, all_of = cases.beam_best(logits, scores, count), cases.beam_candidates(logits, scores)
+    off = np.abs(got[0] - want[0])
+    assert (off <= np.abs(want[0]) * EPS + 120 * EPS).all(), (off / EPS).max()
+    named = all_of[np.arange(len(logits))[:, None], got[1], got[2]]
+    assert (np.abs(named - want[0]) <= 120 * EPS).all()
+    alone = np.diff(want[0], axis=-1, prepend=np.inf, append=-np.inf)
+    alone = (np.abs(alone[:, :-1]) > 240 * EPS) & (np.abs(alone[:, 1:]) > 240 * EPS)
+    alone[:, -1] = False  # what comes after it is not known
+    np.testing.assert_array_equal(got[1][alone], want[1][alone])
+    np.testing.assert_array_equal(got[2][alone], want[2][alone])
+    chosen = got[1].astype(np.int64) * logits.shape[2] + got[2]
+    assert all(len(np.unique(row)) == count for row in chosen)
+
+
+@pytest.mark.parametrize("offset", [20.0, -200.0, 1000.0, -1e4, 1e5])
+@pytest.mark.parametrize("shape", [(2, 3, 9000, 5), (16, 8, 40000, 4)], ids=str)
+def test_select_of_logits_with_an_offset(capi, shape, offset):
+    """A number added to a beam's logits, another for each beam, changes nothing: the
+    sum of exponentials is one of differences from the maximum."""
+    batch, beams, vocabulary, count = shape
+    rng = np.random.default_rng(71)
+    logits = 3 * f32(rng, batch, beams, vocabulary) + np.float32(offset) * (1 + f32(rng, batch, beams, 1) / 8)
+    scores = f32(rng, batch, beams)
+    check_selection(select(capi, logits, scores, count), logits, scores, count)
+
+
+@pytest.mark.parametrize("top", [1000.0, -777.7, 12345.6])
+def test_select_of_a_certain_token(capi, top):
+    """One token far above the rest has a probability of 1, and its score is the beam's."""
+    logits = np.full((1, 2, 20000), np.float32(top) - np.float32(1050), np.float32)
+    logits[0, 0, 17] = logits[0, 1, 9000] = np.float32(top)
+    got = select(capi, logits, np.array([[-1.5, -0.25]], np.float32), 2)
+    np.testing.assert_array_equal(got[0], [[-0.25, -1.5]])
+    assert got[1].tolist() == [[1, 0]] and got[2].tolist() == [[9000, 17]]
+
+
+LOWEST = np.finfo(np.float32).min
+
+
+@pytest.mark.parametrize("low", [LOWEST, np.float32(-3e38), np.float32(-2e38)], ids=str)
+@pytest.mark.parametrize("shape", [(1, 4, 32000, 8), (16, 8, 40000, 16), (1, 2, 50, 3)], ids=str)
+@pytest.mark.parametrize("kept", [0.01, 3])
+def test_select_of_logits_masked_by_the_lowest_value(capi, shape, kept, low):
+    """Tokens masked by float32's lowest value, in some parts of a row all of them: they
+    weigh nothing beside others, and are candidates after those."""
+    batch, beams, vocabulary, count = shape
+    rng = np.random.default_rng(72)
+    logits, scores = f32(rng, batch, beams, vocabulary), f32(rng, batch, beams)
+    allowed = rng.random(logits.shape) < (kept if kept < 1 else 0)
+    allowed[..., rng.permutation(vocabulary)[:3]] = True
+    logits[~allowed] = low
+    want, got = cases.beam_best(logits, scores, count), select(capi, logits, scores, count)
+    real = want[0] > -1e30
+    np.testing.assert_array_equal(got[1][real], want[1][real])
+    np.testing.assert_array_equal(got[2][real], want[2][real])
+    assert (np.abs(got[0] - want[0])[real] <= np.abs(want[0][real]) * EPS + 120 * EPS).all()
+    with np.errstate(over="ignore"):
+        np.testing.assert_allclose(got[0][~real], want[0][~real].astype(np.float32), rtol=2 * EPS)
+
+
+@pytest.mark.parametrize("value", [LOWEST, np.float32(-2.5e38), np.float32(2.5e38), -LOWEST], ids=str)
+@pytest.mark.parametrize("vocabulary", [100, 30000])
+def test_select_of_equal_far_logits(capi, vocabulary, value):
+    """All logits of a beam the same, near either end of float32: each has the probability
+    of one in the vocabulary."""
+    rng = np.random.default_rng(73)
+    logits, scores = f32(rng, 1, 3, vocabulary) / 8, np.zeros((1, 3), np.float32)
+    logits[0, 1] = value
+    got = select(capi, logits, scores, 256)
+    chosen = cases.beam_candidates(logits, scores)[0, got[1][0], got[2][0]]
+    assert np.isfinite(got[0]).all()
+    assert (np.abs(got[0][0] - chosen) <= np.abs(chosen) * EPS + 120 * EPS).all()
