@@ -8,18 +8,22 @@
 // `count` of a sequence's.
 //
 // Both steps find the first of many in the same way. Each thread takes the largest
-// of its candidates; T is the least, over the four waves, of a wave's ceil(count /
-// 4)-th largest thread maximum, so that at least count candidates are >= T. Those,
-// a few times count of them where values are in no special order, go to a list
-// in LDS and are put in order by counting those before each. Where they are too many
-// for that (long runs of equal values, such as masked tokens) the first are taken one
-// by one.
+// of its candidates (the two largest for counts above 128); T is the least, over the
+// four waves, of a wave's ceil(count / 4)-th largest of those, so that at least count
+// candidates are >= T. Those, up to twice count of them where values are in no special
+// order, go to a list in LDS and are put in order by counting those before each. Where
+// they are too many for that (long runs of equal values, such as masked tokens) the
+// first are taken one by one: by a part from its logits, by the merge from the heads
+// of the parts' lists, some 2.3 us each.
 //
 // The parts read the logits once, and hold them in registers. Measured: 128 beams of
 // 128256 logits, 65.7 MB, in 20.5 us with count 16 (a plain read takes 10.5), and
 // 9.5 for the merge; four beams of 32000 with count 4 in 4.8 and 6.7. What is left
 // above the read is the work on what was read: a block waits for its loads, then
-// for the search, the list and its order, three blocks a CU.
+// for the search, the list and its order, three blocks a CU. Eight beams of 128256:
+// count 16 in 33 us, 64 in 110, 128 in 217, 256 in 420: a sequence's merge is one
+// block's work. (A bound from the largest alone, over lists in their own order, left
+// counts of 64, 128 and 256 to be taken one by one at times: 3.9, 15 and 59 ms.)
 
 #include <algorithm>
 
@@ -43,6 +47,7 @@ struct BeamArgs {
   int beams, vocabulary, count, eos, parts;
   std::uint64_t* places;  // [batch * beams, parts, count]: the key, and the token inverted; 0: none
   float* sums;            // [batch * beams, parts, 2]: maximum, sum of exp
+  std::int32_t* heads;    // [batch * beams, parts]: of the merge of lists that are too long to be put in order
 };
 
 // Larger keys come first; NaN above every number, +0 and -0 alike. No key is 0.
@@ -58,27 +63,32 @@ __device__ __forceinline__ std::uint64_t place_of(std::uint32_t key, std::uint32
   return (static_cast<std::uint64_t>(key) << 32) | static_cast<std::uint32_t>(~token);
 }
 
-// T of the block from its threads' largest keys, to the upper 20 bits (a lower one
-// is a bound as well, and spares steps of the search). One barrier; `shared`
-// holds a word for each wave.
-__device__ __forceinline__ std::uint32_t block_bound(std::uint32_t most, int count, std::uint32_t* shared) {
+// T of the block from its threads' largest keys and, where a wave's rank is above
+// kRanked, their second largest (or 0) too; from bit kLast on (a lower one is a bound
+// as well, and spares steps of the search). One barrier; `shared` holds a word for
+// each wave.
+constexpr int kRanked = 32;
+template <int kLast>
+__device__ __forceinline__ std::uint32_t block_bound(std::uint32_t most, std::uint32_t second, int count, std::uint32_t* shared) {
   const int rank = min((count + 3) / 4, 64);
   std::uint32_t bound = 0;
-  for (int bit = 31; bit >= 12; --bit) {
-    const std::uint32_t trial = bound | (1U << bit);
-    if (__popcll(__ballot(most >= trial)) >= rank) bound = trial;
-  }
+  auto search = [&](auto&& reaching) {
+    for (int bit = 31; bit >= kLast; --bit)
+      if (reaching(bound | (1U << bit)) >= rank) bound |= 1U << bit;
+  };
+  if (rank <= kRanked) search([&](std::uint32_t key) { return __popcll(__ballot(most >= key)); });
+  else search([&](std::uint32_t key) { return __popcll(__ballot(most >= key)) + __popcll(__ballot(second >= key)); });
   if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = bound;
   __syncthreads();
   return min(min(shared[0], shared[1]), min(shared[2], shared[3]));
 }
 
 // Whether `found` of a list are put in order by counting: that takes a thread some 35
-// cycles for each pair, where taking `wanted` one by one costs some 2400 each and
-// more for `more` candidates of a thread (four beams of 32000 logits, one in a
-// hundred not masked: 245 us by counting alone, 16 so).
-__device__ __forceinline__ bool counted(int found, int listed, int wanted, int more) {
-  return found <= listed && (found + 255) / 256 * found <= wanted * (70 + 4 * more);
+// cycles for each pair, where taking `wanted` one by one costs some 2400 each, of a
+// merge 4500 (four beams of 32000 logits, one in a hundred not masked: 245 us by
+// counting alone, 16 so).
+__device__ __forceinline__ bool counted(int found, int listed, int wanted) {
+  return found <= listed && (found + 255) / 256 * found <= wanted * 70;
 }
 
 // How many of a list come before one of them.
@@ -138,7 +148,18 @@ __global__ __launch_bounds__(256, kEach == 32 ? 3 : 4) void beam_part_kernel(Bea
 #pragma unroll
     for (int offset = 32; offset > 0; offset >>= 1) top = fmaxf(top, __shfl_xor(top, offset, kWave));
     if (lane == 0) wave_top[wave] = top;
-    const std::uint32_t bound = block_bound(most, a.count, wave_key);
+    std::uint32_t second = 0;
+    if (a.count > 4 * kRanked) {
+      // (A NaN makes the largest number the second as well, and is itself above it.)
+      float first = value[0], next = -__builtin_inff();
+#pragma unroll
+      for (int e = 1; e < kEach; ++e) {
+        next = fmaxf(next, fminf(first, value[e]));
+        first = fmaxf(first, value[e]);
+      }
+      if (at(0) < n) second = logit_key(next);
+    }
+    const std::uint32_t bound = block_bound<12>(most, second, a.count, wave_key);
     top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
     // Differences from the maximum, which are as good as the logits, and 0 where those
     // are equal, float32's lowest value too. (top log2 e, rounded, would be a factor of
@@ -176,7 +197,7 @@ __global__ __launch_bounds__(256, kEach == 32 ? 3 : 4) void beam_part_kernel(Bea
     }
     std::uint64_t* out = a.places + static_cast<std::int64_t>(item) * a.count;
     const int found = listed_count, wanted = min(a.count, n);
-    if (counted(found, kListed, wanted, 0)) {
+    if (counted(found, kListed, wanted)) {
       for (int i = t; i < found; i += 256) {
         const std::uint64_t mine = listed[i];
         const int rank = count_before(found, [&](int j) { return listed[j] > mine; });
@@ -232,6 +253,13 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
   return a.logit > b.logit || (a.logit == b.logit && a.token > b.token);
 }
 
+// The candidate that thread t of 256 takes in round h. The candidates lie in lists of
+// `count`, best first: in their own order a thread would see the same ranks of every list
+// where count and 256 have a factor in common, and most threads none of the first
+// (counts of 128 and 256 put thousands above the bound). Turned by another
+// angle each round, every thread meets all ranks.
+__device__ __forceinline__ int merge_candidate(int t, int h) { return 256 * h + ((t + 37 * h) & 255); }
+
 // A block a sequence.
 __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
   constexpr int kHeld = 8;  // candidates of a thread that stay in registers
@@ -252,7 +280,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
     float score[kHeld];
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
-      const int c = min(t + 256 * h, candidates - 1);
+      const int c = min(merge_candidate(t, h), candidates - 1);
       place[h] = a.places[b * candidates + c];
       score[h] = a.scores[b * a.beams + c / each];
     }
@@ -306,15 +334,22 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
       return make(c, a.places[b * candidates + c], a.scores[b * a.beams + c / each]);
     };
     Candidate held[kHeld];
-    std::uint32_t most = 0;
+    std::uint32_t most = 0, second = 0;
+    auto rank = [&](const Candidate& mine) {
+      const auto key = static_cast<std::uint32_t>(mine.key >> 32);
+      second = max(second, min(most, key));
+      most = max(most, key);
+    };
+    const int rounds = (candidates + 255) / 256;
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
-      const int c = t + 256 * h;
+      const int c = merge_candidate(t, h);
       held[h] = c < candidates ? make(c, place[h], score[h]) : Candidate{0, 0, 0};
-      most = max(most, static_cast<std::uint32_t>(held[h].key >> 32));
+      rank(held[h]);
     }
-    for (int c = t + 256 * kHeld; c < candidates; c += 256) most = max(most, static_cast<std::uint32_t>(candidate(c).key >> 32));
-    const std::uint32_t bound = block_bound(most, a.count, wave_key);
+    for (int h = kHeld; h < rounds; ++h)
+      if (const int c = merge_candidate(t, h); c < candidates) rank(candidate(c));
+    const std::uint32_t bound = block_bound<4>(most, second, a.count, wave_key);
     auto list = [&](const Candidate& mine) {
       if (mine.key == 0 || static_cast<std::uint32_t>(mine.key >> 32) < bound) return;
       const int place = atomicAdd(&listed_count, 1);
@@ -325,7 +360,8 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
     };
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) list(held[h]);
-    for (int c = t + 256 * kHeld; c < candidates; c += 256) list(candidate(c));
+    for (int h = kHeld; h < rounds; ++h)
+      if (const int c = merge_candidate(t, h); c < candidates) list(candidate(c));
     __syncthreads();
     auto write = [&](int n, const Candidate& c) {
       a.out_scores[b * a.count + n] = static_cast<float>(key_double(c.key));
@@ -333,7 +369,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
       a.out_tokens[b * a.count + n] = static_cast<std::int32_t>(~c.token);
     };
     const int found = listed_count;
-    if (counted(found, kMerged, a.count, candidates / 256)) {
+    if (counted(found, kMerged, a.count)) {
       for (int i = t; i < found; i += 256) {
         const std::uint64_t key = listed_key[i];
         int rank = count_before(found, [&](int j) { return listed_key[j] > key; });
@@ -345,29 +381,39 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a) {
         if (rank < a.count) write(rank, mine);
       }
     } else {
-      Candidate last{0, 0, 0};
-      bool first = true;
+      // The first of all lists' heads, `count` times: a thread has the best of its lists
+      // at hand, and looks for it again when that has been taken.
+      const int lists = a.beams * a.parts;
+      std::int32_t* heads = a.heads + b * lists;
+      Candidate best{0, 0, 0};
+      int from = 0;
+      auto offer = [&](int list, const Candidate& head) {
+        if (before(head, best)) best = head, from = list;
+      };
+      for (int i = t; i < lists; i += 256) {
+        heads[i] = 0;
+        offer(i, candidate(i * a.count));
+      }
       for (int n = 0; n < a.count; ++n) {
-        Candidate best{0, 0, 0};
-        for (int c = t; c < candidates; c += 256) {
-          const Candidate mine = candidate(c);
-          if ((first || before(last, mine)) && before(mine, best)) best = mine;
-        }
+        Candidate last = best;
 #pragma unroll
         for (int offset = 32; offset > 0; offset >>= 1) {
-          const Candidate other{__shfl_xor(static_cast<unsigned long long>(best.key), offset, kWave),
-                                __shfl_xor(static_cast<unsigned long long>(best.logit), offset, kWave),
-                                static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(best.token), offset, kWave))};
-          if (before(other, best)) best = other;
+          const Candidate other{__shfl_xor(static_cast<unsigned long long>(last.key), offset, kWave),
+                                __shfl_xor(static_cast<unsigned long long>(last.logit), offset, kWave),
+                                static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(last.token), offset, kWave))};
+          if (before(other, last)) last = other;
         }
         __syncthreads();
-        if (lane == 0) wave_best[wave] = best;
+        if (lane == 0) wave_best[wave] = last;
         __syncthreads();
-        last = wave_best[0];
-        for (int w = 1; w < 4; ++w)
+        for (int w = 0; w < 4; ++w)
           if (before(wave_best[w], last)) last = wave_best[w];
-        first = false;
         if (t == 0) write(n, last);
+        if (best.key != last.key || best.logit != last.logit || best.token != last.token) continue;
+        ++heads[from];
+        best = {0, 0, 0};
+        for (int i = t; i < lists; i += 256)
+          if (const int at = heads[i]; at < a.count) offer(i, candidate(i * a.count + at));
       }
     }
     __syncthreads();
@@ -441,7 +487,7 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
 struct BeamLayout {
   int each;  // logits of a thread
   std::int64_t parts;
-  std::size_t sums, bytes;
+  std::size_t sums, heads, bytes;
 };
 
 // Parts of 8192 logits, or of 2048 where those would not give every CU a block. (128
@@ -454,7 +500,8 @@ BeamLayout beam_layout(std::int64_t batch, std::int64_t beams, std::int64_t voca
   l.parts = (vocabulary + 256 * l.each - 1) / (256 * l.each);
   const auto lists = static_cast<std::size_t>(batch * beams * l.parts);
   l.sums = (lists * count * sizeof(std::uint64_t) + 15) / 16 * 16;
-  l.bytes = l.sums + lists * 2 * sizeof(float);
+  l.heads = l.sums + lists * 2 * sizeof(float);
+  l.bytes = l.heads + lists * sizeof(std::int32_t);
   return l;
 }
 
@@ -512,6 +559,7 @@ int tcx_hip_beam_select_f32(const float* logits, const float* scores, const uint
   a.parts = static_cast<int>(layout.parts);
   a.places = static_cast<std::uint64_t*>(workspace);
   a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + layout.sums);
+  a.heads = reinterpret_cast<std::int32_t*>(static_cast<char*>(workspace) + layout.heads);
   const auto s = static_cast<hipStream_t>(stream);
   const auto items = static_cast<std::uint32_t>(batch * beams * layout.parts);
   const dim3 grid(grid_for(items, 1, kStrideBlocks));

@@ -7,6 +7,8 @@ workspace, with its keys split over blocks, and from packed tiles."""
 
 from __future__ import annotations
 
+import time
+
 import numpy as np
 import pytest
 
@@ -335,3 +337,67 @@ def test_select_of_equal_far_logits(capi, vocabulary, value):
     chosen = cases.beam_candidates(logits, scores)[0, got[1][0], got[2][0]]
     assert np.isfinite(got[0]).all()
     assert (np.abs(got[0][0] - chosen) <= np.abs(chosen) * EPS + 120 * EPS).all()
+
+
+@pytest.mark.parametrize("shape", [(1, 8, 128256, 128), (1, 8, 32000, 256), (1, 64, 20000, 128), (3, 5, 9001, 200), (2, 64, 300, 256),
+                                   (1, 16, 50000, 64)], ids=str)
+def test_select_of_many_candidates(capi, shape):
+    """Counts of which a merge has many thousand candidates."""
+    batch, beams, vocabulary, count = shape
+    rng = np.random.default_rng(74)
+    logits, scores = 3 * f32(rng, batch, beams, vocabulary), f32(rng, batch, beams)
+    check_selection(select(capi, logits, scores, count), logits, scores, count)
+
+
+def test_select_behind_long_sequences(capi):
+    """Scores of many tokens' logarithms: far from zero, and close together for their size."""
+    rng = np.random.default_rng(75)
+    logits, scores = 3 * f32(rng, 1, 16, 32000), (-800 + f32(rng, 1, 16)).astype(np.float32)
+    for count in (16, 100, 256):
+        check_selection(select(capi, logits, scores, count), logits, scores, count)
+
+
+@pytest.mark.parametrize("beams,vocabulary,count", [(64, 300, 256), (8, 9001, 200), (3, 40000, 256)])
+def test_select_of_ties_beside_finished_beams(capi, beams, vocabulary, count):
+    """Candidates that all tie, of which a merge takes the heads of its lists one by one."""
+    rng = np.random.default_rng(76)
+    logits, scores = np.zeros((3, beams, vocabulary), np.float32), np.zeros((3, beams), np.float32)
+    logits[1, :, ::3] = -np.inf
+    scores[2, ::2] = -np.inf
+    finished = rng.random((3, beams)) < 0.4
+    finished[:, 0] = True
+    dx, ds, df = (capi.DeviceArray.from_numpy(x) for x in (logits, scores, finished))
+    outs = [capi.DeviceArray((3, count)), *(capi.DeviceArray((3, count), np.int32) for _ in range(2))]
+    ws = capi.beam_select_workspace(3, beams, vocabulary, count)
+    capi.beam_select(dx.ptr, ds.ptr, *(o.ptr for o in outs), 3, beams, vocabulary, count, finished=df.ptr, eos=7, workspace=ws)
+    capi.synchronize()
+    want = cases.beam_best(logits, scores, count, finished, 7)
+    np.testing.assert_array_equal(outs[1].numpy(), want[1])
+    np.testing.assert_array_equal(outs[2].numpy(), want[2])
+
+
+def test_select_takes_alike_times_for_alike_counts(capi):
+    """What the search leaves to be put in order depends on the count, not on what it has in
+    common with the block's size: no count takes eight times as long as a larger one,
+    where taking them one by one took seventy times and more."""
+    rng = np.random.default_rng(77)
+    batch, beams, vocabulary = 1, 8, 32000
+    dx = capi.DeviceArray.from_numpy(3 * f32(rng, batch, beams, vocabulary))
+    ds = capi.DeviceArray.from_numpy(f32(rng, batch, beams))
+    outs = [capi.DeviceArray((batch, 256)), *(capi.DeviceArray((batch, 256), np.int32) for _ in range(2))]
+    ws = capi.beam_select_workspace(batch, beams, vocabulary, 256)
+
+    def seconds(count):
+        taken = []
+        for _ in range(5):
+            capi.synchronize()
+            start = time.perf_counter()
+            for _ in range(4):
+                capi.beam_select(dx.ptr, ds.ptr, *(o.ptr for o in outs), batch, beams, vocabulary, count, workspace=ws)
+            capi.synchronize()
+            taken.append(time.perf_counter() - start)
+        return min(taken)
+    times = {count: seconds(count) for count in (32, 64, 96, 128, 192, 256)}
+    largest = seconds(250)
+    assert all(taken < 8 * largest for taken in times.values()), (times, largest)
+    assert largest < 20 * times[32], (times, largest)
