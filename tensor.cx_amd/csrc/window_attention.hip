@@ -262,10 +262,10 @@ WindowForm window_form(const DecodeArgs& a, std::size_t workspace_bytes) {
     f.prompt = true;
     f.waves = 4;
     f.each = 1;
-    const std::size_t tiles = static_cast<std::size_t>(heads * most_tiles(a)) * tile_bytes(a);
-    if ((total >= 1024 || (total >= 256 && blocks(64) >= 192)) && tiles <= workspace_bytes) {
+    const auto places = static_cast<std::size_t>(heads * most_tiles(a));  // below 2^55; their bytes may pass 64 bits
+    if ((total >= 1024 || (total >= 256 && blocks(64) >= 192)) && places <= workspace_bytes / tile_bytes(a)) {
       f.packed = true;
-      f.tiles = tiles;
+      f.tiles = places * tile_bytes(a);
       if (blocks(128) >= 256) f.waves = 8;
       if (a.features > 64 && a.window > 0 && blocks(256) >= 256) f.each = 2;
     }
