@@ -52,8 +52,10 @@ def _count(value, name: str, least: int) -> int:
         number = operator.index(value)
     except TypeError:
         raise TypeError(f"{name} must be an integer") from None
-    if not least <= number < 2**32:
+    if number < least:
         raise ValueError(f"{name} must be at least {least}")
+    if number >= 2**32:
+        raise ValueError(f"{name} must be below 2^32")
     return number
 
 

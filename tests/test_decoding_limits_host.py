@@ -5,6 +5,8 @@ from __future__ import annotations
 
 import ctypes
 
+import pytest
+
 import tensorcx_hip_capi as capi
 
 
@@ -24,3 +26,10 @@ def test_workspaces_past_64_bits_are_not_asked_for():
         for cols in (64, 1000, 2 ** 20):
             keys = batch * cols * 128 * 4 * 2
             assert keys <= wanted(batch=batch, cols=cols, **sizes) <= 1.1 * keys + batch * 70000
+
+
+def test_numbers_past_32_bits_are_named():
+    import tensorcx as cx
+    for number, words in ((2 ** 32, "below 2"), (2 ** 70, "below 2"), (-1, "at least 0")):
+        with pytest.raises(ValueError, match=words):
+            cx.hip.new_cache(1, 1, number, 64)
