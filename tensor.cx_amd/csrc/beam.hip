@@ -435,7 +435,7 @@ struct ReorderArgs {
   int width[kReorderTensors];            // bytes of a unit: 16, 4 or 1
   int tensors;
   const std::int32_t* index;
-  std::int64_t items, rows;
+  std::int64_t items;
   int beams, count;
   std::int32_t* flag;
 };
@@ -597,7 +597,6 @@ int tcx_hip_beam_reorder(const void* const* in, void* const* out, const int64_t*
   for (int from = 0; from < tensors; from += kReorderTensors) {
     ReorderArgs a{};
     a.index = index;
-    a.rows = rows;
     a.beams = static_cast<int>(beams);
     a.count = static_cast<int>(count);
     a.flag = flag;

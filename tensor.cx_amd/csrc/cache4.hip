@@ -222,8 +222,6 @@ __global__ __launch_bounds__(256) void cache_load_kernel(const std::int32_t* __r
   }
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15U) == 0; }
-
 // Rows of a block: 4 where a head has no more, else 16 (cache_attention_kernel:
 // 16 sequences of 4096 to 8192 tokens, 8 heads of 128 features, one row each 50.2
 // -> 38.2 us, four 49.3 -> 38.2).

@@ -55,6 +55,8 @@ struct DecodeArgs {
   float* part_ml;
 };
 
+inline bool aligned16(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15U) == 0; }
+
 // Checks desc and fills `a`; true with *rc = TCX_OK in `done` when there is
 // nothing to compute. `cache`: k and v are 4-bit caches.
 int decode_args(const float* q, const void* k, const void* v, float* out, const tcx_hip_window_attention_desc_t* desc,

@@ -430,9 +430,12 @@ struct PromptRows {
   }
 };
 
-template <int D, int kWaves, int kQ>
-__global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(DecodeArgs a, std::uint32_t items, int row_tiles) {
-  constexpr int kThreads = 64 * kWaves, kRows = 16 * kQ * kWaves, kTile = 64;
+// Rows of a block, 16 a wave.
+constexpr int kPromptRows = 64;
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void prompt_attention_kernel(DecodeArgs a, std::uint32_t items, int row_tiles) {
+  constexpr int kThreads = 256, kRows = kPromptRows, kTile = 64;
   constexpr int kKeyChunks = D / 8;  // of 8 features a key
   constexpr int kKeyTasks = (kTile * kKeyChunks + kThreads - 1) / kThreads;
   constexpr int kQuads = D / 4;      // of 4 features of a key's values
@@ -508,11 +511,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Decode
       }
     };
 
-    PromptRows<D, kQ> rows;
+    PromptRows<D, 1> rows;
     if (t < 2) value_bad[t] = 0;
     __syncthreads();
     if (u0 < u1) load_keys(u0);
-    rows.start(a, b, kv, n, r0 + wave * kQ * 16, r1, lane);
+    rows.start(a, b, kv, n, r0 + wave * 16, r1, lane);
     if (u0 < u1) {
       store_keys();
       load_values(u0);
@@ -534,7 +537,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Decode
       const bool all_seen = u + kTile <= u1 &&
                             (!with_window || (last <= rows.first_row && (a.window == 0 || from > rows.last_row - a.window)));
       auto key_of = [&](int k) { return u + k < u1 ? seen.key(u + k) : 1 << 30; };
-      half8_t p_hi[kQ][2], p_lo[kQ][2];
+      half8_t p_hi[1][2], p_lo[1][2];
       if (any_seen)
         rows.scores(a, key_hi, key_lo, key_factor, value_exp[buffer], value_unit[buffer],
                     largest(value_most[buffer]), all_seen, key_of, p_hi, p_lo);

@@ -116,8 +116,6 @@ bool fill_strides(const std::int64_t (&in)[3], std::int64_t heads, std::int64_t 
   return true;
 }
 
-bool aligned(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15U) == 0; }
-
 constexpr int kMostSplits = 64;  // join_splits_kernel: a lane each
 
 }  // namespace
@@ -143,7 +141,7 @@ int decode_args(const float* q, const void* k, const void* v, float* out, const 
   // Lengths may leave cols keys unread, but a call of no keys needs none.
   if (q == nullptr || out == nullptr || (d.cols > 0 && (k == nullptr || v == nullptr)))
     return fail(TCX_INVALID_ARGUMENT, "attention buffers are null");
-  if (!aligned(q) || !aligned(k) || !aligned(v) || !aligned(out))
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
     return fail(TCX_INVALID_ARGUMENT, "attention buffers must be 16-byte aligned");
   a.q = q;
   a.k = k;
@@ -318,7 +316,7 @@ int launch_prompt(const DecodeArgs& a, const WindowForm& form, hipStream_t s) {
   const int tiles = (a.rows * a.share + form.rows - 1) / form.rows;
   std::uint32_t items;
   if (int rc = count_items(a, tiles, items); rc != TCX_OK) return rc;
-  hipLaunchKernelGGL((prompt_attention_kernel<D, 4, 1>), dim3(grid_for(items, 1, 1 << 22)), dim3(256), 0, s, a, items, tiles);
+  hipLaunchKernelGGL(prompt_attention_kernel<D>, dim3(grid_for(items, 1, 1 << 22)), dim3(256), 0, s, a, items, tiles);
   return check(hipGetLastError(), "attention launch");
 }
 
@@ -357,7 +355,7 @@ int tcx_hip_window_attention_f32(const float* q, const float* k, const float* v,
   DecodeArgs a{};
   bool done = false;
   if (int rc = decode_args(q, k, v, out, desc, false, a, done); rc != TCX_OK || done) return rc;
-  if (workspace != nullptr && (reinterpret_cast<std::uintptr_t>(workspace) & 15U))
+  if (!aligned16(workspace))
     return fail(TCX_INVALID_ARGUMENT, "attention workspace must be 16-byte aligned");
   if (int rc = ready(); rc != TCX_OK) return rc;
   const auto s = static_cast<hipStream_t>(stream);
