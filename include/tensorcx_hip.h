@@ -537,13 +537,25 @@ int tcx_hip_window_attention_supported(int64_t features);
  * at its last key) and sees key j of 0 <= j <= p when the window is 0, j > p -
  * window or j < sinks: out = softmax over those of scale * q.k, times v. A query
  * that sees no key gets zeros. Hidden keys have no influence, whatever they
- * hold; a row that sees a NaN is NaN, and what infinities that it sees make of
- * it is not specified. Pointers are 16-byte aligned, strides multiples of 4, rows *
- * heads / kv_heads, cols and batch * kv_heads below 2^30, and no more than 2^31
- * blocks (of at least a row of a key head each) may be asked for. The workspace (16-byte
- * aligned, may be NULL) takes the states of keys split over blocks, as far as
- * it has room; the query says how much such a call can use, and it must stay
- * allocated until the stream has run the call. */
+ * hold; a row that sees a NaN is NaN (of a value, in its feature), and what
+ * infinities that it sees make of it is not specified.
+ *
+ * Everything is float32's: products with errors of a few 2^-24, and sums of
+ * weights times values that are divided by the sum of the weights at the end, so
+ * that values near float32's largest, seen by the dozen, may give infinity. With more
+ * than eight rows of a key head (rows * heads / kv_heads) each factor is held
+ * to 22 bits, and a weight no finer than 2^-35 of the row's largest product of a
+ * weight and its key's largest value (to a power of two): seen where one key's values
+ * are thousands of times another's.
+ *
+ * Pointers are 16-byte aligned, strides multiples of 4, rows * heads / kv_heads,
+ * cols and batch * kv_heads below 2^30, and no more than 2^31 blocks (of at least a
+ * row of a key head each) may be asked for. The workspace (16-byte aligned, may be
+ * NULL) takes the states of keys split over blocks, as far as it has room, and for
+ * prompts of many rows the keys and values that they see, about as many bytes as
+ * those have, if it has room for all (without it such a prompt takes up to twice as
+ * long); the query says how much such a call can use, and it must stay allocated
+ * until the stream has run the call. */
 size_t tcx_hip_window_attention_workspace_bytes(const tcx_hip_window_attention_desc_t* desc);
 int tcx_hip_window_attention_f32(const float* q, const float* k, const float* v, float* out,
                                  const tcx_hip_window_attention_desc_t* desc, void* workspace, size_t workspace_bytes,
@@ -584,15 +596,18 @@ int tcx_hip_cache4_attention_f32(const float* q, const int32_t* key_cache, const
 /* Beam search's choice: of the candidates (beam k, token v) of each sequence, at
  * scores[b, k] + logits[b, k, v] - log(sum over the beam of exp(logits)), the
  * `count` best in descending order: their scores, beams and tokens, [batch,
- * count] each. Candidates are compared in 64 bits; of equal scores the lower
+ * count] each. A beam's sum is float32's, of differences from its largest logit;
+ * candidates are made of it and compared in 64 bits. Of equal scores the lower
  * beam comes first, and of one beam the larger logit, then the lower token. NaN
  * comes before every number, and a beam with a NaN or +inf among its logits offers
- * NaN alone; a beam whose logits are all -inf offers -inf. A
- * beam with finished[b, k] != 0 (may be NULL) offers token `eos` at its own
- * score and -inf for the others. beams * vocabulary is below 2^31, count at most
- * TCX_HIP_BEAM_MAX_COUNT and beams * vocabulary. The workspace (16-byte aligned,
- * of at least the query's bytes) must stay allocated until the stream has run
- * the call. */
+ * NaN alone; a beam whose logits are all -inf offers -inf. A beam with
+ * finished[b, k] != 0 (may be NULL) offers token `eos` at its own score and -inf for
+ * the others. Up to 64 beams, beams * vocabulary below 2^31, count at most
+ * TCX_HIP_BEAM_MAX_COUNT and beams * vocabulary. A sequence's merge is one block's work,
+ * which grows with beams * vocabulary * count; more than a thousand candidates alike
+ * (all -inf, say) at the end of it are taken one by one, some 2 us each. The workspace
+ * (16-byte aligned, of at least the query's bytes) must stay allocated until the stream
+ * has run the call. */
 size_t tcx_hip_beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocabulary, int64_t count);
 int tcx_hip_beam_select_f32(const float* logits, const float* scores, const uint8_t* finished, int32_t eos,
                             float* out_scores, int32_t* out_beams, int32_t* out_tokens, int64_t batch, int64_t beams,

@@ -17,8 +17,8 @@
 // of the parts' lists, some 2.3 us each.
 //
 // The parts read the logits once, and hold them in registers. Measured: 128 beams of
-// 128256 logits, 65.7 MB, in 20.5 us with count 16 (a plain read takes 10.5), and
-// 9.5 for the merge; four beams of 32000 with count 4 in 4.8 and 6.7. What is left
+// 128256 logits, 65.7 MB, in 21 us with count 16 (a plain read takes 10.5), and
+// 9.6 for the merge; four beams of 32000 with count 4 in 4.9 and 6.8. What is left
 // above the read is the work on what was read: a block waits for its loads, then
 // for the search, the list and its order, three blocks a CU. Eight beams of 128256:
 // count 16 in 33 us, 64 in 110, 128 in 217, 256 in 420: a sequence's merge is one

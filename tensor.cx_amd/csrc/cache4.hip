@@ -223,14 +223,14 @@ __global__ __launch_bounds__(256) void cache_load_kernel(const std::int32_t* __r
 }
 
 // Rows of a block: 4 where a head has no more, else 16 (cache_attention_kernel:
-// 16 sequences of 4096 to 8192 tokens, 8 heads of 128 features, one row each 50.2
-// -> 38.2 us, four 49.3 -> 38.2).
+// 16 sequences of 4096 to 8192 tokens, 8 heads of 128 features, one row each 47.3
+// -> 38.5 us, four 46.0 -> 38.7).
 int cache_rows(const DecodeArgs& a) { return a.rows * a.share <= 4 ? 4 : 16; }
 
-// 768 blocks fill the GPU three to a CU (512 and 1024: 38.9 and 38.4 us against
-// 38.2), and a split of fewer than 256 keys costs more than it spares; nor do two or
-// three pay for the join (8 heads of 64 features, one sequence: 512 keys 8.1 us
-// whole, 9.2 in two; 1024 keys 11.7 whole, 9.5 in four).
+// 768 blocks fill the GPU three to a CU (512 and 1024: 40.3 and 39.2 us against
+// 38.5), and a split of fewer than 256 keys costs more than it spares; nor do two or
+// three pay for the join (8 heads of 64 features, one sequence: 512 keys 8.6 us
+// whole, 10.1 in two; 1024 keys 12.5 whole, 9.9 in four).
 int cache_splits(const DecodeArgs& a, std::size_t workspace_bytes) {
   const int rows = cache_rows(a);
   const std::int64_t blocks = static_cast<std::int64_t>(a.batch) * a.kv_heads * ((a.rows * a.share + rows - 1) / rows);

@@ -36,11 +36,14 @@
 // not four times.
 //
 // Measured: 16 sequences of up to 8192 tokens, 32 heads on 8 of 128 features, 129
-// MB in 38 us and 4 more for the join (a vector kernel of a key at a time: 98 us);
-// 131072 tokens of 16 heads of 64, 168 MB, in 45 and 7. A copy would take 23 and 31.
-// What bounds it is the waves' issue: a tile of 32 tokens is some 500 instructions
-// on 5 KB (four query rows that share a key head, and one, take the same time). Tiles brought by asynchronous copies into an LDS ring, and splits of a
-// fixed length, were no faster.
+// MB in 38.5 us and 4.7 more for the join (a vector kernel of a key at a time: 98 us);
+// 131072 tokens of 16 heads of 64, 168 MB, in 47 and 7. A copy would take 23 and 31.
+// One sequence of 8192, 32 heads on 8 of 128: 16 rows 23 and 5, 64 rows 52 and 5, 512
+// rows 295, each block of 16 rows unpacking all that it sees. What bounds it is issue
+// and latency together: a tile of 32 tokens is some 500 instructions on 5 KB, 20 us
+// of the 38.5 on vector pipes, and waves wait 38 % of their time (four query rows that
+// share a key head, and one, take the same time). Tiles brought by asynchronous copies
+// into an LDS ring, and splits of a fixed length, were no faster.
 #pragma once
 
 #include "decoding.hpp"

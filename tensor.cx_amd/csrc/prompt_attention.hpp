@@ -40,7 +40,7 @@
 //
 // Measured: 3 sequences of 37 rows, 6 heads on 2 of 80 features, windows of 50, in 16 us,
 // 12 blocks and a chain of loads, splitting and products for each tile; 2 sequences of
-// 64 rows, 16 heads on 4 of 128 features and 8192 keys in 64 us. Asking for a tile's K and
+// 64 rows, 16 heads on 4 of 128 features and 8192 keys in 65 us. Asking for a tile's K and
 // V together was no faster (50 -> 55 us for 8 sequences of 20 rows): what bounds it
 // there is splitting them into halves.
 #pragma once
@@ -564,11 +564,14 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(DecodeArgs a, 
 // block's buffers hold it, to the workspace, and prompt_tile_kernel takes the
 // tiles from there straight into LDS, two buffers and one barrier a tile.
 //
-// Measured: 4096 rows, 16 heads on 4 of 128 features, window 1024, in 9.4 us of packing
-// (its chain of load, split and store; a block a CU) and 106 to 114 of products, 91
-// GFLOP in halves at 0.8 PFLOP/s; 8192 rows, 16 heads of 64 features, window 2048: 25
-// (134 MB, at a copy's rate) and 213. Counters: matrix pipes busy 96 k cycles of 230 k
-// a SIMD, a third of the waves' time waits (LDS, barrier) and a third waits to issue.
+// Measured: 4096 rows, 16 heads on 4 of 128 features, window 1024, in 9.6 us of packing
+// (its chain of load, split and store; a block a CU) and some 108 of products, 91
+// GFLOP in halves at 0.8 PFLOP/s, of a call of 117 (128 for the products alone under the
+// profiler, which runs them with pauses between, at a lower clock); 8192 rows, 16 heads
+// of 64 features, window 2048: 26 (134 MB, at a copy's rate) and 209 of 235 (250).
+// Counters: matrix pipes busy 96 k cycles of 230 k a SIMD, 182 k of 430 k for the latter,
+// where 58 k vector instructions a SIMD at four cycles are as much again; a third of the
+// waves' time waits (LDS, barrier) and a third waits to issue.
 // A higher priority for half of the waves, and operands read from LDS one step ahead
 // (127 -> 123 us under the profiler for the scores; for both products the registers
 // spill), gave little.

@@ -233,21 +233,21 @@ std::size_t tile_bytes(const DecodeArgs& a) {
 
 // Which kernel, for `total` rows of `heads` key heads:
 // * up to 8 rows stream the keys past them (4 sequences of 12 rows, 8 heads of 128
-//   features, 2000 keys: 47 -> 32 us on matrix instructions; of 8 rows 28 -> 32, in
-//   15 parts of the keys);
+//   features, 2000 keys: 44 -> 27 us on matrix instructions; of 8 rows 26.7 and 26.2,
+//   and one row would leave fifteen columns of sixteen idle);
 // * more take matrix instructions, in blocks of 64 rows that pack what they see for
 //   themselves (prompt_attention_kernel);
 // * where a tile of keys would be packed by four blocks and more of a GPU that is
 //   nearly full, or by sixteen, it is packed once instead (prompt_pack_kernel and
 //   prompt_tile_kernel): 4 sequences of 200 rows, 16 heads on 8 of 128 features and
-//   1000 keys 71 -> 57 us, a prompt of 2048, 16 heads on 4 of 64, 107 -> 63; 2
+//   1000 keys 68 -> 55 us, a prompt of 2048, 16 heads on 4 of 64, 109 -> 63; 2
 //   sequences of 64 rows, 16 heads on 4 of 128 features and 8192 keys, 32 blocks, 65
 //   -> 80 the other way, one of 512, 8 heads of 64 features, 64 blocks, 17 -> 20;
 // * in blocks of 128 rows where those are at least 256, one a CU (2048 rows, 16
-//   heads on 4 of 128 features: 137 -> 107 us; 8 heads of their own, 128 blocks:
-//   90 -> 103 the other way), and of 256 where those are, heads have more than 64
-//   features and a window leaves the blocks alike (4096 rows, window 1024: 139 ->
-//   119 us; a causal prompt without a window 163 -> 173 the other way).
+//   heads on 4 of 128 features: 131 -> 102 us; the 200 rows above, 128 blocks: 55 ->
+//   62 the other way), and of 256 where those are, heads have more than 64
+//   features and a window leaves the blocks alike (4096 rows, window 1024: 134 ->
+//   118 us; without a window 286 -> 296 the other way).
 WindowForm window_form(const DecodeArgs& a, std::size_t workspace_bytes) {
   const int total = a.rows * a.share;
   const std::int64_t heads = static_cast<std::int64_t>(a.batch) * a.kv_heads;
@@ -271,7 +271,7 @@ WindowForm window_form(const DecodeArgs& a, std::size_t workspace_bytes) {
   }
   // A CU holds four blocks that stream, two of four waves with tiles in LDS and
   // one of eight. Packed tiles are split only where a part keeps 512 keys (512
-  // rows, 16 heads on 4, 512 keys: 34 us whole, 40 in four parts). Others from 512
+  // rows, 16 heads on 4, 512 keys: 32 us whole, 40 in four parts). Others from 512
   // keys on, of 128 (8 heads of 64 features, one row: 256 keys 4.9 us whole, 7.8 in
   // two; of 128 features 512 keys 11.8 whole, 9.8 in four).
   f.splits = plan_splits(a, blocks(f.rows), f.prompt ? 2048 / f.waves : 1024, f.packed ? 512 : 128, f.packed ? 1024 : 512,

@@ -14,6 +14,10 @@ The others are the operators of a decoding loop:
   attention over them;
 * ``beam_select`` and ``beam_reorder``: beam search's choice over beams and
   vocabulary, and the states of the chosen beams.
+
+They allocate their outputs and what workspace they use, and return when the
+result is there. Loops that keep buffers, run ahead or capture graphs call the C
+ABI's functions of the same names (``tensorcx_hip_capi``), which do neither.
 """
 
 from __future__ import annotations
@@ -153,11 +157,12 @@ def beam_select(logits, scores, count: int, *, finished=None, eos: int | None = 
     """(scores, beams, tokens), (batch, count) each: of the candidates (beam k,
     token v) of every sequence the best ``count`` (at most 256) by scores[b, k] +
     log_softmax(logits[b, k])[v], in descending order, for logits (batch, beams,
-    vocabulary) and scores (batch, beams) of up to 64 beams. Candidates are
-    compared in 64 bits; of equal scores the lower beam comes first, and of one beam
-    the larger logit, then the lower token. NaN comes before every number, and a beam
-    with a NaN or +inf among its logits offers NaN alone. A beam that is finished (bool (batch, beams)) offers the token ``eos`` at its own
-    score and nothing (-inf) besides."""
+    vocabulary) and scores (batch, beams) of up to 64 beams. A beam's sum of
+    exponentials is float32's; candidates are compared in 64 bits. Of equal scores the
+    lower beam comes first, and of one beam the larger logit, then the lower token. NaN
+    comes before every number, and a beam with a NaN or +inf among its logits offers
+    NaN alone. A beam that is finished (bool (batch, beams)) offers the token ``eos``
+    at its own score and nothing (-inf) besides."""
     from . import Tensor, _core, _inference
     if (finished is None) != (eos is None):
         raise ValueError("finished and eos come together")
