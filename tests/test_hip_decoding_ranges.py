@@ -401,3 +401,17 @@ def test_select_takes_alike_times_for_alike_counts(capi):
     largest = seconds(250)
     assert all(taken < 8 * largest for taken in times.values()), (times, largest)
     assert largest < 20 * times[32], (times, largest)
+
+
+@pytest.mark.parametrize("score", [-1e30, np.nan])
+@pytest.mark.parametrize("count", [3, 200, 256])
+def test_select_by_logits_alone(capi, count, score):
+    """Scores that all round to the same, or are all NaN: the first beam's largest logits,
+    found from thousands of candidates whose scores tie."""
+    rng = np.random.default_rng(78)
+    logits = f32(rng, 2, 8, 32000)
+    got = select(capi, logits, np.full((2, 8), score, np.float32), count)
+    for b in range(2):
+        assert (got[1][b] == 0).all()
+        np.testing.assert_array_equal(got[2][b], np.argsort(-logits[b, 0], kind="stable")[:count])
+    np.testing.assert_array_equal(got[0], np.full((2, count), score, np.float32))
