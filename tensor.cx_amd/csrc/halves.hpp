@@ -130,8 +130,8 @@ struct RowBase {
   template <typename Row, typename Each, typename Product>
   __device__ __forceinline__ int move(float& l, Row&& row, Each&& each, Product&& product) {
     top = row(top);
-    const float high = row(product()) + rest;
-    const bool past = first || high > kMost, need = top > -__builtin_inff() && (past || top > kFar);
+    const float high = row(product());
+    const bool past = first || high + rest > kMost, need = top > -__builtin_inff() && (past || top > kFar);
     float to = base, aim = rest, gone = 0.F;
     bool plain = true, far = false;
     if (need) {
@@ -141,6 +141,7 @@ struct RowBase {
       far = fabsf(to) >= kWhole;
       if (far) to = base + top;  // the largest score itself, which the others are then rounded like
       plain = by == all && !far;
+      if (past && plain) aim = 0.F;
       gone = to - base;
     }
     if (__any(!plain)) [[unlikely]] {
@@ -148,7 +149,7 @@ struct RowBase {
       top = far ? 0.F : top - gone;
       gone = 0.F;
       const float now = row(product());
-      if (!plain && (first || now + rest > kMost)) aim = kAim - ceilf(now);
+      if (!plain && (past || now + rest > kMost)) aim = kAim - ceilf(now);
     }
     top -= gone;
     each([&](float s) { return s - gone; });
