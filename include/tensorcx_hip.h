@@ -620,6 +620,63 @@ int tcx_hip_beam_reorder(const void* const* in, void* const* out, const int64_t*
                          const int32_t* index, int64_t batch, int64_t beams, int64_t count, int32_t* flag,
                          tcx_stream_t stream);
 
+/* -------------------------------------------------------- 8-bit rows and products */
+
+/* Rows in 8-bit floating point (e4m3: a sign, four bits of exponent, three of
+ * mantissa; 448 at most, steps of 2^-9 at the least, no infinities), each 128
+ * features of a row in units of a power of two of their own. A matrix of `rows` rows
+ * is int32 codes [rows, code words], four codes a word in the features' order, in
+ * whole blocks of 128 with zeros behind the last feature; and int32 scales [rows, scale
+ * words], four blocks' exponents e a word as bytes e + 127, zeros behind the last
+ * block. A block's exponent is the least from -100 on that leaves its largest finite
+ * value at most 448 * 2^e; values are rounded to the nearest code, ties to even, at
+ * most 2^-4 of themselves off, or 2^-10 of 2^e. NaN and infinities are held as NaN; a
+ * value next to float32's largest may round to infinity. Codes are 16-byte aligned,
+ * scales and float32 buffers 4-byte aligned. Nothing here allocates or waits. */
+int64_t tcx_hip_block8_code_words(int64_t features);
+int64_t tcx_hip_block8_scale_words(int64_t features);
+/* x: rows of `features` float32, x_stride apart (0: features). Fewer than 2^31 words
+ * of scales, features below 2^30; so too for the next two. */
+int tcx_hip_quantise8(const float* x, int32_t* codes, int32_t* scales, int64_t rows, int64_t features, int64_t x_stride,
+                      tcx_stream_t stream);
+/* What codes and scales stand for, as float32. */
+int tcx_hip_dequantise8(const int32_t* codes, const int32_t* scales, float* out, int64_t rows, int64_t features,
+                        int64_t out_stride, tcx_stream_t stream);
+typedef struct {
+  int64_t rows, features;
+  float epsilon;                                  /* finite, not negative */
+  int64_t x_stride, residual_stride, sum_stride; /* floats between rows; 0: features */
+} tcx_hip_rmsnorm8_desc_t;
+/* s = x + residual (x for NULL), y = s / sqrt(mean of s^2 + epsilon) * weight (1 for
+ * NULL), all float32; y is quantised, and s written to sum unless that is NULL. sum
+ * may be x or residual itself. */
+int tcx_hip_rmsnorm8(const float* x, const float* residual, const float* weight, float* sum, int32_t* codes, int32_t* scales,
+                     const tcx_hip_rmsnorm8_desc_t* desc, tcx_stream_t stream);
+
+typedef struct {
+  int64_t rows, features, outputs; /* below 2^30, 2^22 and 2^29 */
+  const float* bias;               /* [outputs], or [2 * outputs] of the gated product; may be NULL */
+  int32_t activation;              /* TCX_ACT_* */
+  int64_t out_stride;              /* floats between rows of out; 0: outputs */
+} tcx_hip_linear8_desc_t;
+/* out = act(x w^T + bias) of x [rows, features] and w [outputs, features], both in 8
+ * bits, as float32. Products are exact and summed in float32, in an order that goes
+ * by the sizes, not by the call; a NaN makes its row (of w: its column) NaN. Scales
+ * hold bytes of 27 to 247 as the functions above write them, and codes and scales
+ * behind the last feature are zeros. The workspace (16-byte aligned, may be NULL)
+ * takes the parts of sums split over blocks; the query says how much a call can use,
+ * and it must stay allocated until the stream has run the call. */
+size_t tcx_hip_linear8_workspace_bytes(const tcx_hip_linear8_desc_t* desc);
+int tcx_hip_linear8(const int32_t* x_codes, const int32_t* x_scales, const int32_t* w_codes, const int32_t* w_scales, float* out,
+                    const tcx_hip_linear8_desc_t* desc, void* workspace, size_t workspace_bytes, tcx_stream_t stream);
+/* act(x g^T + bias) * (x u^T + bias'), quantised: w holds the `outputs` rows of g, then
+ * those of u, bias likewise; codes and scales have `outputs` features a row.
+ * out_stride is 0. The workspace must have the query's size. */
+size_t tcx_hip_gated_linear8_workspace_bytes(const tcx_hip_linear8_desc_t* desc);
+int tcx_hip_gated_linear8(const int32_t* x_codes, const int32_t* x_scales, const int32_t* w_codes, const int32_t* w_scales,
+                          int32_t* codes, int32_t* scales, const tcx_hip_linear8_desc_t* desc, void* workspace,
+                          size_t workspace_bytes, tcx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

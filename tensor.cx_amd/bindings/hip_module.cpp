@@ -272,6 +272,9 @@ PYBIND11_MODULE(_core, m) {
   });
 
   m.def("_kernel", &kernel, py::arg("entry"), py::arg("inputs"), py::arg("scalars"), py::arg("outputs"));
+  m.def("_block8_words", [](std::int64_t features) {
+    return py::make_tuple(tcx_hip_block8_code_words(features), tcx_hip_block8_scale_words(features));
+  });
   m.def("_cache4_words", [](std::int64_t features) { return tcx_hip_cache4_words(features); });
 
   for (const auto& [name, kind] : std::vector<std::pair<const char*, OpKind>>{

@@ -1458,6 +1458,144 @@ void beam_reorder(const KernelCall& c, Stream& s) {
   flag.finish(s, "beam reorder indices must name a beam");
 }
 
+// ------------------------------------------------------------ 8-bit rows
+// Rows in 8-bit floating point: int32 codes (..., code words) and scales (..., scale words).
+
+Dim rows_of(const Shape& shape) { return numel(Shape(shape.begin(), shape.end() - 1)); }
+Shape with_last(Shape shape, Dim last) {
+  shape.back() = last;
+  return shape;
+}
+// Checks codes and scales as those of rows of `shape`, whose last axis is the features.
+void expect_rows8(const KernelCall& c, const Tensor& codes, const Tensor& scales, const Shape& shape) {
+  c.expect_dtype(codes, DType::kInt32, "codes");
+  c.expect_dtype(scales, DType::kInt32, "scales");
+  c.expect_shape(codes, with_last(shape, tcx_hip_block8_code_words(shape.back())), "codes");
+  c.expect_shape(scales, with_last(shape, tcx_hip_block8_scale_words(shape.back())), "scales");
+}
+// The shape of rows that codes and scales hold, in whole blocks.
+Shape shape_of_rows8(const KernelCall& c, const Tensor& codes, const Tensor& scales) {
+  if (codes.shape.empty() || codes.shape.back() % 32 != 0) c.refuse("takes codes in whole blocks of 32 words");
+  const Shape shape = with_last(codes.shape, codes.shape.back() * 4);
+  expect_rows8(c, codes, scales, shape);
+  return shape;
+}
+const std::int32_t* i32(const Tensor& t) { return static_cast<const std::int32_t*>(device_ptr(t)); }
+std::int32_t* out_i32(const Tensor& t) { return static_cast<std::int32_t*>(out_ptr(t)); }
+void expect_code_outputs(const KernelCall& c, std::size_t first, const Shape& shape) {
+  expect_rows8(c, c.outputs[first], c.outputs[first + 1], shape);
+  if (!aligned16(out_ptr(c.outputs[first]))) c.refuse("codes must be 16-byte aligned");
+}
+
+// "quantise8": x; outputs codes and scales.
+void quantise8(const KernelCall& c, Stream& s) {
+  c.expect(1, 1, 0, 2);
+  const Tensor& x = *c.tensors[0];
+  c.expect_dtype(x, DType::kFloat32, "input");
+  if (x.shape.empty()) c.refuse("takes rows");
+  expect_code_outputs(c, 0, x.shape);
+  c.expect_apart();
+  if (numel(x.shape) == 0) return;
+  ok_or_throw(tcx_hip_quantise8(f32(x), out_i32(c.outputs[0]), out_i32(c.outputs[1]), rows_of(x.shape), x.shape.back(), 0, s),
+              "HIP quantise8");
+  if (s.used()) synchronize(s);
+}
+
+// "dequantise8": codes, scales; output the float32 rows.
+void dequantise8(const KernelCall& c, Stream& s) {
+  c.expect(2, 2, 0, 1);
+  const Tensor& out = c.outputs[0];
+  c.expect_dtype(out, DType::kFloat32, "output");
+  if (out.shape.empty()) c.refuse("writes rows");
+  expect_rows8(c, *c.tensors[0], *c.tensors[1], out.shape);
+  c.expect_apart();
+  if (numel(out.shape) == 0) return;
+  const Tensor codes = on_boundary(*c.tensors[0]);
+  ok_or_throw(tcx_hip_dequantise8(i32(codes), i32(*c.tensors[1]), static_cast<float*>(out_ptr(out)), rows_of(out.shape),
+                                  out.shape.back(), 0, s),
+              "HIP dequantise8");
+  if (s.used()) synchronize(s);
+}
+
+// "rmsnorm8": x[, residual][, weight]; epsilon bits, whether there is a residual, a
+// weight; outputs codes, scales, and with a residual the sum.
+void rmsnorm8(const KernelCall& c, Stream& s) {
+  if (c.scalars.size() != 3 || c.scalars[1] > 1 || c.scalars[2] > 1) c.refuse("takes an epsilon and two truth values");
+  const bool residual = c.scalars[1] != 0, weight = c.scalars[2] != 0;
+  c.expect(1 + residual + weight, 1 + residual + weight, 3, residual ? 3 : 2);
+  const Tensor& x = *c.tensors[0];
+  c.expect_dtype(x, DType::kFloat32, "input");
+  if (x.shape.empty()) c.refuse("takes rows");
+  if (residual) {
+    c.expect_dtype(*c.tensors[1], DType::kFloat32, "residual");
+    c.expect_shape(*c.tensors[1], x.shape, "residual");
+    c.expect_dtype(c.outputs[2], DType::kFloat32, "sum");
+    c.expect_shape(c.outputs[2], x.shape, "sum");
+  }
+  if (weight) {
+    c.expect_dtype(*c.tensors.back(), DType::kFloat32, "weight");
+    c.expect_shape(*c.tensors.back(), Shape{x.shape.back()}, "weight (features,)");
+  }
+  expect_code_outputs(c, 0, x.shape);
+  c.expect_apart();
+  tcx_hip_rmsnorm8_desc_t d{};
+  d.rows = rows_of(x.shape);
+  d.features = x.shape.back();
+  d.epsilon = float_of(c.scalars[0]);
+  ok_or_throw(tcx_hip_rmsnorm8(f32(x), residual ? f32(*c.tensors[1]) : nullptr, weight ? f32(*c.tensors.back()) : nullptr,
+                               residual ? static_cast<float*>(out_ptr(c.outputs[2])) : nullptr, out_i32(c.outputs[0]),
+                               out_i32(c.outputs[1]), &d, s),
+              "HIP rmsnorm8");
+  if (numel(x.shape) != 0 && s.used()) synchronize(s);
+}
+
+// "linear8": x codes, x scales, weight codes, weight scales[, bias]; activation; output.
+// "gated_linear8": the same; outputs codes and scales.
+void linear8(const KernelCall& c, bool gated, Stream& s) {
+  c.expect(4, 5, 1, gated ? 2 : 1);
+  const Shape shape = shape_of_rows8(c, *c.tensors[0], *c.tensors[1]);
+  const Shape weights = shape_of_rows8(c, *c.tensors[2], *c.tensors[3]);
+  if (weights.size() != 2) c.refuse("weights must have rank 2");
+  if (weights[1] != shape.back()) c.refuse("weights must have the input's features");
+  if (gated && weights[0] % 2 != 0) c.refuse("weights must have as many gate rows as up rows");
+  tcx_hip_linear8_desc_t d{};
+  d.rows = rows_of(shape);
+  d.features = shape.back();
+  d.outputs = gated ? weights[0] / 2 : weights[0];
+  d.activation = static_cast<std::int32_t>(c.scalars[0]);
+  if (c.tensors.size() == 5) {
+    c.expect_dtype(*c.tensors[4], DType::kFloat32, "bias");
+    c.expect_shape(*c.tensors[4], Shape{weights[0]}, "bias (weight rows,)");
+    d.bias = f32(*c.tensors[4]);
+  }
+  const Shape result = with_last(shape, d.outputs);
+  if (gated) {
+    expect_code_outputs(c, 0, result);
+  } else {
+    c.expect_dtype(c.outputs[0], DType::kFloat32, "output");
+    c.expect_shape(c.outputs[0], result, "output");
+  }
+  c.expect_apart();
+  const Tensor x = on_boundary(*c.tensors[0]), w = on_boundary(*c.tensors[2]);
+  const std::size_t ws = gated ? tcx_hip_gated_linear8_workspace_bytes(&d) : tcx_hip_linear8_workspace_bytes(&d);
+  std::shared_ptr<HipBuffer> workspace;
+  if (ws != 0) {
+    auto created = HipBuffer::create(ws);
+    if (created) workspace = created.move_value();
+    else if (gated) throw std::runtime_error(created.status().message());
+  }
+  void* const at = workspace ? workspace->data() : nullptr;
+  if (gated)
+    ok_or_throw(tcx_hip_gated_linear8(i32(x), i32(*c.tensors[1]), i32(w), i32(*c.tensors[3]), out_i32(c.outputs[0]),
+                                      out_i32(c.outputs[1]), &d, at, workspace ? ws : 0, s),
+                "HIP gated_linear8");
+  else
+    ok_or_throw(tcx_hip_linear8(i32(x), i32(*c.tensors[1]), i32(w), i32(*c.tensors[3]), static_cast<float*>(out_ptr(c.outputs[0])),
+                                &d, at, workspace ? ws : 0, s),
+                "HIP linear8");
+  if (numel(result) != 0 && s.used()) synchronize(s);
+}
+
 // ------------------------------------------------------------ kernel class
 Status execute_builtin_kernel(const BackendExecution& e) {
   if (Status s = validate_kernel_execution_contract(e); !s.ok()) return s;
@@ -1465,7 +1603,8 @@ Status execute_builtin_kernel(const BackendExecution& e) {
   if (target.artifact_kind != KernelArtifactKind::kStaticLibrary || target.artifact != kStaticArtifact)
     return Status(StatusCode::kInvalidArgument, "HIP kernels must name the tensorcx_hip static library");
   static constexpr std::string_view kEntries[] = {"linear_bias_act", "bias_act", "window_attention", "cache4_attention",
-                                                  "cache4_store", "cache4_load", "beam_select", "beam_reorder"};
+                                                  "cache4_store", "cache4_load", "beam_select", "beam_reorder",
+                                                  "quantise8", "dequantise8", "rmsnorm8", "linear8", "gated_linear8"};
   if (std::find(std::begin(kEntries), std::end(kEntries), target.entry_point) == std::end(kEntries))
     return Status(StatusCode::kInvalidArgument, "unknown HIP built-in kernel entry point");
   std::vector<const Tensor*> tensors;
@@ -1486,7 +1625,11 @@ Status execute_builtin_kernel(const BackendExecution& e) {
     else if (target.entry_point == "cache4_store") cache_store(call, s);
     else if (target.entry_point == "cache4_load") cache_load(call, s);
     else if (target.entry_point == "beam_select") beam_select(call, s);
-    else beam_reorder(call, s);
+    else if (target.entry_point == "beam_reorder") beam_reorder(call, s);
+    else if (target.entry_point == "quantise8") quantise8(call, s);
+    else if (target.entry_point == "dequantise8") dequantise8(call, s);
+    else if (target.entry_point == "rmsnorm8") rmsnorm8(call, s);
+    else linear8(call, target.entry_point == "gated_linear8", s);
     return Status::Ok();
   }
   if (e.outputs.size() != 1) return Status(StatusCode::kInvalidArgument, "HIP built-in kernels write one output");

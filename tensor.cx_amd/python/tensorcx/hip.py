@@ -5,7 +5,7 @@ and "bias_act": act(x @ weight^T + bias) in one GEMM epilogue, and act(x + bias)
 in one pass. activation is "none", "silu" or "gelu"; results equal linear()
 followed by silu()/gelu() up to the exp/tanh implementation.
 
-The others are the operators of a decoding loop:
+Operators of a decoding loop:
 
 * ``window_attention``: attention in which a query sees a window of the last
   keys and a few first ones, with query heads that share a key head;
@@ -14,6 +14,14 @@ The others are the operators of a decoding loop:
   attention over them;
 * ``beam_select`` and ``beam_reorder``: beam search's choice over beams and
   vocabulary, and the states of the chosen beams.
+
+A layer's products with 8-bit operands, rows held as codes with a power of two for
+each 128 features:
+
+* ``quantise8`` and ``dequantise8``: float32 rows to that form, and back;
+* ``rmsnorm8``: a residual added, the root-mean-square norm, its output in that form;
+* ``linear8``: act(x @ weight^T + bias) of activations and weights in that form, as
+  float32; ``gated_linear8``: the gated half of a layer, its output in that form.
 
 They allocate their outputs and what workspace they use, and return when the
 result is there. Loops that keep buffers, run ahead or capture graphs call the C
@@ -199,3 +207,122 @@ def beam_reorder(states, beams):
     _core._kernel("beam_reorder", impls, [], outputs)
     results = tuple(Tensor(t) for t in outputs)
     return results[0] if single else results
+
+
+def _rows8(rows, name: str):
+    """The codes and scales of a pair, as quantise8 makes it."""
+    from . import Tensor
+    if not isinstance(rows, tuple) or len(rows) != 2 or not all(isinstance(t, Tensor) for t in rows):
+        raise TypeError(f"{name} must be a pair of codes and scales")
+    codes, scales = rows
+    if codes.dtype != "int32" or scales.dtype != "int32":
+        raise ValueError(f"{name} codes and scales must be int32")
+    if not codes.shape or len(scales.shape) != len(codes.shape) or codes.shape[-1] % 32 or \
+            scales.shape != (*codes.shape[:-1], (codes.shape[-1] // 32 + 3) // 4):
+        raise ValueError(f"{name} codes and scales do not belong together")
+    return codes, scales
+
+
+def _empty8(shape):
+    from . import _core
+    code_words, scale_words = _core._block8_words(shape[-1])
+    return [_core.empty([*shape[:-1], words], "int32") for words in (code_words, scale_words)]
+
+
+def _float_rows(tensor, name: str) -> None:
+    if tensor.dtype != "float32":
+        raise ValueError(f"{name} must be float32")
+    if not tensor.shape:
+        raise ValueError(f"{name} must have at least one axis")
+
+
+def quantise8(input):
+    """(codes, scales), int32 (..., 32 * blocks) and (..., ceil(blocks / 4)), of float32
+    (..., features): each value in 8-bit floating point (four bits of exponent, three
+    of mantissa), in units of a power of two that each block of 128 features has for
+    itself, the least that leaves its largest value at 448 units or below (2^-100 at
+    the least). Values are rounded to the nearest code, at most 2^-4 of themselves off;
+    NaN and infinities become NaN."""
+    from . import Tensor, _core, _inference
+    (x,) = _inference("quantise8", input)
+    _float_rows(input, "input")
+    outputs = _empty8(input.shape)
+    _core._kernel("quantise8", [x], [], outputs)
+    return tuple(Tensor(t) for t in outputs)
+
+
+def dequantise8(rows, features: int | None = None):
+    """The float32 (..., features) that a pair of codes and scales stands for (None: as
+    many features as its blocks hold)."""
+    from . import Tensor, _core, _inference
+    codes, scales = _rows8(rows, "rows")
+    impls = _inference("dequantise8", codes, scales)
+    held = 4 * codes.shape[-1]
+    features = held if features is None else _count(features, "features", 0)
+    if (features + 127) // 128 * 128 != held:
+        raise ValueError("features do not fill the blocks of the codes")
+    out = _core.empty([*codes.shape[:-1], features], "float32")
+    _core._kernel("dequantise8", impls, [], [out])
+    return Tensor(out)
+
+
+def _epsilon_bits(eps) -> int:
+    if isinstance(eps, (bool, np.bool_)) or not isinstance(eps, (int, float, np.integer, np.floating)):
+        raise TypeError("eps must be a real scalar")
+    try:
+        with np.errstate(over="ignore"):
+            narrowed = np.float32(float(eps))
+    except OverflowError:
+        raise ValueError("eps is out of range") from None
+    if not np.isfinite(narrowed) or narrowed < 0:
+        raise ValueError("eps must be finite and not negative")
+    return struct.unpack("<I", struct.pack("<f", narrowed))[0]
+
+
+def rmsnorm8(input, weight=None, eps: float = 1.0e-5, *, residual=None):
+    """(codes, scales) of y = s / sqrt(mean(s^2) + eps) * weight over the last axis, with
+    s = input + residual; with a residual (codes, scales, s). weight is (features,)."""
+    from . import Tensor, _core, _inference
+    inputs = (input,) + (() if residual is None else (residual,)) + (() if weight is None else (weight,))
+    impls = _inference("rmsnorm8", *inputs)
+    _float_rows(input, "input")
+    scalars = [_epsilon_bits(eps), int(residual is not None), int(weight is not None)]
+    outputs = _empty8(input.shape)
+    if residual is not None:
+        outputs.append(_core.empty(list(input.shape), "float32"))
+    _core._kernel("rmsnorm8", impls, scalars, outputs)
+    return tuple(Tensor(t) for t in outputs)
+
+
+def _product8(entry: str, input, weight, bias, activation: str):
+    from . import _inference
+    x, w = _rows8(input, "input"), _rows8(weight, "weight")
+    impls = _inference(entry, *x, *w, *(() if bias is None else (bias,)))
+    if len(w[0].shape) != 2:
+        raise ValueError("weight must have rank 2")
+    if w[0].shape[1] != x[0].shape[-1]:
+        raise ValueError("input and weight must have the same features")
+    return impls, [_act(activation)], x[0].shape[:-1], w[0].shape[0]
+
+
+def linear8(input, weight, bias=None, activation: str = "none"):
+    """act(input @ weight^T + bias) as float32 (..., outputs) of pairs of codes and scales:
+    input (..., features), weight (outputs, features). The products are exact, their
+    sums float32. activation is "none", "silu" or "gelu"."""
+    from . import Tensor, _core
+    impls, scalars, lead, rows = _product8("linear8", input, weight, bias, activation)
+    out = _core.empty([*lead, rows], "float32")
+    _core._kernel("linear8", impls, scalars, [out])
+    return Tensor(out)
+
+
+def gated_linear8(input, weight, bias=None, activation: str = "silu"):
+    """(codes, scales) of act(input @ gate^T + bias) * (input @ up^T + bias'), for weight
+    rows (and biases) of gate, then as many of up."""
+    from . import Tensor, _core
+    impls, scalars, lead, rows = _product8("gated_linear8", input, weight, bias, activation)
+    if rows % 2:
+        raise ValueError("weight must have as many gate rows as up rows")
+    outputs = _empty8((*lead, rows // 2))
+    _core._kernel("gated_linear8", impls, scalars, outputs)
+    return tuple(Tensor(t) for t in outputs)

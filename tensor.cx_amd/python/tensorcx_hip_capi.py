@@ -52,7 +52,9 @@ EXPORTS = [
     "tcx_hip_window_attention_workspace_bytes", "tcx_hip_window_attention_f32", "tcx_hip_cache4_words",
     "tcx_hip_cache4_store", "tcx_hip_cache4_load", "tcx_hip_cache4_attention_workspace_bytes",
     "tcx_hip_cache4_attention_f32", "tcx_hip_beam_select_workspace_bytes", "tcx_hip_beam_select_f32",
-    "tcx_hip_beam_reorder",
+    "tcx_hip_beam_reorder", "tcx_hip_block8_code_words", "tcx_hip_block8_scale_words", "tcx_hip_quantise8",
+    "tcx_hip_dequantise8", "tcx_hip_rmsnorm8", "tcx_hip_linear8_workspace_bytes", "tcx_hip_linear8",
+    "tcx_hip_gated_linear8_workspace_bytes", "tcx_hip_gated_linear8",
 ]
 
 
@@ -96,6 +98,16 @@ class Cache4StoreDesc(ctypes.Structure):
 ALLOCATE_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.POINTER(ctypes.c_void_p), ctypes.c_size_t)
 FREE_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p)
 CLEAR_FN = ctypes.CFUNCTYPE(ctypes.c_int)
+
+
+class Rmsnorm8Desc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("features", ctypes.c_int64), ("epsilon", ctypes.c_float),
+                ("x_stride", ctypes.c_int64), ("residual_stride", ctypes.c_int64), ("sum_stride", ctypes.c_int64)]
+
+
+class Linear8Desc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("features", ctypes.c_int64), ("outputs", ctypes.c_int64),
+                ("bias", ctypes.c_void_p), ("activation", ctypes.c_int32), ("out_stride", ctypes.c_int64)]
 
 
 class PoolRuntime(ctypes.Structure):
@@ -185,6 +197,16 @@ def lib() -> ctypes.CDLL:
         L.tcx_hip_beam_select_workspace_bytes.restype = sz
         L.tcx_hip_beam_select_f32.argtypes = [vp, vp, vp, ctypes.c_int32, vp, vp, vp, i64, i64, i64, i64, vp, sz, vp]
         L.tcx_hip_beam_reorder.argtypes = [vp, vp, vp, ctypes.c_int32, vp, i64, i64, i64, vp, vp]
+        for name in ("tcx_hip_block8_code_words", "tcx_hip_block8_scale_words"):
+            getattr(L, name).argtypes, getattr(L, name).restype = [i64], i64
+        L.tcx_hip_quantise8.argtypes = [vp, vp, vp, i64, i64, i64, vp]
+        L.tcx_hip_dequantise8.argtypes = [vp, vp, vp, i64, i64, i64, vp]
+        L.tcx_hip_rmsnorm8.argtypes = [vp, vp, vp, vp, vp, vp, ctypes.POINTER(Rmsnorm8Desc), vp]
+        for name in ("tcx_hip_linear8", "tcx_hip_gated_linear8"):
+            query = getattr(L, name + "_workspace_bytes")
+            query.argtypes, query.restype = [ctypes.POINTER(Linear8Desc)], sz
+        L.tcx_hip_linear8.argtypes = [vp, vp, vp, vp, vp, ctypes.POINTER(Linear8Desc), vp, sz, vp]
+        L.tcx_hip_gated_linear8.argtypes = [vp, vp, vp, vp, vp, vp, ctypes.POINTER(Linear8Desc), vp, sz, vp]
         _LIB = L
     return _LIB
 
@@ -503,3 +525,57 @@ def beam_reorder(plan: BeamReorderPlan, index: int, batch: int, beams: int, coun
                  s=None) -> None:
     check(lib().tcx_hip_beam_reorder(plan.sources, plan.targets, plan.row_bytes, len(plan.sources), index, batch, beams,
                                      count, flag, _on(s)), "beam_reorder")
+
+
+# ------------------------------------------------------------------ 8-bit rows
+def block8_words(features: int) -> tuple[int, int]:
+    """int32 words of a row's codes and of its scales."""
+    return lib().tcx_hip_block8_code_words(features), lib().tcx_hip_block8_scale_words(features)
+
+
+def quantise8(x: int, codes: int, scales: int, rows: int, features: int, x_stride: int = 0, s=None) -> None:
+    check(lib().tcx_hip_quantise8(x, codes, scales, rows, features, x_stride, _on(s)), "quantise8")
+
+
+def dequantise8(codes: int, scales: int, out: int, rows: int, features: int, out_stride: int = 0, s=None) -> None:
+    check(lib().tcx_hip_dequantise8(codes, scales, out, rows, features, out_stride, _on(s)), "dequantise8")
+
+
+def rmsnorm8_desc(rows: int, features: int, epsilon: float = 1e-5, *, x_stride: int = 0, residual_stride: int = 0,
+                  sum_stride: int = 0) -> Rmsnorm8Desc:
+    return Rmsnorm8Desc(rows, features, epsilon, x_stride, residual_stride, sum_stride)
+
+
+def rmsnorm8(x: int, codes: int, scales: int, desc: Rmsnorm8Desc, *, residual: int | None = None, weight: int | None = None,
+             sum: int | None = None, s=None) -> None:
+    check(lib().tcx_hip_rmsnorm8(x, residual, weight, sum, codes, scales, ctypes.byref(desc), _on(s)), "rmsnorm8")
+
+
+def linear8_desc(rows: int, features: int, outputs: int, *, bias: int | None = None, activation: str = "none",
+                 out_stride: int = 0) -> Linear8Desc:
+    """Arguments of linear8 and gated_linear8."""
+    return Linear8Desc(rows, features, outputs, bias, ACT[activation], out_stride)
+
+
+def linear8_workspace_bytes(desc: Linear8Desc, gated: bool = False) -> int:
+    """Bytes of workspace that linear8 can use (that gated_linear8 needs, with `gated`)."""
+    query = lib().tcx_hip_gated_linear8_workspace_bytes if gated else lib().tcx_hip_linear8_workspace_bytes
+    return query(ctypes.byref(desc))
+
+
+def linear8_workspace(desc: Linear8Desc, gated: bool = False) -> DeviceBuffer | None:
+    """A workspace of that size (None when none is of use)."""
+    nbytes = linear8_workspace_bytes(desc, gated)
+    return DeviceBuffer(nbytes) if nbytes else None
+
+
+def linear8(x_codes: int, x_scales: int, w_codes: int, w_scales: int, out: int, desc: Linear8Desc, workspace=None,
+            s=None) -> None:
+    check(lib().tcx_hip_linear8(x_codes, x_scales, w_codes, w_scales, out, ctypes.byref(desc), *_ws_args(workspace), _on(s)),
+          "linear8")
+
+
+def gated_linear8(x_codes: int, x_scales: int, w_codes: int, w_scales: int, codes: int, scales: int, desc: Linear8Desc,
+                  workspace=None, s=None) -> None:
+    check(lib().tcx_hip_gated_linear8(x_codes, x_scales, w_codes, w_scales, codes, scales, ctypes.byref(desc),
+                                      *_ws_args(workspace), _on(s)), "gated_linear8")
