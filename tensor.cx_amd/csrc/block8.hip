@@ -81,9 +81,6 @@ __device__ __forceinline__ float inverse_rms(const Norm8& a, float squares) {
   return 1.0F / sqrtf(squares / static_cast<float>(a.features) + a.epsilon);
 }
 
-__device__ __forceinline__ float4_t add4(float4_t p, float4_t q) {
-  return float4_t{p[0] + q[0], p[1] + q[1], p[2] + q[2], p[3] + q[3]};
-}
 __device__ __forceinline__ float squares4(float4_t v) { return (v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3]); }
 
 // A block a row, U groups of it in each wave's registers: one read of x and the

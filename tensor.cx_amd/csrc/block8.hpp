@@ -42,6 +42,10 @@ __device__ __forceinline__ void store_features(float* row, int f, int features, 
     if (f + e < features) row[f + e] = v[e];
 }
 
+__device__ __forceinline__ float4_t add4(float4_t p, float4_t q) {
+  return float4_t{p[0] + q[0], p[1] + q[1], p[2] + q[2], p[3] + q[3]};
+}
+
 // Maximum over the sixteen lanes of a group, in all of them.
 __device__ __forceinline__ std::uint32_t lanes16_max(std::uint32_t x) {
   auto take = [&]<int kControl>() {

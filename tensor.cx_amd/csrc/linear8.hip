@@ -31,23 +31,29 @@ struct Product8 {
   int m, n, blocks, pitch, scale_pitch;  // blocks of 128 features; bytes and words between rows
   int activation;
   int tiles_m, tiles_n;
+  FastDiv by_group;  // work items in eight tile rows
+  // Sums over shares of the features, one to a row of blocks: share s has `each` blocks
+  // (or units of four) and one more if s < extra, and its sums go to parts [s][m][n].
+  float* parts;  // null: one share, whose results go to out
+  int each, extra;
 };
+// The features of a share: [first, last).
+struct Share8 {
+  int first, last;
+};
+__device__ __forceinline__ Share8 share_of(const Product8& a, int s) {
+  const int first = s * a.each + min(s, a.extra);
+  return {first, first + a.each + (s < a.extra ? 1 : 0)};
+}
 
-// Sixteen codes as two operands of eight.
-struct Wide8 {
-  bf8_t half[2];
-};
-__device__ __forceinline__ Wide8 widen(int4_t codes, float unit) {
-  Wide8 r;
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const bf2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[2 * s], unit, false);
-    const bf2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[2 * s], unit, true);
-    const bf2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[2 * s + 1], unit, false);
-    const bf2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[2 * s + 1], unit, true);
-    r.half[s] = bf8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-  }
-  return r;
+// Codes 8 h to 8 h + 7 of sixteen as an operand.
+template <int h>
+__device__ __forceinline__ bf8_t widen(int4_t codes, float unit) {
+  const bf2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[2 * h], unit, false);
+  const bf2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[2 * h], unit, true);
+  const bf2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[2 * h + 1], unit, false);
+  const bf2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[2 * h + 1], unit, true);
+  return bf8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 // The unit of block kt, from the word of exponents that has it.
 __device__ __forceinline__ float unit_of(std::uint32_t word, int kt) {
@@ -60,11 +66,22 @@ __device__ __forceinline__ float unit_of(std::uint32_t word, int kt) {
 struct Tile8 {
   int m, n;
 };
-__device__ __forceinline__ Tile8 tile_of(int block, int tiles_m, int tiles_n) {
-  const int total = tiles_m * tiles_n, share = total / 8, rest = total % 8, xcd = block % 8;
-  const int id = xcd * share + min(xcd, rest) + block / 8;
-  const int width = 8 * tiles_n, group = id / width, first = group * 8, deep = min(tiles_m - first, 8), in = id - group * width;
-  return {first + in % deep, in / deep};
+__device__ __forceinline__ Tile8 tile_of(const Product8& a, int block) {
+  const int total = a.tiles_m * a.tiles_n, share = total >> 3, rest = total & 7, xcd = block & 7;
+  const int id = xcd * share + min(xcd, rest) + (block >> 3);
+  const int group = static_cast<int>(a.by_group(static_cast<std::uint32_t>(id))), in = id - group * 8 * a.tiles_n;
+  const int deep = min(a.tiles_m - group * 8, 8);
+  if (deep == 8) return {group * 8 + (in & 7), in >> 3};
+  return {group * 8 + in % deep, in / deep};
+}
+
+// Rows [first, first + rows) of an operand's codes.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const std::uint8_t* codes, int first, int rows, int pitch) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<std::uint8_t*>(codes + static_cast<std::int64_t>(first) * pitch),
+                                           static_cast<short>(0), rows * pitch, 0x00020000);
+}
+__device__ __forceinline__ int4_t load16(__amdgpu_buffer_rsrc_t r, int voffset, int soffset) {
+  return __builtin_bit_cast(int4_t, __builtin_amdgcn_raw_buffer_load_b128(r, voffset, soffset, 0));
 }
 
 // Sixteen bytes a lane straight into LDS, lane after lane from `lds` on.
@@ -72,130 +89,491 @@ __device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, void* lds, 
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voffset, soffset, 0, 0);
 }
 
-// A tile of kM x kN results, a wave's part of it kWM x kWN in 32 x 32 blocks. Each
-// step brings a block of 128 features of the tile's rows from memory straight into
-// one of two buffers in LDS while the other is computed. Row r's sixteen-byte pieces
-// stand in the order piece ^ (r & 7), so that the reads of eight neighbouring rows
-// lie in different banks.
-template <int kM, int kN, int kWM, int kWN>
-__global__ __launch_bounds__(kM / kWM * (kN / kWN) * 64) void product_kernel(Product8 a) {
-  constexpr int kWavesN = kN / kWN, kWaves = kM / kWM * kWavesN, kI = kWM / 32, kJ = kWN / 32;
-  constexpr int kRows = kM + kN;  // LDS rows of a buffer: x, then w
-  constexpr int kLoads = kRows / 8 / kWaves;
-  static_assert(kM % (8 * kWaves) == 0 && kN % (8 * kWaves) == 0, "a load is of one operand");
-  __shared__ __attribute__((aligned(1024))) std::uint8_t lds[2][kRows * 128];
+// Four bytes a lane straight into LDS.
+__device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t r, void* lds, int voffset, int soffset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 4, voffset, soffset, 0, 0);
+}
+// Waits until at most `count` of this wave's loads are under way.
+template <int kCount>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(kCount < 64);
+  __builtin_amdgcn_s_waitcnt((kCount & 15) | (7 << 4) | (15 << 8) | ((kCount >> 4) << 14));
+}
 
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Tile8 tile = tile_of(blockIdx.x, a.tiles_m, a.tiles_n);
+// The block's waves meet, their reads of LDS done; loads may still be under way.
+__device__ __forceinline__ void block_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// A wave's own reads and writes of LDS are done.
+__device__ __forceinline__ void wave_lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// A tile of kM x kN results, a wave's part of it kWM x kWN in 32 x 32 blocks. Each
+// step takes a block of 128 features of the tile's rows, brought from memory straight
+// into one of kStages buffers in LDS, kStages - 1 steps ahead. Row r's sixteen-byte
+// pieces stand in the order piece ^ (r & 7), so that the reads of eight neighbouring
+// rows lie in different banks. Words of exponents, of four steps each, have two
+// buffers of their own.
+//
+// With kSets > 1 a wave has the whole tile to itself, for every kSets-th step, with LDS of
+// its own: no barriers until the waves' sums meet at the end, and for small tiles half the
+// conversions that waves with a quarter of the tile each would make.
+//
+// The features may be split over the grid's rows (Product8::parts).
+template <int kM, int kN, int kWM, int kWN, int kSets, int kStages>
+struct Tiles8 {
+  static constexpr int kWavesN = kN / kWN, kWaves = kM / kWM * kWavesN, kThreads = 64 * kWaves * kSets;  // waves of a set
+  static constexpr int kI = kWM / 32, kJ = kWN / 32;
+  static constexpr int kRows = kM + kN;  // LDS rows of a buffer: x, then w
+  static constexpr int kLoads = kRows / 8 / kWaves;
+  static constexpr int kScaleX = (kM + 63) / 64 * 64;  // words of exponents before those of w
+  static constexpr int kScaleLoads = (kScaleX + kN) / 64;
+  static constexpr int kScaleBuffers = kSets == 1 ? 2 : kStages;
+  static constexpr int kStageBytes = kRows * 128, kScales = kStageBytes * kStages;  // where the words of exponents are
+  static constexpr int kScaleBytes = kScaleLoads * 256;
+  static constexpr int kSetBytes = kScales + kScaleBuffers * kScaleBytes, kLds = kSetBytes * kSets;
+  static_assert(kLds <= 160 * 1024 && kStages <= 4);
+  static_assert(kSets == 1 ? kM % (8 * kWaves) == 0 && kN % (8 * kWaves) == 0 && kScaleLoads <= kWaves && kM % 64 == 0 : kWaves == 1);
+  // Results on their way out through LDS: rows 4 apart lie in different halves of the banks.
+  static constexpr int kStride = kWN + 8;
+  static_assert(kSets == 1 ? kWaves * 32 * kStride * 4 <= kScales : kM * kStride * 4 <= kScales);
+};
+template <int kM, int kN, int kWM, int kWN, int kSets, int kStages>
+__global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads)) void product_kernel(Product8 a) {
+  using T = Tiles8<kM, kN, kWM, kWN, kSets, kStages>;
+  constexpr int kWavesN = T::kWavesN, kWaves = T::kWaves, kI = T::kI, kJ = T::kJ, kLoads = T::kLoads;
+  constexpr int kScaled = kSets == 1 ? 0 : T::kScaleLoads;  // loads of exponents in every step
+  __shared__ __attribute__((aligned(1024))) std::uint8_t memory[T::kLds];
+
+  const int lane = threadIdx.x & 63, thread_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int set = kSets == 1 ? 0 : thread_wave, wave = kSets == 1 ? thread_wave : 0;
+  std::uint8_t* const lds = memory + set * T::kSetBytes;
+  const Tile8 tile = tile_of(a, static_cast<int>(blockIdx.x));
+  const auto [share_first, last] = share_of(a, static_cast<int>(blockIdx.y));
+  const int first = share_first + set;
   const int m0 = tile.m * kM, n0 = tile.n * kN;
   const int r = lane & 31, g = lane >> 5;
 
   // Loads: instruction t of a wave brings rows 8 (t kWaves + wave) on of the buffer; rows
   // past the operand's end are its last one again.
-  const auto x_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<std::uint8_t*>(a.x + static_cast<std::int64_t>(m0) * a.pitch), static_cast<short>(0),
-      min(a.m - m0, kM) * a.pitch, 0x00020000);
-  const auto w_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<std::uint8_t*>(a.w + static_cast<std::int64_t>(n0) * a.pitch), static_cast<short>(0),
-      min(a.n - n0, kN) * a.pitch, 0x00020000);
+  const int m_last = min(a.m - m0, kM) - 1, n_last = min(a.n - n0, kN) - 1;
   int offset[kLoads];
+  bool of_x[kLoads];
 #pragma unroll
   for (int t = 0; t < kLoads; ++t) {
-    const int first = 8 * (t * kWaves + wave), row = first + (lane >> 3);
-    const int in = t * 8 * kWaves < kM ? min(row, a.m - m0 - 1) : min(row - kM, a.n - n0 - 1);
-    offset[t] = in * a.pitch + (((lane & 7) ^ (lane >> 3)) << 4);
+    const int at = 8 * (t * kWaves + wave), row = at + (lane >> 3);
+    of_x[t] = kM % (8 * kWaves) == 0 ? t * 8 * kWaves < kM : at < kM;
+    offset[t] = (of_x[t] ? min(row, m_last) : min(row - kM, n_last)) * a.pitch + (((lane & 7) ^ (lane >> 3)) << 4);
   }
-  auto load = [&](int kt, int buffer) {
+  // Exponents: words of 64 rows a load, one for each of the first waves, or all for a set's one.
+  int scale_offset[kSets == 1 ? 1 : T::kScaleLoads];
 #pragma unroll
-    for (int t = 0; t < kLoads; ++t) {
-      const int first = 8 * (t * kWaves + wave);
-      load_lds16(t * 8 * kWaves < kM ? x_rsrc : w_rsrc, lds[buffer] + first * 128, offset[t], kt * 128);
+  for (int t = 0; t < (kSets == 1 ? 1 : T::kScaleLoads); ++t) {
+    const int row = 64 * (kSets == 1 ? wave : t) + lane;
+    scale_offset[t] = 4 * a.scale_pitch * (row < T::kScaleX ? min(row, m_last) : min(row - T::kScaleX, n_last));
+  }
+  const auto xs_rsrc = row_buffer(reinterpret_cast<const std::uint8_t*>(a.x_scale), m0, m_last + 1, 4 * a.scale_pitch);
+  const auto ws_rsrc = row_buffer(reinterpret_cast<const std::uint8_t*>(a.w_scale), n0, n_last + 1, 4 * a.scale_pitch);
+  // Loads t0 to t1 - 1 of step kt. Past the last step they are issued all the same, without
+  // memory behind them, so that every step counts as many.
+  auto load = [&](int kt, int buffer, int t0, int t1) {
+    std::uint8_t* const at = lds + buffer * T::kStageBytes;
+    const bool any = kt < last;
+    const auto x_now = row_buffer(a.x, m0, any ? m_last + 1 : 0, a.pitch), w_now = row_buffer(a.w, n0, any ? n_last + 1 : 0, a.pitch);
+#pragma unroll
+    for (int t = t0; t < t1; ++t)
+      load_lds16(of_x[t] ? x_now : w_now, at + 8 * (t * kWaves + wave) * 128, offset[t], any ? kt * 128 : 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto scale_buffer = [&](int kt, int buffer) { return T::kScales + (kSets == 1 ? (kt >> 2) & 1 : buffer) * T::kScaleBytes; };
+  auto load_scales = [&](int kt, int buffer) {  // of four steps, with the first of them; a set's with every step
+    if constexpr (kSets == 1) {
+      if (kt < last && wave < T::kScaleLoads)
+        load_lds4(64 * wave < kM ? xs_rsrc : ws_rsrc, lds + scale_buffer(kt, buffer) + 256 * wave, scale_offset[0], (kt >> 2) * 4);
+    } else {
+      const auto scales = [&](const std::uint32_t* p, int at, int rows) {
+        return row_buffer(reinterpret_cast<const std::uint8_t*>(p), at, kt < last ? rows : 0, 4 * a.scale_pitch);
+      };
+      const auto x_now = scales(a.x_scale, m0, m_last + 1), w_now = scales(a.w_scale, n0, n_last + 1);
+#pragma unroll
+      for (int t = 0; t < T::kScaleLoads; ++t) {
+        std::uint8_t* const to = lds + scale_buffer(kt, buffer) + 256 * t;
+        load_lds4(64 * t < T::kScaleX ? x_now : w_now, to, scale_offset[t], kt < last ? (kt >> 2) * 4 : 0);
+      }
     }
   };
 
-  // Exponents: a lane's rows of the tile, a word every four steps.
   const int wm = wave / kWavesN * kWM, wn = wave % kWavesN * kWN;
-  const std::uint32_t* x_scale[kI];
-  const std::uint32_t* w_scale[kJ];
-  std::uint32_t x_word[kI], w_word[kJ];
-#pragma unroll
-  for (int i = 0; i < kI; ++i)
-    x_scale[i] = a.x_scale + static_cast<std::int64_t>(min(m0 + wm + 32 * i + r, a.m - 1)) * a.scale_pitch;
-#pragma unroll
-  for (int j = 0; j < kJ; ++j)
-    w_scale[j] = a.w_scale + static_cast<std::int64_t>(min(n0 + wn + 32 * j + r, a.n - 1)) * a.scale_pitch;
-
   acc16_t acc[kI][kJ];
 #pragma unroll
   for (int i = 0; i < kI; ++i)
 #pragma unroll
     for (int j = 0; j < kJ; ++j) acc[i][j] = acc16_t{};
 
-  if (a.blocks > 0) load(0, 0);
-  for (int kt = 0; kt < a.blocks; ++kt) {
-    if ((kt & 3) == 0) {
+  // A step is four pairs of sixteen features, a pair's operands read as sixteen-byte
+  // pieces of codes. While the matrix instructions of one half of a pair run, the codes
+  // of the next half are widened; the next pair's are read during the pair, the next
+  // step's first ones during the last, behind the step's one barrier: there every wave
+  // has read all of its step, so that the buffer can take the step kStages further on.
+  struct Codes {
+    int4_t x[kI], w[kJ];
+  };
+  struct Operands {
+    bf8_t x[kI], w[kJ];
+  };
+  float x_unit[kI], w_unit[kJ];
+  auto read = [&](Codes& c, int buffer, int p) {
+    const std::uint8_t* const at = lds + buffer * T::kStageBytes + (((2 * p + g) ^ (r & 7)) << 4);
 #pragma unroll
-      for (int i = 0; i < kI; ++i) x_word[i] = x_scale[i][kt >> 2];
+    for (int i = 0; i < kI; ++i) c.x[i] = *reinterpret_cast<const int4_t*>(at + (wm + 32 * i + r) * 128);
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) w_word[j] = w_scale[j][kt >> 2];
-    }
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (kt + 1 < a.blocks) load(kt + 1, (kt + 1) & 1);
-    const std::uint8_t* x_lds = lds[kt & 1] + (wm + r) * 128;
-    const std::uint8_t* w_lds = lds[kt & 1] + (kM + wn + r) * 128;
+    for (int j = 0; j < kJ; ++j) c.w[j] = *reinterpret_cast<const int4_t*>(at + (kM + wn + 32 * j + r) * 128);
+  };
+  auto read_units = [&](int kt, int buffer) {
+    const std::uint32_t* const scales = reinterpret_cast<const std::uint32_t*>(lds + scale_buffer(kt, buffer));
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int piece = ((2 * q + g) ^ (r & 7)) << 4;
-      Wide8 x[kI], w[kJ];
+    for (int i = 0; i < kI; ++i) x_unit[i] = unit_of(scales[wm + 32 * i + r], kt);
 #pragma unroll
-      for (int i = 0; i < kI; ++i) x[i] = widen(*reinterpret_cast<const int4_t*>(x_lds + i * 4096 + piece), unit_of(x_word[i], kt));
+    for (int j = 0; j < kJ; ++j) w_unit[j] = unit_of(scales[T::kScaleX + wn + 32 * j + r], kt);
+  };
+  auto widen_all = [&]<int h>(Operands& o, const Codes& c) {
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) w[j] = widen(*reinterpret_cast<const int4_t*>(w_lds + j * 4096 + piece), unit_of(w_word[j], kt));
+    for (int i = 0; i < kI; ++i) o.x[i] = widen<h>(c.x[i], x_unit[i]);
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int i = 0; i < kI; ++i)
-#pragma unroll
-          for (int j = 0; j < kJ; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[i].half[s], w[j].half[s], acc[i][j], 0, 0, 0);
-    }
-  }
-
-  // Lane (r, g) has column r of rows 8 (e / 4) + 4 g + e % 4 of each block.
-#pragma unroll
-  for (int j = 0; j < kJ; ++j) {
-    const int n = n0 + wn + 32 * j + r;
-    if (n >= a.n) continue;
-    const float bias = a.bias != nullptr ? a.bias[n] : 0.0F;
+    for (int j = 0; j < kJ; ++j) o.w[j] = widen<h>(c.w[j], w_unit[j]);
+  };
+  auto multiply = [&](const Operands& o) {
 #pragma unroll
     for (int i = 0; i < kI; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int m = m0 + wm + 32 * i + 8 * (e / 4) + 4 * g + e % 4;
-        if (m < a.m) a.out[static_cast<std::int64_t>(m) * a.out_stride + n] = activate8(acc[i][j][e] + bias, a.activation);
+      for (int j = 0; j < kJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o.x[i], o.w[j], acc[i][j], 0, 0, 0);
+  };
+  // Order: loads, reads of LDS, then matrix instructions with conversions between them, as
+  // many to each, the first `alone` without.
+  constexpr int kProducts = kI * kJ, kConversions = (kI + kJ) * 4;
+  auto order = [&]<int kReads, int kAlone>() {
+    if constexpr (kReads > 0) __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+    if constexpr (kAlone > 0) __builtin_amdgcn_sched_group_barrier(0x008, kAlone, 0);
+#pragma unroll
+    for (int t = kAlone; t < kProducts; ++t) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, (kConversions + kProducts - kAlone - 1) / (kProducts - kAlone), 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // A step's loads are issued in four parts: all at once they keep a wave from its matrix
+  // instructions for a quarter of a step.
+  constexpr int kPart = (kLoads + 3) / 4;
+  auto part = [&](int i) { return min(i * kPart, kLoads); };
+
+  auto meet = [&] {
+    if constexpr (kSets == 1) block_barrier();
+    else wave_lds_done();
+  };
+
+#pragma unroll
+  for (int t = 0; t < kStages; ++t) {
+    const int kt = first + t * kSets;
+    if (kSets > 1 || t == 0 || (kt & 3) == 0) load_scales(kt, t);
+    load(kt, t, 0, t + 1 < kStages ? kLoads : part(1));  // the rest of the last one's in the first step
+  }
+  Codes codes;
+  Operands low, high;
+  wait_loads<(kStages - 2) * (kLoads + kScaled) + kScaled + kPart>();
+  meet();
+  read(codes, 0, 0);
+  read_units(first, 0);
+  widen_all.template operator()<0>(low, codes);
+  int buffer = 0, before = kStages - 1;  // of this step and the one before
+  for (int kt = first; kt < last; kt += kSets) {
+    const int next = buffer + 1 == kStages ? 0 : buffer + 1;
+    const int behind = kt + (kStages - 1) * kSets, ahead = behind + kSets;  // loads that the step before began; that this one begins
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      Codes after;
+      if (p < 2) load(behind, before, part(1 + 2 * p), part(2 + 2 * p));
+      read(after, buffer, p + 1);
+      multiply(low);
+      widen_all.template operator()<1>(high, codes);
+      order.template operator()<kI + kJ, 0>();
+      if (p < 1) load(behind, before, part(2), part(3));
+      multiply(high);
+      widen_all.template operator()<0>(low, after);
+      order.template operator()<0, 0>();
+      codes = after;
+    }
+    multiply(low);
+    widen_all.template operator()<1>(high, codes);
+    order.template operator()<0, 0>();
+    wait_loads<(kStages - 2) * (kLoads + kScaled)>();
+    meet();
+    if (kSets > 1 || (ahead & 3) == 0) load_scales(ahead, buffer);
+    load(ahead, buffer, 0, part(1));
+    read(codes, next, 0);
+    read_units(kt + kSets, next);
+    multiply(high);
+    widen_all.template operator()<0>(low, codes);
+    order.template operator()<kI + kJ, kProducts / 2>();
+    before = buffer;
+    buffer = next;
+  }
+  wait_loads<0>();
+
+  // Lane (r, g) has column r of rows 8 (e / 4) + 4 g + e % 4 of each 32 x 32. They pass
+  // through LDS, so that a lane stores four results of a row, and that the activation
+  // stands in the code few times, not once for each register (which cost 2.6 us in
+  // fetching instructions).
+  const bool whole = a.parts == nullptr;
+  float* const out = whole ? a.out : a.parts + static_cast<std::int64_t>(blockIdx.y) * a.m * a.n;
+  const std::int64_t stride = whole ? a.out_stride : a.n;
+  const float* const bias_row = whole ? a.bias : nullptr;
+  const int activation = whole ? a.activation : TCX_ACT_NONE;
+  auto give = [&](float* to, int i, int row0) {
+#pragma unroll
+    for (int j = 0; j < kJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) to[(row0 + 8 * (e / 4) + 4 * g + e % 4) * T::kStride + 32 * j + r] = acc[i][j][e];
+  };
+  auto store = [&](float4_t v, int m, int n, float4_t bias) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = activate8(v[e] + bias[e], activation);
+    store_features(out + m * stride, n, a.n, v);
+  };
+  const float4_t none = {0.0F, 0.0F, 0.0F, 0.0F};
+  constexpr int kAcross = kWN / 4;  // lanes to a row
+  const int column = lane % kAcross * 4;
+  if constexpr (kSets == 1) {  // 32 rows at a time, each wave on its own
+    float* const turn = reinterpret_cast<float*>(lds) + wave * 32 * T::kStride;
+    block_barrier();  // the buffers are done with
+    const int n = n0 + wn + column;
+    const float4_t bias = bias_row != nullptr ? load_features(bias_row, n, a.n) : none;
+#pragma unroll
+    for (int i = 0; i < kI; ++i) {
+      give(turn, i, 0);
+      wave_lds_done();
+#pragma unroll 1
+      for (int row = lane / kAcross; row < 32; row += 64 / kAcross) {
+        const int m = m0 + wm + 32 * i + row;
+        if (m >= a.m) break;
+        store(*reinterpret_cast<const float4_t*>(turn + row * T::kStride + column), m, n, bias);
       }
+      wave_lds_done();
+    }
+  } else {  // every wave the tile's sums in its own LDS, then all of them rows of the whole
+#pragma unroll
+    for (int i = 0; i < kI; ++i) give(reinterpret_cast<float*>(lds), i, 32 * i);
+    block_barrier();
+    const int n = n0 + column;
+    const float4_t bias = bias_row != nullptr ? load_features(bias_row, n, a.n) : none;
+#pragma unroll 1
+    for (int row = static_cast<int>(threadIdx.x) / kAcross; row < kM; row += T::kThreads / kAcross) {
+      const int m = m0 + row;
+      if (m >= a.m) break;
+      float4_t v = none;
+#pragma unroll
+      for (int other = 0; other < kSets; ++other)
+        v = add4(v, *reinterpret_cast<const float4_t*>(reinterpret_cast<const float*>(memory + other * T::kSetBytes) + row * T::kStride + column));
+      store(v, m, n, bias);
+    }
   }
 }
 
-template <int kM, int kN, int kWM, int kWN>
-int launch_product(Product8 a, hipStream_t s) {
+void share_out(Product8& a, int units, int splits, float* parts) {
+  a.parts = parts;
+  a.each = units / splits;
+  a.extra = units % splits;
+}
+
+template <int kM, int kN, int kWM, int kWN, int kSets, int kStages>
+int launch_product(Product8 a, int splits, float* parts, hipStream_t s) {
   a.tiles_m = (a.m + kM - 1) / kM;
   a.tiles_n = (a.n + kN - 1) / kN;
-  constexpr int kThreads = kM / kWM * (kN / kWN) * 64;
+  a.by_group = FastDiv(static_cast<std::uint32_t>(8 * a.tiles_n));
+  share_out(a, a.blocks, splits, parts);
+  constexpr int kThreads = Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads;
   const std::int64_t tiles = static_cast<std::int64_t>(a.tiles_m) * a.tiles_n;
-  if (tiles * kThreads > kMaxLaunchWorkItems || tiles >= (std::int64_t{1} << 30))
+  if (tiles * splits * kThreads > kMaxLaunchWorkItems || tiles >= (std::int64_t{1} << 30))
     return fail(TCX_INVALID_ARGUMENT, "linear8 has too many results");
-  hipLaunchKernelGGL((product_kernel<kM, kN, kWM, kWN>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL((product_kernel<kM, kN, kWM, kWN, kSets, kStages>), dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(splits)),
+                     dim3(kThreads), 0, s, a);
   return check(hipGetLastError(), "linear8 launch");
 }
 
-// act(gate) * up of float32 rows [gate | up], in 8 bits: a wave a group of four blocks.
+// Few rows: each weight is read once, straight into the registers that multiply it.
+// The eight waves of a block share the features of a tile of sixteen weights' rows: wave
+// p takes units (four blocks of 128) p, p + 8 and so on, kU of them, whose part of x it
+// keeps in registers from tile to tile while the next unit's weights are under way.
+// Lane (r, g) holds 16-byte pieces g and 4 + g of each block of row r. The waves' sums
+// of a tile meet in LDS.
+// The units may be split over the grid's rows (Product8::parts).
+template <int kT, int kU>
+__global__ __launch_bounds__(512) void few_rows_kernel(Product8 a) {
+  __shared__ float4_t sums[2][8][kT][64];
+  constexpr int kStaged = 8;
+  __shared__ int4_t stages[kT == 1 && kU == 1 ? 8 : 1][kT == 1 && kU == 1 ? kStaged * 32 : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const auto [first, units] = share_of(a, static_cast<int>(blockIdx.y));
+
+  struct Weights {
+    int4_t piece[8];
+    std::uint32_t word;
+  };
+  auto load = [&](Weights& w, int tile, int u) {
+    const int rows = min(a.n - 16 * tile, 16), unit = min(first + wave + 8 * u, units - 1);
+    const auto rsrc = row_buffer(a.w, 16 * tile, rows, a.pitch);
+    const int row = min(r, rows - 1), at = row * a.pitch + 16 * g;
+    w.word = a.w_scale[static_cast<std::int64_t>(16 * tile + row) * a.scale_pitch + unit];
+#pragma unroll
+    for (int p = 0; p < 8; ++p) w.piece[p] = load16(rsrc, at + 64 * (p & 1), min(4 * unit + p / 2, a.blocks - 1) * 128);
+  };
+  // Blocks past the row's end are zeros in x, so whatever w has there adds nothing; w's are
+  // read from the row's last block.
+  int4_t x[kU][kT][8];
+  std::uint32_t x_word[kU][kT];
+  const auto x_rsrc = row_buffer(a.x, 0, a.m, a.pitch);
+  const bool staged = kT == 1 && kU == 1 && a.m <= kStaged;
+  int4_t stage[kStaged / 2];
+  if (staged) {
+#pragma unroll
+    for (int t = 0; t < kStaged / 2; ++t) {
+      const int row = 2 * t + (lane >> 5), unit = first + wave;
+      if (2 * t < a.m)
+        stage[t] = load16(x_rsrc, row < a.m && unit < units && 16 * (lane & 31) < (a.blocks - 4 * unit) * 128 ? row * a.pitch + 16 * (lane & 31) : -1,
+                          unit * 512);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const int unit = first + wave + 8 * u;
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      const int row = min(16 * t + r, a.m - 1);
+      x_word[u][t] = unit < units ? a.x_scale[static_cast<std::int64_t>(row) * a.scale_pitch + unit] : 0;
+      if (staged) continue;
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+        x[u][t][p] = load16(x_rsrc, unit < units && 4 * unit + p / 2 < a.blocks ? row * a.pitch + 16 * g + 64 * p : -1, unit * 512);
+    }
+  }
+  int tile = static_cast<int>(blockIdx.x);
+  Weights now, next;
+  load(now, tile, 0);
+  if (staged) {
+    // A wave's own rows, its own LDS: piece q of row r at q ^ (r & 7).
+    int4_t* const own = stages[wave];
+#pragma unroll
+    for (int t = 0; t < kStaged / 2; ++t) {
+      const int row = 2 * t + (lane >> 5);
+      if (2 * t < a.m) own[row * 32 + ((lane & 31) ^ (row & 7))] = stage[t];
+    }
+    const int row = min(r, a.m - 1);
+#pragma unroll
+    for (int p = 0; p < 8; ++p) x[0][0][p] = own[row * 32 + ((4 * p + g) ^ (row & 7))];
+  }
+  float4_t acc[kT];
+  auto compute = [&](const Weights& w, int u) {
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const float w_unit = unit_of(w.word, p / 2);
+      const bf8_t w0 = widen<0>(w.piece[p], w_unit), w1 = widen<1>(w.piece[p], w_unit);
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        int4_t codes = x[u][t][p];
+        if constexpr (kT * kU > 1) asm volatile("" : "+v"(codes));  // kept as codes: widened once they would take twice the registers
+        const float x_unit = unit_of(x_word[u][t], p / 2);
+        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w0, widen<0>(codes, x_unit), acc[t], 0, 0, 0);
+        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w1, widen<1>(codes, x_unit), acc[t], 0, 0, 0);
+      }
+    }
+  };
+  auto finish = [&](int tile, int turn) {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) sums[turn][wave][t][lane] = acc[t];
+    __syncthreads();
+    // Thread i of the first kT * 256: result i % 16 of the tile and row i / 16 (lane (row, g) had results 4 g on).
+    for (int i = threadIdx.x; i < kT * 256; i += 512) {
+      const int m = i >> 4, n = 16 * tile + (i & 15);
+      const float* at = reinterpret_cast<const float*>(&sums[turn][0][m >> 4][(m & 15) + 16 * ((i & 15) >> 2)]) + (i & 3);
+      float v = 0.0F;
+#pragma unroll
+      for (int p = 0; p < 8; ++p) v += at[p * kT * 256];
+      if (m >= a.m || n >= a.n) continue;
+      if (a.parts != nullptr) {
+        a.parts[(static_cast<std::int64_t>(blockIdx.y) * a.m + m) * a.n + n] = v;
+      } else {
+        if (a.bias != nullptr) v += a.bias[n];
+        a.out[m * a.out_stride + n] = activate8(v, a.activation);
+      }
+    }
+  };
+
+  int turn = 0;
+  while (true) {
+    const int after = tile + static_cast<int>(gridDim.x);
+#pragma unroll
+    for (int t = 0; t < kT; ++t) acc[t] = float4_t{0.0F, 0.0F, 0.0F, 0.0F};
+#pragma unroll
+    for (int u = 0; u + 1 < kU; ++u) {
+      load(next, tile, u + 1);
+      compute(now, u);
+      now = next;
+    }
+    if (after >= a.tiles_n) break;
+    load(next, after, 0);
+    compute(now, kU - 1);
+    finish(tile, turn);
+    now = next;
+    tile = after;
+    turn ^= 1;
+  }
+  compute(now, kU - 1);
+  finish(tile, turn);
+}
+
+template <int kT, int kU>
+int launch_few_rows(Product8 a, int splits, float* parts, hipStream_t s) {
+  a.tiles_n = (a.n + 15) / 16;
+  share_out(a, a.scale_pitch, splits, parts);
+  const int grid = std::max(1, std::min(a.tiles_n, 256 / splits));
+  hipLaunchKernelGGL((few_rows_kernel<kT, kU>), dim3(static_cast<unsigned>(grid), static_cast<unsigned>(splits)), dim3(512), 0, s, a);
+  return check(hipGetLastError(), "linear8 launch");
+}
+
+// Sums of shares of the features, [splits][m][n], joined in their order. (Without features
+// there are none, and this is the whole product.)
+struct Join8 {
+  const float* parts;
+  const float* bias;
+  float* out;
+  std::int64_t out_stride, part;  // floats between rows of out; between shares
+  int m, n, splits, activation;
+  std::uint32_t items;  // four results of a row each
+  FastDiv by_row;
+};
+__device__ __forceinline__ float4_t sum_parts(const float* parts, std::int64_t row, int n, int width, int splits, std::int64_t part) {
+  float4_t v = {0.0F, 0.0F, 0.0F, 0.0F};
+  for (int s = 0; s < splits; ++s) v = add4(v, load_features(parts + s * part + row, n, width));
+  return v;
+}
+__global__ __launch_bounds__(256) void join_kernel(Join8 a) {
+  for (std::uint32_t item = blockIdx.x * 256 + threadIdx.x; item < a.items; item += gridDim.x * 256) {
+    const std::uint32_t m = a.by_row(item);
+    const int n = static_cast<int>(item - m * a.by_row.divisor) * 4;
+    float4_t v = sum_parts(a.parts, static_cast<std::int64_t>(m) * a.n, n, a.n, a.splits, a.part);
+    if (a.bias != nullptr) v = add4(v, load_features(a.bias, n, a.n));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = activate8(v[e], a.activation);
+    store_features(a.out + m * a.out_stride, n, a.n, v);
+  }
+}
+
+// act(gate + bias) * (up + bias) of rows [gate | up], in 8 bits: a wave a group of four blocks.
 struct Gate8 {
-  const float* gate_up;  // [rows][2 * width]
+  const float* parts;  // [splits][rows][2 * width]
+  const float* bias;
   std::uint32_t* codes;
   std::uint8_t* scales;
-  int width, blocks, groups, activation;
+  std::int64_t part;
+  int width, blocks, groups, activation, splits;
   std::uint32_t items;
   FastDiv by_groups;
 };
@@ -205,18 +583,89 @@ __global__ __launch_bounds__(256) void gate_kernel(Gate8 a) {
   for (std::uint32_t item = blockIdx.x * 4 + (threadIdx.x >> 6); item < a.items; item += step) {
     const std::uint32_t row = a.by_groups(item);
     const Place8 p = place8(lane, static_cast<int>(item - row * a.groups));
-    const float* gate = a.gate_up + static_cast<std::int64_t>(row) * 2 * a.width;
+    const std::int64_t at = static_cast<std::int64_t>(row) * 2 * a.width;
     float4_t v[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float4_t first = load_features(gate, p.feature + 64 * h, a.width);
-      const float4_t second = load_features(gate + a.width, p.feature + 64 * h, a.width);
+      const int f = p.feature + 64 * h;
+      float4_t gate = sum_parts(a.parts, at, f, a.width, a.splits, a.part);
+      float4_t up = sum_parts(a.parts + a.width, at, f, a.width, a.splits, a.part);
+      if (a.bias != nullptr) {
+        gate = add4(gate, load_features(a.bias, f, a.width));
+        up = add4(up, load_features(a.bias + a.width, f, a.width));
+      }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[h][e] = activate8(first[e], a.activation) * second[e];
+      for (int e = 0; e < 4; ++e) v[h][e] = f + e < a.width ? activate8(gate[e], a.activation) * up[e] : 0.0F;
     }
     store_group(a.codes + static_cast<std::int64_t>(row) * a.blocks * 32, a.scales + static_cast<std::int64_t>(row) * a.groups * 4, p,
                 a.blocks, encode_block(v));
   }
+}
+
+// The ways to a product, and what a round of blocks on all 256 CUs took, in us: `fixed`
+// (start, first loads, results) and `step` for each block of 128 features, with one
+// block a CU and with as many as fit (n = 4096, 1024 to 8192 features, weights in the
+// cache; few rows and tiles that leave CUs empty a little less).
+struct Way8 {
+  int kind, m, n, sets, fit;  // tile, and blocks that a CU holds
+  float fixed[2], step[2];
+};
+constexpr Way8 kWays[] = {
+    {0, 32, 64, 4, 1, {1.5F, 1.5F}, {0.20F, 0.20F}},   {1, 64, 64, 4, 1, {2.8F, 2.8F}, {0.25F, 0.25F}},
+    {2, 64, 64, 2, 2, {3.1F, 3.7F}, {0.40F, 0.535F}},  {3, 128, 128, 1, 2, {7.0F, 7.7F}, {1.05F, 1.87F}},
+    {4, 256, 128, 1, 1, {7.0F, 7.0F}, {1.71F, 1.71F}}, {5, 256, 256, 1, 1, {13.7F, 13.7F}, {2.75F, 2.75F}},
+};
+constexpr int kFewRows = 6;
+struct Plan8 {
+  int kind, splits;
+};
+// What shares of the features cost in a second launch and in bytes at 4.5 TB/s.
+float join_cost(const Product8& a, int splits) {
+  return splits == 1 ? 0.0F : 2.0F + (splits + 1) * 4.0F * static_cast<float>(a.m) * static_cast<float>(a.n) / 4.5e6F;
+}
+// `joined`: a launch that joins the shares comes anyway.
+Plan8 plan_product(const Product8& a, bool joined, std::size_t workspace_bytes) {
+  // Few rows of any number of weights, as far as a wave's registers hold its part of x:
+  // 16 x 22528 x 4096 in 23.5 us (32 x 64 tiles: 24), 1 x 4096 x 4096 in 5.5 (8.9).
+  if (a.m <= 16 && a.scale_pitch <= 24) return {kFewRows, 1};
+  Plan8 best{5, 1};
+  float least = 1e30F;
+  for (const Way8& w : kWays) {
+    const std::int64_t tiles = static_cast<std::int64_t>((a.m + w.m - 1) / w.m) * ((a.n + w.n - 1) / w.n);
+    for (int splits = 1; splits <= 16; splits = splits < 4 ? splits + 1 : splits * 3 / 2) {
+      const std::int64_t blocks = tiles * splits;
+      if (splits > 1 && (blocks > 256 * w.fit || a.blocks < splits * w.sets ||
+                         static_cast<std::size_t>(a.m) * a.n * splits * sizeof(float) > workspace_bytes))
+        break;
+      const float steps = static_cast<float>((a.blocks + splits - 1) / splits);
+      const std::int64_t rounds = blocks / (256 * w.fit), rest = blocks - rounds * 256 * w.fit;
+      float time = static_cast<float>(rounds) * (w.fixed[1] + steps * w.step[1]);
+      if (rest > 0) time += w.fixed[rest > 256] + steps * w.step[rest > 256];
+      time += joined ? join_cost(a, splits) - (splits > 1 ? 2.0F : 0.0F) : join_cost(a, splits);
+      if (time < least) {
+        least = time;
+        best = {w.kind, splits};
+      }
+    }
+  }
+  return best;
+}
+std::size_t part_bytes(const Product8& a, int splits) {
+  return static_cast<std::size_t>(a.m) * static_cast<std::size_t>(a.n) * static_cast<std::size_t>(splits) * sizeof(float);
+}
+int run_plan(const Product8& a, const Plan8& plan, float* parts, hipStream_t s) {
+  switch (plan.kind) {
+    case 0: return launch_product<32, 64, 32, 64, 4, 3>(a, plan.splits, parts, s);
+    case 1: return launch_product<64, 64, 64, 64, 4, 2>(a, plan.splits, parts, s);
+    case 2: return launch_product<64, 64, 64, 64, 2, 2>(a, plan.splits, parts, s);
+    case 3: return launch_product<128, 128, 64, 64, 1, 2>(a, plan.splits, parts, s);
+    case 4: return launch_product<256, 128, 64, 64, 1, 3>(a, plan.splits, parts, s);
+    case 5: return launch_product<256, 256, 128, 64, 1, 2>(a, plan.splits, parts, s);
+    default: break;
+  }
+  if (a.scale_pitch <= 8) return launch_few_rows<1, 1>(a, plan.splits, parts, s);
+  if (a.scale_pitch <= 16) return launch_few_rows<1, 2>(a, plan.splits, parts, s);
+  return launch_few_rows<1, 3>(a, plan.splits, parts, s);
 }
 
 // Checks a descriptor and fills what follows from it; `gated`: weights of 2 * outputs rows.
@@ -256,10 +705,6 @@ int operand_args(const std::int32_t* x_codes, const std::int32_t* x_scales, cons
   return TCX_OK;
 }
 
-int run_product(const Product8& a, hipStream_t s) { return launch_product<128, 128, 64, 64>(a, s); }
-
-std::size_t gate_bytes(const Product8& a) { return static_cast<std::size_t>(a.m) * a.n * sizeof(float); }
-
 }  // namespace
 }  // namespace tcx
 
@@ -269,7 +714,8 @@ size_t tcx_hip_linear8_workspace_bytes(const tcx_hip_linear8_desc_t* desc) {
   using namespace tcx;
   Product8 a;
   if (product_args(desc, false, a) != TCX_OK || a.m == 0 || a.n == 0) return 0;
-  return 0;
+  const Plan8 plan = plan_product(a, false, SIZE_MAX);
+  return plan.splits > 1 ? part_bytes(a, plan.splits) : 0;
 }
 
 int tcx_hip_linear8(const int32_t* x_codes, const int32_t* x_scales, const int32_t* w_codes, const int32_t* w_scales, float* out,
@@ -284,15 +730,35 @@ int tcx_hip_linear8(const int32_t* x_codes, const int32_t* x_scales, const int32
   if (int rc = operand_args(x_codes, x_scales, w_codes, w_scales, a); rc != TCX_OK) return rc;
   if (int rc = ready(); rc != TCX_OK) return rc;
   a.out = out;
-  (void)workspace_bytes;
-  return run_product(a, static_cast<hipStream_t>(stream));
+  const auto s = static_cast<hipStream_t>(stream);
+  Plan8 plan{0, 0};
+  if (a.blocks > 0) {
+    plan = plan_product(a, false, workspace != nullptr ? workspace_bytes : 0);
+    if (plan.splits == 1) return run_plan(a, plan, nullptr, s);
+    if (int rc = run_plan(a, plan, static_cast<float*>(workspace), s); rc != TCX_OK) return rc;
+  }
+  Join8 j{};
+  j.parts = static_cast<const float*>(workspace);
+  j.bias = a.bias;
+  j.out = out;
+  j.out_stride = a.out_stride;
+  j.part = static_cast<std::int64_t>(a.m) * a.n;
+  j.m = a.m;
+  j.n = a.n;
+  j.splits = plan.splits;
+  j.activation = a.activation;
+  j.by_row = FastDiv(static_cast<std::uint32_t>((a.n + 3) / 4));
+  if (a.m >= (std::int64_t{1} << 31) / j.by_row.divisor) return fail(TCX_INVALID_ARGUMENT, "linear8 has too many results");
+  j.items = static_cast<std::uint32_t>(a.m) * j.by_row.divisor;
+  hipLaunchKernelGGL(join_kernel, dim3(grid_for(j.items, 256, kStrideBlocks)), dim3(256), 0, s, j);
+  return check(hipGetLastError(), "linear8 join launch");
 }
 
 size_t tcx_hip_gated_linear8_workspace_bytes(const tcx_hip_linear8_desc_t* desc) {
   using namespace tcx;
   Product8 a;
   if (product_args(desc, true, a) != TCX_OK || a.m == 0 || a.n == 0) return 0;
-  return gate_bytes(a);
+  return part_bytes(a, plan_product(a, true, SIZE_MAX).splits);
 }
 
 int tcx_hip_gated_linear8(const int32_t* x_codes, const int32_t* x_scales, const int32_t* w_codes, const int32_t* w_scales,
@@ -307,7 +773,7 @@ int tcx_hip_gated_linear8(const int32_t* x_codes, const int32_t* x_scales, const
   if (!aligned8(codes, 16) || !aligned8(scales, 4))
     return fail(TCX_INVALID_ARGUMENT, "linear8 codes must be 16-byte aligned and scales 4-byte aligned");
   if (int rc = operand_args(x_codes, x_scales, w_codes, w_scales, a); rc != TCX_OK) return rc;
-  if (workspace == nullptr || !aligned8(workspace, 16) || workspace_bytes < gate_bytes(a))
+  if (workspace == nullptr || !aligned8(workspace, 16) || workspace_bytes < part_bytes(a, plan_product(a, true, SIZE_MAX).splits))
     return fail(TCX_INVALID_ARGUMENT, "gated_linear8 needs a 16-byte aligned workspace of the query's size");
   Gate8 t{};
   t.width = static_cast<int>(desc->outputs);
@@ -316,9 +782,15 @@ int tcx_hip_gated_linear8(const int32_t* x_codes, const int32_t* x_scales, const
   if (a.m >= (std::int64_t{1} << 31) / t.groups) return fail(TCX_INVALID_ARGUMENT, "linear8 has too many results");
   if (int rc = ready(); rc != TCX_OK) return rc;
   const auto s = static_cast<hipStream_t>(stream);
-  a.out = static_cast<float*>(workspace);
-  if (int rc = run_product(a, s); rc != TCX_OK) return rc;
-  t.gate_up = a.out;
+  Plan8 plan{0, 0};
+  if (a.blocks > 0) {
+    plan = plan_product(a, true, workspace_bytes);
+    if (int rc = run_plan(a, plan, static_cast<float*>(workspace), s); rc != TCX_OK) return rc;
+  }
+  t.parts = static_cast<const float*>(workspace);
+  t.bias = a.bias;
+  t.part = static_cast<std::int64_t>(a.m) * a.n;
+  t.splits = plan.splits;
   t.codes = reinterpret_cast<std::uint32_t*>(codes);
   t.scales = reinterpret_cast<std::uint8_t*>(scales);
   t.activation = desc->activation;
