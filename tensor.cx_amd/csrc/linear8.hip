@@ -36,6 +36,10 @@ struct Product8 {
   // (or units of four) and one more if s < extra, and its sums go to parts [s][m][n].
   float* parts;  // null: one share, whose results go to out
   int each, extra;
+  // Of a gated product in one launch: w has `outputs` rows of gate, then those of up.
+  std::uint32_t* gate_codes;
+  std::uint8_t* gate_scales;
+  int outputs, gate_blocks, gate_groups, gate_activation;
 };
 // The features of a share: [first, last).
 struct Share8 {
@@ -75,10 +79,10 @@ __device__ __forceinline__ Tile8 tile_of(const Product8& a, int block) {
   return {group * 8 + in % deep, in / deep};
 }
 
-// Rows [first, first + rows) of an operand's codes.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const std::uint8_t* codes, int first, int rows, int pitch) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<std::uint8_t*>(codes + static_cast<std::int64_t>(first) * pitch),
-                                           static_cast<short>(0), rows * pitch, 0x00020000);
+// Rows [first, first + rows) of an operand's codes (or exponents).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const std::uint8_t* codes, std::int64_t first, int rows, int pitch) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<std::uint8_t*>(codes + first * pitch), static_cast<short>(0), rows * pitch,
+                                           0x00020000);
 }
 __device__ __forceinline__ int4_t load16(__amdgpu_buffer_rsrc_t r, int voffset, int soffset) {
   return __builtin_bit_cast(int4_t, __builtin_amdgcn_raw_buffer_load_b128(r, voffset, soffset, 0));
@@ -117,6 +121,10 @@ __device__ __forceinline__ void wave_lds_done() { asm volatile("s_waitcnt lgkmcn
 // its own: no barriers until the waves' sums meet at the end, and for small tiles half the
 // conversions that waves with a quarter of the tile each would make.
 //
+// With kGate the tile has 128 columns of gate and the same ones of up, 32 of each by turns,
+// and its results leave in 8 bits: 4096 x (2 x 11264) x 4096 in 586 us, in two launches
+// with float32 between them 709.
+//
 // The features may be split over the grid's rows (Product8::parts).
 template <int kM, int kN, int kWM, int kWN, int kSets, int kStages>
 struct Tiles8 {
@@ -136,7 +144,7 @@ struct Tiles8 {
   static constexpr int kStride = kWN + 8;
   static_assert(kSets == 1 ? kWaves * 32 * kStride * 4 <= kScales : kM * kStride * 4 <= kScales);
 };
-template <int kM, int kN, int kWM, int kWN, int kSets, int kStages>
+template <int kM, int kN, int kWM, int kWN, int kSets, int kStages, bool kGate>
 __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads)) void product_kernel(Product8 a) {
   using T = Tiles8<kM, kN, kWM, kWN, kSets, kStages>;
   constexpr int kWavesN = T::kWavesN, kWaves = T::kWaves, kI = T::kI, kJ = T::kJ, kLoads = T::kLoads;
@@ -149,35 +157,41 @@ __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads
   const Tile8 tile = tile_of(a, static_cast<int>(blockIdx.x));
   const auto [share_first, last] = share_of(a, static_cast<int>(blockIdx.y));
   const int first = share_first + set;
-  const int m0 = tile.m * kM, n0 = tile.n * kN;
+  const int m0 = tile.m * kM, n0 = tile.n * (kGate ? kN / 2 : kN);
   const int r = lane & 31, g = lane >> 5;
 
   // Loads: instruction t of a wave brings rows 8 (t kWaves + wave) on of the buffer; rows
   // past the operand's end are its last one again.
-  const int m_last = min(a.m - m0, kM) - 1, n_last = min(a.n - n0, kN) - 1;
+  const int m_last = min(a.m - m0, kM) - 1, n_last = kGate ? min(a.outputs - n0, kN / 2) - 1 : min(a.n - n0, kN) - 1;
+  // Row of w, from n0 on, that row `row` of w's part of the buffer holds (of gate or up, by bit 5).
+  auto w_row = [&](int row) { return min(kGate ? (row >> 6 << 5) + (row & 31) : row, n_last); };
+  const std::int64_t w_first = n0 + (kGate && ((wave >> 2) & 1) ? a.outputs : 0);  // a wave's loads are of gate, or of up
+  static_assert(!kGate || (kWaves == 8 && kM == 256 && kN == 256 && kWN == 64 && kSets == 1));
   int offset[kLoads];
   bool of_x[kLoads];
 #pragma unroll
   for (int t = 0; t < kLoads; ++t) {
     const int at = 8 * (t * kWaves + wave), row = at + (lane >> 3);
     of_x[t] = kM % (8 * kWaves) == 0 ? t * 8 * kWaves < kM : at < kM;
-    offset[t] = (of_x[t] ? min(row, m_last) : min(row - kM, n_last)) * a.pitch + (((lane & 7) ^ (lane >> 3)) << 4);
+    offset[t] = (of_x[t] ? min(row, m_last) : w_row(row - kM)) * a.pitch + (((lane & 7) ^ (lane >> 3)) << 4);
   }
   // Exponents: words of 64 rows a load, one for each of the first waves, or all for a set's one.
   int scale_offset[kSets == 1 ? 1 : T::kScaleLoads];
 #pragma unroll
   for (int t = 0; t < (kSets == 1 ? 1 : T::kScaleLoads); ++t) {
     const int row = 64 * (kSets == 1 ? wave : t) + lane;
-    scale_offset[t] = 4 * a.scale_pitch * (row < T::kScaleX ? min(row, m_last) : min(row - T::kScaleX, n_last));
+    const int w = row - T::kScaleX;
+    scale_offset[t] = 4 * a.scale_pitch * (row < T::kScaleX ? min(row, m_last) : w_row(w) + (kGate && (w >> 5 & 1) ? a.outputs : 0));
   }
   const auto xs_rsrc = row_buffer(reinterpret_cast<const std::uint8_t*>(a.x_scale), m0, m_last + 1, 4 * a.scale_pitch);
-  const auto ws_rsrc = row_buffer(reinterpret_cast<const std::uint8_t*>(a.w_scale), n0, n_last + 1, 4 * a.scale_pitch);
+  const auto ws_rsrc = row_buffer(reinterpret_cast<const std::uint8_t*>(a.w_scale), n0,
+                                  n_last + 1 + (kGate ? a.outputs : 0), 4 * a.scale_pitch);
   // Loads t0 to t1 - 1 of step kt. Past the last step they are issued all the same, without
   // memory behind them, so that every step counts as many.
   auto load = [&](int kt, int buffer, int t0, int t1) {
     std::uint8_t* const at = lds + buffer * T::kStageBytes;
     const bool any = kt < last;
-    const auto x_now = row_buffer(a.x, m0, any ? m_last + 1 : 0, a.pitch), w_now = row_buffer(a.w, n0, any ? n_last + 1 : 0, a.pitch);
+    const auto x_now = row_buffer(a.x, m0, any ? m_last + 1 : 0, a.pitch), w_now = row_buffer(a.w, w_first, any ? n_last + 1 : 0, a.pitch);
 #pragma unroll
     for (int t = t0; t < t1; ++t)
       load_lds16(of_x[t] ? x_now : w_now, at + 8 * (t * kWaves + wave) * 128, offset[t], any ? kt * 128 : 0);
@@ -321,6 +335,53 @@ __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads
   // through LDS, so that a lane stores four results of a row, and that the activation
   // stands in the code few times, not once for each register (which cost 2.6 us in
   // fetching instructions).
+  if constexpr (kGate) {  // 32 rows of both halves at a time: a wave's 32 columns of gate, and of up
+    constexpr int kGateStride = kN + 8;
+    static_assert(64 * kGateStride * 4 <= T::kScales);
+    float* const turn = reinterpret_cast<float*>(lds);
+    const int wave_row = wm / kWM, column = wn / 2;
+#pragma unroll 1
+    for (int i0 = 0; i0 < kI; ++i0) {
+      block_barrier();  // the buffers, or the rows before, are done with
+#pragma unroll
+      for (int i = 0; i < kI; ++i) {
+        if (i != i0) continue;
+#pragma unroll
+        for (int j = 0; j < kJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            turn[(32 * wave_row + 8 * (e / 4) + 4 * g + e % 4) * kGateStride + kN / 2 * j + column + r] = acc[i][j][e];
+      }
+      block_barrier();
+      // Sixteen lanes a row, its block of 128 features as encode_block has it.
+#pragma unroll 1
+      for (int row = static_cast<int>(threadIdx.x) >> 4; row < 64; row += 32) {
+        const int m = m0 + (row >> 5) * kWM + 32 * i0 + (row & 31), lane16 = static_cast<int>(threadIdx.x) & 15;
+        float4_t v[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int f = 64 * h + 4 * lane16;
+          const float* const at = turn + row * kGateStride + f;
+          float4_t gate = *reinterpret_cast<const float4_t*>(at), up = *reinterpret_cast<const float4_t*>(at + kN / 2);
+          if (a.bias != nullptr) {
+            gate = add4(gate, load_features(a.bias, n0 + f, a.outputs));
+            up = add4(up, load_features(a.bias + a.outputs, n0 + f, a.outputs));
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[h][e] = f + e <= n_last ? activate8(gate[e], a.gate_activation) * up[e] : 0.0F;
+        }
+        const Coded8 c = encode_block(v);
+        if (m >= a.m) continue;
+        std::uint32_t* const codes = a.gate_codes + (static_cast<std::int64_t>(m) * a.gate_blocks + tile.n) * 32;
+        codes[lane16] = c.word[0];
+        codes[16 + lane16] = c.word[1];
+        std::uint8_t* const scale = a.gate_scales + static_cast<std::int64_t>(m) * a.gate_groups * 4 + tile.n;
+        if (lane16 == 0) *scale = static_cast<std::uint8_t>(c.byte);
+        else if (tile.n + 1 == a.gate_blocks && tile.n + lane16 < a.gate_groups * 4) scale[lane16] = 0;  // the last word filled up
+      }
+    }
+    return;
+  }
   const bool whole = a.parts == nullptr;
   float* const out = whole ? a.out : a.parts + static_cast<std::int64_t>(blockIdx.y) * a.m * a.n;
   const std::int64_t stride = whole ? a.out_stride : a.n;
@@ -382,17 +443,17 @@ void share_out(Product8& a, int units, int splits, float* parts) {
   a.extra = units % splits;
 }
 
-template <int kM, int kN, int kWM, int kWN, int kSets, int kStages>
+template <int kM, int kN, int kWM, int kWN, int kSets, int kStages, bool kGate = false>
 int launch_product(Product8 a, int splits, float* parts, hipStream_t s) {
   a.tiles_m = (a.m + kM - 1) / kM;
-  a.tiles_n = (a.n + kN - 1) / kN;
+  a.tiles_n = kGate ? a.gate_blocks : (a.n + kN - 1) / kN;
   a.by_group = FastDiv(static_cast<std::uint32_t>(8 * a.tiles_n));
   share_out(a, a.blocks, splits, parts);
   constexpr int kThreads = Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads;
   const std::int64_t tiles = static_cast<std::int64_t>(a.tiles_m) * a.tiles_n;
   if (tiles * splits * kThreads > kMaxLaunchWorkItems || tiles >= (std::int64_t{1} << 30))
     return fail(TCX_INVALID_ARGUMENT, "linear8 has too many results");
-  hipLaunchKernelGGL((product_kernel<kM, kN, kWM, kWN, kSets, kStages>), dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(splits)),
+  hipLaunchKernelGGL((product_kernel<kM, kN, kWM, kWN, kSets, kStages, kGate>), dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(splits)),
                      dim3(kThreads), 0, s, a);
   return check(hipGetLastError(), "linear8 launch");
 }
@@ -615,16 +676,20 @@ constexpr Way8 kWays[] = {
     {2, 64, 64, 2, 2, {3.1F, 3.7F}, {0.40F, 0.535F}},  {3, 128, 128, 1, 2, {7.0F, 7.7F}, {1.05F, 1.87F}},
     {4, 256, 128, 1, 1, {7.0F, 7.0F}, {1.71F, 1.71F}}, {5, 256, 256, 1, 1, {13.7F, 13.7F}, {2.75F, 2.75F}},
 };
-constexpr int kFewRows = 6;
+constexpr int kFewRows = 6, kFusedGate = 7;
 struct Plan8 {
   int kind, splits;
 };
+std::size_t part_bytes(const Product8& a, int splits) {
+  return static_cast<std::size_t>(a.m) * static_cast<std::size_t>(a.n) * static_cast<std::size_t>(splits) * sizeof(float);
+}
 // What shares of the features cost in a second launch and in bytes at 4.5 TB/s.
 float join_cost(const Product8& a, int splits) {
   return splits == 1 ? 0.0F : 2.0F + (splits + 1) * 4.0F * static_cast<float>(a.m) * static_cast<float>(a.n) / 4.5e6F;
 }
-// `joined`: a launch that joins the shares comes anyway.
-Plan8 plan_product(const Product8& a, bool joined, std::size_t workspace_bytes) {
+// `gated`: the results go through float32 and a second launch to 8 bits, unless the tiles
+// of 256 x 256 do that themselves.
+Plan8 plan_product(const Product8& a, bool gated, std::size_t workspace_bytes) {
   // Few rows of any number of weights, as far as a wave's registers hold its part of x:
   // 16 x 22528 x 4096 in 23.5 us (32 x 64 tiles: 24), 1 x 4096 x 4096 in 5.5 (8.9).
   if (a.m <= 16 && a.scale_pitch <= 24) return {kFewRows, 1};
@@ -634,24 +699,23 @@ Plan8 plan_product(const Product8& a, bool joined, std::size_t workspace_bytes) 
     const std::int64_t tiles = static_cast<std::int64_t>((a.m + w.m - 1) / w.m) * ((a.n + w.n - 1) / w.n);
     for (int splits = 1; splits <= 16; splits = splits < 4 ? splits + 1 : splits * 3 / 2) {
       const std::int64_t blocks = tiles * splits;
-      if (splits > 1 && (blocks > 256 * w.fit || a.blocks < splits * w.sets ||
-                         static_cast<std::size_t>(a.m) * a.n * splits * sizeof(float) > workspace_bytes))
-        break;
+      if (splits > 1 && (blocks > 256 * w.fit || a.blocks < splits * w.sets || part_bytes(a, splits) > workspace_bytes)) break;
       const float steps = static_cast<float>((a.blocks + splits - 1) / splits);
       const std::int64_t rounds = blocks / (256 * w.fit), rest = blocks - rounds * 256 * w.fit;
       float time = static_cast<float>(rounds) * (w.fixed[1] + steps * w.step[1]);
       if (rest > 0) time += w.fixed[rest > 256] + steps * w.step[rest > 256];
-      time += joined ? join_cost(a, splits) - (splits > 1 ? 2.0F : 0.0F) : join_cost(a, splits);
+      time += gated ? join_cost(a, splits + 1) : join_cost(a, splits);
       if (time < least) {
         least = time;
         best = {w.kind, splits};
       }
     }
   }
+  if (gated && (static_cast<std::int64_t>(a.outputs) + 256) * 4 * a.scale_pitch < (std::int64_t{1} << 31)) {
+    const std::int64_t tiles = static_cast<std::int64_t>((a.m + 255) / 256) * a.gate_blocks;
+    if (static_cast<float>((tiles + 255) / 256) * (12.0F + static_cast<float>(a.blocks) * 2.75F) < least) best = {kFusedGate, 1};
+  }
   return best;
-}
-std::size_t part_bytes(const Product8& a, int splits) {
-  return static_cast<std::size_t>(a.m) * static_cast<std::size_t>(a.n) * static_cast<std::size_t>(splits) * sizeof(float);
 }
 int run_plan(const Product8& a, const Plan8& plan, float* parts, hipStream_t s) {
   switch (plan.kind) {
@@ -661,6 +725,7 @@ int run_plan(const Product8& a, const Plan8& plan, float* parts, hipStream_t s) 
     case 3: return launch_product<128, 128, 64, 64, 1, 2>(a, plan.splits, parts, s);
     case 4: return launch_product<256, 128, 64, 64, 1, 3>(a, plan.splits, parts, s);
     case 5: return launch_product<256, 256, 128, 64, 1, 2>(a, plan.splits, parts, s);
+    case kFusedGate: return launch_product<256, 256, 128, 64, 1, 2, true>(a, 1, nullptr, s);
     default: break;
   }
   if (a.scale_pitch <= 8) return launch_few_rows<1, 1>(a, plan.splits, parts, s);
@@ -688,6 +753,12 @@ int product_args(const tcx_hip_linear8_desc_t* desc, bool gated, Product8& a) {
   a.activation = gated ? TCX_ACT_NONE : d.activation;
   a.out_stride = gated || d.out_stride == 0 ? a.n : d.out_stride;
   if (a.out_stride < a.n) return fail(TCX_INVALID_ARGUMENT, "linear8 output rows must not overlap");
+  if (gated) {
+    a.outputs = static_cast<int>(d.outputs);
+    a.gate_blocks = static_cast<int>(blocks8(d.outputs));
+    a.gate_groups = static_cast<int>(scale_words8(d.outputs));
+    a.gate_activation = d.activation;
+  }
   return TCX_OK;
 }
 int operand_args(const std::int32_t* x_codes, const std::int32_t* x_scales, const std::int32_t* w_codes,
@@ -757,8 +828,9 @@ int tcx_hip_linear8(const int32_t* x_codes, const int32_t* x_scales, const int32
 size_t tcx_hip_gated_linear8_workspace_bytes(const tcx_hip_linear8_desc_t* desc) {
   using namespace tcx;
   Product8 a;
-  if (product_args(desc, true, a) != TCX_OK || a.m == 0 || a.n == 0) return 0;
-  return part_bytes(a, plan_product(a, true, SIZE_MAX).splits);
+  if (product_args(desc, true, a) != TCX_OK || a.m == 0 || a.n == 0 || a.blocks == 0) return 0;
+  const Plan8 plan = plan_product(a, true, SIZE_MAX);
+  return plan.kind == kFusedGate ? 0 : part_bytes(a, plan.splits);
 }
 
 int tcx_hip_gated_linear8(const int32_t* x_codes, const int32_t* x_scales, const int32_t* w_codes, const int32_t* w_scales,
@@ -773,27 +845,32 @@ int tcx_hip_gated_linear8(const int32_t* x_codes, const int32_t* x_scales, const
   if (!aligned8(codes, 16) || !aligned8(scales, 4))
     return fail(TCX_INVALID_ARGUMENT, "linear8 codes must be 16-byte aligned and scales 4-byte aligned");
   if (int rc = operand_args(x_codes, x_scales, w_codes, w_scales, a); rc != TCX_OK) return rc;
-  if (workspace == nullptr || !aligned8(workspace, 16) || workspace_bytes < part_bytes(a, plan_product(a, true, SIZE_MAX).splits))
-    return fail(TCX_INVALID_ARGUMENT, "gated_linear8 needs a 16-byte aligned workspace of the query's size");
-  Gate8 t{};
-  t.width = static_cast<int>(desc->outputs);
-  t.blocks = static_cast<int>(blocks8(t.width));
-  t.groups = static_cast<int>(scale_words8(t.width));
-  if (a.m >= (std::int64_t{1} << 31) / t.groups) return fail(TCX_INVALID_ARGUMENT, "linear8 has too many results");
-  if (int rc = ready(); rc != TCX_OK) return rc;
-  const auto s = static_cast<hipStream_t>(stream);
+  if (!aligned8(workspace, 16)) return fail(TCX_INVALID_ARGUMENT, "linear8 workspace must be 16-byte aligned");
+  if (a.m >= (std::int64_t{1} << 31) / a.gate_groups) return fail(TCX_INVALID_ARGUMENT, "linear8 has too many results");
   Plan8 plan{0, 0};
   if (a.blocks > 0) {
-    plan = plan_product(a, true, workspace_bytes);
-    if (int rc = run_plan(a, plan, static_cast<float*>(workspace), s); rc != TCX_OK) return rc;
+    plan = plan_product(a, true, SIZE_MAX);
+    if (plan.kind != kFusedGate && (workspace == nullptr || workspace_bytes < part_bytes(a, plan.splits)))
+      return fail(TCX_INVALID_ARGUMENT, "gated_linear8 needs a workspace of the query's size");
   }
+  if (int rc = ready(); rc != TCX_OK) return rc;
+  const auto s = static_cast<hipStream_t>(stream);
+  a.gate_codes = reinterpret_cast<std::uint32_t*>(codes);
+  a.gate_scales = reinterpret_cast<std::uint8_t*>(scales);
+  if (plan.kind == kFusedGate) return run_plan(a, plan, nullptr, s);
+  if (a.blocks > 0)
+    if (int rc = run_plan(a, plan, static_cast<float*>(workspace), s); rc != TCX_OK) return rc;
+  Gate8 t{};
   t.parts = static_cast<const float*>(workspace);
   t.bias = a.bias;
   t.part = static_cast<std::int64_t>(a.m) * a.n;
   t.splits = plan.splits;
-  t.codes = reinterpret_cast<std::uint32_t*>(codes);
-  t.scales = reinterpret_cast<std::uint8_t*>(scales);
-  t.activation = desc->activation;
+  t.width = a.outputs;
+  t.blocks = a.gate_blocks;
+  t.groups = a.gate_groups;
+  t.codes = a.gate_codes;
+  t.scales = a.gate_scales;
+  t.activation = a.gate_activation;
   t.items = static_cast<std::uint32_t>(static_cast<std::int64_t>(a.m) * t.groups);
   t.by_groups = FastDiv(static_cast<std::uint32_t>(t.groups));
   hipLaunchKernelGGL(gate_kernel, dim3(grid_for(t.items, 4, kStrideBlocks)), dim3(256), 0, s, t);

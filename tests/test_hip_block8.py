@@ -256,7 +256,7 @@ def test_linear_of_nothing(cx):
 
 # rows, outputs, features
 GATED = [(1, 1, 128), (1, 300, 1000), (2, 128, 256), (7, 129, 300), (16, 1100, 384), (33, 513, 640), (70, 256, 100), (129, 260, 1300),
-         (300, 140, 513), (520, 900, 256)]
+         (300, 140, 513), (520, 900, 256), (1100, 3000, 129), (2050, 1000, 384), (2300, 2570, 200)]
 
 
 @pytest.mark.parametrize("bias", [False, True])
