@@ -117,9 +117,10 @@ __device__ __forceinline__ void wave_lds_done() { asm volatile("s_waitcnt lgkmcn
 // rows lie in different banks. Words of exponents, of four steps each, have two
 // buffers of their own.
 //
-// With kSets > 1 a wave has the whole tile to itself, for every kSets-th step, with LDS of
-// its own: no barriers until the waves' sums meet at the end, and for small tiles half the
-// conversions that waves with a quarter of the tile each would make.
+// With kSets > 1 there are as many sets of waves, each with the whole tile for every
+// kSets-th step and with LDS of its own; their sums meet at the end. A set of one wave
+// needs no barriers until then, and makes half the conversions that waves with a quarter of
+// a small tile each would make. Sets of more waves share the barriers.
 //
 // With kGate the tile has 128 columns of gate and the same ones of up, 32 of each by turns,
 // and its results leave in 8 bits: 4096 x (2 x 11264) x 4096 in 586 us, in two launches
@@ -139,20 +140,21 @@ struct Tiles8 {
   static constexpr int kScaleBytes = kScaleLoads * 256;
   static constexpr int kSetBytes = kScales + kScaleBuffers * kScaleBytes, kLds = kSetBytes * kSets;
   static_assert(kLds <= 160 * 1024 && kStages <= 4);
-  static_assert(kSets == 1 ? kM % (8 * kWaves) == 0 && kN % (8 * kWaves) == 0 && kScaleLoads <= kWaves && kM % 64 == 0 : kWaves == 1);
+  static constexpr int kScaled = kSets == 1 ? 0 : (kScaleLoads + kWaves - 1) / kWaves;  // a wave's loads of them in every step
+  static_assert(kM % (8 * kWaves) == 0 && kN % (8 * kWaves) == 0 && (kSets > 1 || kM % 64 == 0));
   // Results on their way out through LDS: rows 4 apart lie in different halves of the banks.
-  static constexpr int kStride = kWN + 8;
+  static constexpr int kStride = (kSets == 1 ? kWN : kN) + 8;
   static_assert(kSets == 1 ? kWaves * 32 * kStride * 4 <= kScales : kM * kStride * 4 <= kScales);
 };
 template <int kM, int kN, int kWM, int kWN, int kSets, int kStages, bool kGate>
 __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads)) void product_kernel(Product8 a) {
   using T = Tiles8<kM, kN, kWM, kWN, kSets, kStages>;
   constexpr int kWavesN = T::kWavesN, kWaves = T::kWaves, kI = T::kI, kJ = T::kJ, kLoads = T::kLoads;
-  constexpr int kScaled = kSets == 1 ? 0 : T::kScaleLoads;  // loads of exponents in every step
+  constexpr int kScaled = T::kScaled;
   __shared__ __attribute__((aligned(1024))) std::uint8_t memory[T::kLds];
 
   const int lane = threadIdx.x & 63, thread_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int set = kSets == 1 ? 0 : thread_wave, wave = kSets == 1 ? thread_wave : 0;
+  const int set = thread_wave / kWaves, wave = thread_wave % kWaves;
   std::uint8_t* const lds = memory + set * T::kSetBytes;
   const Tile8 tile = tile_of(a, static_cast<int>(blockIdx.x));
   const auto [share_first, last] = share_of(a, static_cast<int>(blockIdx.y));
@@ -175,11 +177,13 @@ __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads
     of_x[t] = kM % (8 * kWaves) == 0 ? t * 8 * kWaves < kM : at < kM;
     offset[t] = (of_x[t] ? min(row, m_last) : w_row(row - kM)) * a.pitch + (((lane & 7) ^ (lane >> 3)) << 4);
   }
-  // Exponents: words of 64 rows a load, one for each of the first waves, or all for a set's one.
-  int scale_offset[kSets == 1 ? 1 : T::kScaleLoads];
+  // Exponents: words of 64 rows a load, spread over the waves.
+  constexpr int kScaleParts = (T::kScaleLoads + kWaves - 1) / kWaves;
+  auto scale_part = [&](int t) { return (t * kWaves + wave) % T::kScaleLoads; };
+  int scale_offset[kScaleParts];
 #pragma unroll
-  for (int t = 0; t < (kSets == 1 ? 1 : T::kScaleLoads); ++t) {
-    const int row = 64 * (kSets == 1 ? wave : t) + lane;
+  for (int t = 0; t < kScaleParts; ++t) {
+    const int row = 64 * scale_part(t) + lane;
     const int w = row - T::kScaleX;
     scale_offset[t] = 4 * a.scale_pitch * (row < T::kScaleX ? min(row, m_last) : w_row(w) + (kGate && (w >> 5 & 1) ? a.outputs : 0));
   }
@@ -200,17 +204,20 @@ __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads
   auto scale_buffer = [&](int kt, int buffer) { return T::kScales + (kSets == 1 ? (kt >> 2) & 1 : buffer) * T::kScaleBytes; };
   auto load_scales = [&](int kt, int buffer) {  // of four steps, with the first of them; a set's with every step
     if constexpr (kSets == 1) {
-      if (kt < last && wave < T::kScaleLoads)
-        load_lds4(64 * wave < kM ? xs_rsrc : ws_rsrc, lds + scale_buffer(kt, buffer) + 256 * wave, scale_offset[0], (kt >> 2) * 4);
+      if (kt >= last) return;
+#pragma unroll
+      for (int t = 0; t < kScaleParts; ++t)
+        if (t * kWaves + wave < T::kScaleLoads)
+          load_lds4(64 * scale_part(t) < kM ? xs_rsrc : ws_rsrc, lds + scale_buffer(kt, buffer) + 256 * scale_part(t), scale_offset[t], (kt >> 2) * 4);
     } else {
       const auto scales = [&](const std::uint32_t* p, int at, int rows) {
         return row_buffer(reinterpret_cast<const std::uint8_t*>(p), at, kt < last ? rows : 0, 4 * a.scale_pitch);
       };
       const auto x_now = scales(a.x_scale, m0, m_last + 1), w_now = scales(a.w_scale, n0, n_last + 1);
 #pragma unroll
-      for (int t = 0; t < T::kScaleLoads; ++t) {
-        std::uint8_t* const to = lds + scale_buffer(kt, buffer) + 256 * t;
-        load_lds4(64 * t < T::kScaleX ? x_now : w_now, to, scale_offset[t], kt < last ? (kt >> 2) * 4 : 0);
+      for (int t = 0; t < kScaleParts; ++t) {
+        std::uint8_t* const to = lds + scale_buffer(kt, buffer) + 256 * scale_part(t);
+        load_lds4(64 * scale_part(t) < T::kScaleX ? x_now : w_now, to, scale_offset[t], kt < last ? (kt >> 2) * 4 : 0);
       }
     }
   };
@@ -279,7 +286,7 @@ __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads
   auto part = [&](int i) { return min(i * kPart, kLoads); };
 
   auto meet = [&] {
-    if constexpr (kSets == 1) block_barrier();
+    if constexpr (kSets == 1 || kWaves > 1) block_barrier();
     else wave_lds_done();
   };
 
@@ -297,35 +304,41 @@ __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads
   read_units(first, 0);
   widen_all.template operator()<0>(low, codes);
   int buffer = 0, before = kStages - 1;  // of this step and the one before
-  for (int kt = first; kt < last; kt += kSets) {
+  for (int kt0 = share_first; kt0 < last; kt0 += kSets) {  // as many steps for every set, the last ones perhaps without a block
+    const int kt = kt0 + set;
+    const bool live = kSets == 1 || kt < last;
     const int next = buffer + 1 == kStages ? 0 : buffer + 1;
     const int behind = kt + (kStages - 1) * kSets, ahead = behind + kSets;  // loads that the step before began; that this one begins
+    if (live) {
 #pragma unroll
-    for (int p = 0; p < 3; ++p) {
-      Codes after;
-      if (p < 2) load(behind, before, part(1 + 2 * p), part(2 + 2 * p));
-      read(after, buffer, p + 1);
+      for (int p = 0; p < 3; ++p) {
+        Codes after;
+        if (p < 2) load(behind, before, part(1 + 2 * p), part(2 + 2 * p));
+        read(after, buffer, p + 1);
+        multiply(low);
+        widen_all.template operator()<1>(high, codes);
+        order.template operator()<kI + kJ, 0>();
+        if (p < 1) load(behind, before, part(2), part(3));
+        multiply(high);
+        widen_all.template operator()<0>(low, after);
+        order.template operator()<0, 0>();
+        codes = after;
+      }
       multiply(low);
       widen_all.template operator()<1>(high, codes);
-      order.template operator()<kI + kJ, 0>();
-      if (p < 1) load(behind, before, part(2), part(3));
-      multiply(high);
-      widen_all.template operator()<0>(low, after);
       order.template operator()<0, 0>();
-      codes = after;
     }
-    multiply(low);
-    widen_all.template operator()<1>(high, codes);
-    order.template operator()<0, 0>();
     wait_loads<(kStages - 2) * (kLoads + kScaled)>();
     meet();
-    if (kSets > 1 || (ahead & 3) == 0) load_scales(ahead, buffer);
-    load(ahead, buffer, 0, part(1));
-    read(codes, next, 0);
-    read_units(kt + kSets, next);
-    multiply(high);
-    widen_all.template operator()<0>(low, codes);
-    order.template operator()<kI + kJ, kProducts / 2>();
+    if (live) {
+      if (kSets > 1 || (ahead & 3) == 0) load_scales(ahead, buffer);
+      load(ahead, buffer, 0, part(1));
+      read(codes, next, 0);
+      read_units(kt + kSets, next);
+      multiply(high);
+      widen_all.template operator()<0>(low, codes);
+      order.template operator()<kI + kJ, kProducts / 2>();
+    }
     before = buffer;
     buffer = next;
   }
@@ -399,7 +412,7 @@ __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads
     store_features(out + m * stride, n, a.n, v);
   };
   const float4_t none = {0.0F, 0.0F, 0.0F, 0.0F};
-  constexpr int kAcross = kWN / 4;  // lanes to a row
+  constexpr int kAcross = (kSets == 1 ? kWN : kN) / 4;  // lanes to a row
   const int column = lane % kAcross * 4;
   if constexpr (kSets == 1) {  // 32 rows at a time, each wave on its own
     float* const turn = reinterpret_cast<float*>(lds) + wave * 32 * T::kStride;
@@ -418,9 +431,10 @@ __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads
       }
       wave_lds_done();
     }
-  } else {  // every wave the tile's sums in its own LDS, then all of them rows of the whole
+  } else {  // every set its sums of the tile in its own LDS, then all of them rows of the whole
+    if constexpr (kWaves > 1) block_barrier();
 #pragma unroll
-    for (int i = 0; i < kI; ++i) give(reinterpret_cast<float*>(lds), i, 32 * i);
+    for (int i = 0; i < kI; ++i) give(reinterpret_cast<float*>(lds) + wn, i, wm + 32 * i);
     block_barrier();
     const int n = n0 + column;
     const float4_t bias = bias_row != nullptr ? load_features(bias_row, n, a.n) : none;
@@ -612,7 +626,15 @@ struct Join8 {
 };
 __device__ __forceinline__ float4_t sum_parts(const float* parts, std::int64_t row, int n, int width, int splits, std::int64_t part) {
   float4_t v = {0.0F, 0.0F, 0.0F, 0.0F};
-  for (int s = 0; s < splits; ++s) v = add4(v, load_features(parts + s * part + row, n, width));
+  if (splits == 1) return load_features(parts + row, n, width);
+  for (int s = 0; s < splits; s += 4) {  // four loads at a time
+    float4_t p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = load_features(parts + min(s + i, splits - 1) * part + row, n, width);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (s + i < splits) v = add4(v, p[i]);
+  }
   return v;
 }
 __global__ __launch_bounds__(256) void join_kernel(Join8 a) {
@@ -673,10 +695,11 @@ struct Way8 {
 };
 constexpr Way8 kWays[] = {
     {0, 32, 64, 4, 1, {1.5F, 1.5F}, {0.20F, 0.20F}},   {1, 64, 64, 4, 1, {2.8F, 2.8F}, {0.25F, 0.25F}},
-    {2, 64, 64, 2, 2, {3.1F, 3.7F}, {0.40F, 0.535F}},  {3, 128, 128, 1, 2, {7.0F, 7.7F}, {1.05F, 1.87F}},
-    {4, 256, 128, 1, 1, {7.0F, 7.0F}, {1.71F, 1.71F}}, {5, 256, 256, 1, 1, {13.7F, 13.7F}, {2.75F, 2.75F}},
+    {2, 64, 64, 2, 2, {3.1F, 3.7F}, {0.40F, 0.535F}},  {3, 128, 64, 2, 1, {2.7F, 2.7F}, {0.535F, 0.535F}},
+    {4, 128, 128, 1, 2, {7.0F, 7.7F}, {1.05F, 1.87F}}, {5, 256, 128, 1, 1, {7.0F, 7.0F}, {1.71F, 1.71F}},
+    {6, 256, 256, 1, 1, {13.7F, 13.7F}, {2.75F, 2.75F}},
 };
-constexpr int kFewRows = 6, kFusedGate = 7;
+constexpr int kFewRows = 7, kFusedGate = 8;
 struct Plan8 {
   int kind, splits;
 };
@@ -685,7 +708,7 @@ std::size_t part_bytes(const Product8& a, int splits) {
 }
 // What shares of the features cost in a second launch and in bytes at 4.5 TB/s.
 float join_cost(const Product8& a, int splits) {
-  return splits == 1 ? 0.0F : 2.0F + (splits + 1) * 4.0F * static_cast<float>(a.m) * static_cast<float>(a.n) / 4.5e6F;
+  return splits == 1 ? 0.0F : 4.5F + (splits + 1) * 4.0F * static_cast<float>(a.m) * static_cast<float>(a.n) / 4.5e6F;
 }
 // `gated`: the results go through float32 and a second launch to 8 bits, unless the tiles
 // of 256 x 256 do that themselves.
@@ -693,7 +716,7 @@ Plan8 plan_product(const Product8& a, bool gated, std::size_t workspace_bytes) {
   // Few rows of any number of weights, as far as a wave's registers hold its part of x:
   // 16 x 22528 x 4096 in 23.5 us (32 x 64 tiles: 24), 1 x 4096 x 4096 in 5.5 (8.9).
   if (a.m <= 16 && a.scale_pitch <= 24) return {kFewRows, 1};
-  Plan8 best{5, 1};
+  Plan8 best{0, 1};
   float least = 1e30F;
   for (const Way8& w : kWays) {
     const std::int64_t tiles = static_cast<std::int64_t>((a.m + w.m - 1) / w.m) * ((a.n + w.n - 1) / w.n);
@@ -722,9 +745,10 @@ int run_plan(const Product8& a, const Plan8& plan, float* parts, hipStream_t s) 
     case 0: return launch_product<32, 64, 32, 64, 4, 3>(a, plan.splits, parts, s);
     case 1: return launch_product<64, 64, 64, 64, 4, 2>(a, plan.splits, parts, s);
     case 2: return launch_product<64, 64, 64, 64, 2, 2>(a, plan.splits, parts, s);
-    case 3: return launch_product<128, 128, 64, 64, 1, 2>(a, plan.splits, parts, s);
-    case 4: return launch_product<256, 128, 64, 64, 1, 3>(a, plan.splits, parts, s);
-    case 5: return launch_product<256, 256, 128, 64, 1, 2>(a, plan.splits, parts, s);
+    case 3: return launch_product<128, 64, 64, 32, 2, 2>(a, plan.splits, parts, s);
+    case 4: return launch_product<128, 128, 64, 64, 1, 2>(a, plan.splits, parts, s);
+    case 5: return launch_product<256, 128, 64, 64, 1, 3>(a, plan.splits, parts, s);
+    case 6: return launch_product<256, 256, 128, 64, 1, 2>(a, plan.splits, parts, s);
     case kFusedGate: return launch_product<256, 256, 128, 64, 1, 2, true>(a, 1, nullptr, s);
     default: break;
   }
