@@ -632,7 +632,8 @@ int tcx_hip_beam_reorder(const void* const* in, void* const* out, const int64_t*
  * value at most 448 * 2^e; values are rounded to the nearest code, ties to even, at
  * most 2^-4 of themselves off, or 2^-10 of 2^e. NaN and infinities are held as NaN; a
  * value next to float32's largest may round to infinity. Codes are 16-byte aligned,
- * scales and float32 buffers 4-byte aligned. Nothing here allocates or waits. */
+ * scales and float32 buffers 4-byte aligned; outputs overlap no inputs but where that is
+ * said. Nothing here allocates or waits. */
 int64_t tcx_hip_block8_code_words(int64_t features);
 int64_t tcx_hip_block8_scale_words(int64_t features);
 /* x: rows of `features` float32, x_stride apart (0: features). Fewer than 2^31 words
@@ -649,7 +650,7 @@ typedef struct {
 } tcx_hip_rmsnorm8_desc_t;
 /* s = x + residual (x for NULL), y = s / sqrt(mean of s^2 + epsilon) * weight (1 for
  * NULL), all float32; y is quantised, and s written to sum unless that is NULL. sum
- * may be x or residual itself. */
+ * may be x or residual itself, with the same stride. */
 int tcx_hip_rmsnorm8(const float* x, const float* residual, const float* weight, float* sum, int32_t* codes, int32_t* scales,
                      const tcx_hip_rmsnorm8_desc_t* desc, tcx_stream_t stream);
 
@@ -661,17 +662,18 @@ typedef struct {
 } tcx_hip_linear8_desc_t;
 /* out = act(x w^T + bias) of x [rows, features] and w [outputs, features], both in 8
  * bits, as float32. Products are exact and summed in float32, in an order that goes
- * by the sizes, not by the call; a NaN makes its row (of w: its column) NaN. Scales
+ * by the sizes and the workspace's; a NaN makes its row (of w: its column) NaN. Scales
  * hold bytes of 27 to 247 as the functions above write them, and codes and scales
- * behind the last feature are zeros. The workspace (16-byte aligned, may be NULL)
- * takes the parts of sums split over blocks; the query says how much a call can use,
- * and it must stay allocated until the stream has run the call. */
+ * behind the last feature are zeros. No more results than 2^23 tiles of 32 x 64 or
+ * larger may be asked for. The workspace (16-byte aligned, may be NULL) takes the parts
+ * of sums split over blocks, as far as it has room; the query says how much a call can
+ * use, and it must stay allocated until the stream has run the call. */
 size_t tcx_hip_linear8_workspace_bytes(const tcx_hip_linear8_desc_t* desc);
 int tcx_hip_linear8(const int32_t* x_codes, const int32_t* x_scales, const int32_t* w_codes, const int32_t* w_scales, float* out,
                     const tcx_hip_linear8_desc_t* desc, void* workspace, size_t workspace_bytes, tcx_stream_t stream);
 /* act(x g^T + bias) * (x u^T + bias'), quantised: w holds the `outputs` rows of g, then
  * those of u, bias likewise; codes and scales have `outputs` features a row.
- * out_stride is 0. The workspace must have the query's size. */
+ * out_stride is 0. The workspace must have the query's size (0 for large products). */
 size_t tcx_hip_gated_linear8_workspace_bytes(const tcx_hip_linear8_desc_t* desc);
 int tcx_hip_gated_linear8(const int32_t* x_codes, const int32_t* x_scales, const int32_t* w_codes, const int32_t* w_scales,
                           int32_t* codes, int32_t* scales, const tcx_hip_linear8_desc_t* desc, void* workspace,

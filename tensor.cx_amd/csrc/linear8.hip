@@ -93,6 +93,9 @@ __device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, void* lds, 
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voffset, soffset, 0, 0);
 }
 
+// An offset past every buffer here (of at most 256 rows of 2^22 bytes), with any scalar
+// offset added: such a load gives zeros.
+constexpr int kNowhere = 0x7fff0000;
 // Four bytes a lane straight into LDS.
 __device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t r, void* lds, int voffset, int soffset) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 4, voffset, soffset, 0, 0);
@@ -123,7 +126,7 @@ __device__ __forceinline__ void wave_lds_done() { asm volatile("s_waitcnt lgkmcn
 // a small tile each would make. Sets of more waves share the barriers.
 //
 // With kGate the tile has 128 columns of gate and the same ones of up, 32 of each by turns,
-// and its results leave in 8 bits: 4096 x (2 x 11264) x 4096 in 586 us, in two launches
+// and its results leave in 8 bits: 4096 x (2 x 11264) x 4096 in 609 us, in two launches
 // with float32 between them 709.
 //
 // The features may be split over the grid's rows (Product8::parts).
@@ -472,144 +475,142 @@ int launch_product(Product8 a, int splits, float* parts, hipStream_t s) {
   return check(hipGetLastError(), "linear8 launch");
 }
 
-// Few rows: each weight is read once, straight into the registers that multiply it.
-// The eight waves of a block share the features of a tile of sixteen weights' rows: wave
+// Up to sixteen rows: each weight is read once, straight into the registers that multiply
+// it. The eight waves of a block share the features of a tile of sixteen weights' rows: wave
 // p takes units (four blocks of 128) p, p + 8 and so on, kU of them, whose part of x it
 // keeps in registers from tile to tile while the next unit's weights are under way.
 // Lane (r, g) holds 16-byte pieces g and 4 + g of each block of row r. The waves' sums
 // of a tile meet in LDS.
-// The units may be split over the grid's rows (Product8::parts).
-template <int kT, int kU>
+//
+// Bound by reading the weights: 8 x 128256 x 4096 in 95 us, 5.6 TB/s; 1 x 4096 x 4096 in
+// 6.6 (5.8 from the cache), of which 2.4 are the launch. Loads that stay out of the caches
+// (106), a unit more under way (97) and two (102), 512 blocks (97) and waves with all
+// features of a tile of their own (124) were slower for the first.
+template <int kU>
 __global__ __launch_bounds__(512) void few_rows_kernel(Product8 a) {
-  __shared__ float4_t sums[2][8][kT][64];
+  __shared__ float4_t sums[2][8][64];
   constexpr int kStaged = 8;
-  __shared__ int4_t stages[kT == 1 && kU == 1 ? 8 : 1][kT == 1 && kU == 1 ? kStaged * 32 : 1];
+  __shared__ int4_t stages[kU == 1 ? 8 : 1][kU == 1 ? kStaged * 32 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & 15, g = lane >> 4;
-  const auto [first, units] = share_of(a, static_cast<int>(blockIdx.y));
+  const int r = lane & 15, g = lane >> 4, units = a.scale_pitch;
+
+  // Blocks past the row's end are zeros in x, so whatever w has there adds nothing; w's are
+  // read from the row's last block. Of few rows each is brought once, 512 bytes of two rows
+  // a load, and spread through the wave's own LDS: 1 x 4096 x 4096 in 6.7 us for 7.4.
+  int4_t x[kU][8], stage[kStaged / 2];
+  std::uint32_t x_word[kU];
+  const auto x_rsrc = row_buffer(a.x, 0, a.m, a.pitch);
+  const bool staged = kU == 1 && a.m <= kStaged;
+  if (staged) {
+#pragma unroll
+    for (int t = 0; t < kStaged / 2; ++t) {
+      const int row = 2 * t + (lane >> 5), at = 16 * (lane & 31);
+      if (2 * t < a.m)
+        stage[t] = load16(x_rsrc, row < a.m && wave < units && at < (a.blocks - 4 * wave) * 128 ? row * a.pitch + at : kNowhere, wave * 512);
+    }
+  }
+  const int x_row = min(r, a.m - 1);
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const int unit = wave + 8 * u;
+    x_word[u] = unit < units ? a.x_scale[static_cast<std::int64_t>(x_row) * a.scale_pitch + unit] : 0;
+    if (staged) continue;
+#pragma unroll
+    for (int p = 0; p < 8; ++p)
+      x[u][p] = load16(x_rsrc, unit < units && 4 * unit + p / 2 < a.blocks ? x_row * a.pitch + 16 * g + 64 * p : kNowhere, unit * 512);
+  }
 
   struct Weights {
     int4_t piece[8];
     std::uint32_t word;
   };
   auto load = [&](Weights& w, int tile, int u) {
-    const int rows = min(a.n - 16 * tile, 16), unit = min(first + wave + 8 * u, units - 1);
+    const int rows = min(a.n - 16 * tile, 16), unit = min(wave + 8 * u, units - 1);
     const auto rsrc = row_buffer(a.w, 16 * tile, rows, a.pitch);
     const int row = min(r, rows - 1), at = row * a.pitch + 16 * g;
     w.word = a.w_scale[static_cast<std::int64_t>(16 * tile + row) * a.scale_pitch + unit];
 #pragma unroll
     for (int p = 0; p < 8; ++p) w.piece[p] = load16(rsrc, at + 64 * (p & 1), min(4 * unit + p / 2, a.blocks - 1) * 128);
   };
-  // Blocks past the row's end are zeros in x, so whatever w has there adds nothing; w's are
-  // read from the row's last block.
-  int4_t x[kU][kT][8];
-  std::uint32_t x_word[kU][kT];
-  const auto x_rsrc = row_buffer(a.x, 0, a.m, a.pitch);
-  const bool staged = kT == 1 && kU == 1 && a.m <= kStaged;
-  int4_t stage[kStaged / 2];
-  if (staged) {
-#pragma unroll
-    for (int t = 0; t < kStaged / 2; ++t) {
-      const int row = 2 * t + (lane >> 5), unit = first + wave;
-      if (2 * t < a.m)
-        stage[t] = load16(x_rsrc, row < a.m && unit < units && 16 * (lane & 31) < (a.blocks - 4 * unit) * 128 ? row * a.pitch + 16 * (lane & 31) : -1,
-                          unit * 512);
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < kU; ++u) {
-    const int unit = first + wave + 8 * u;
-#pragma unroll
-    for (int t = 0; t < kT; ++t) {
-      const int row = min(16 * t + r, a.m - 1);
-      x_word[u][t] = unit < units ? a.x_scale[static_cast<std::int64_t>(row) * a.scale_pitch + unit] : 0;
-      if (staged) continue;
-#pragma unroll
-      for (int p = 0; p < 8; ++p)
-        x[u][t][p] = load16(x_rsrc, unit < units && 4 * unit + p / 2 < a.blocks ? row * a.pitch + 16 * g + 64 * p : -1, unit * 512);
-    }
-  }
   int tile = static_cast<int>(blockIdx.x);
   Weights now, next;
   load(now, tile, 0);
   if (staged) {
-    // A wave's own rows, its own LDS: piece q of row r at q ^ (r & 7).
+    // Piece q of row m stands at q ^ (m & 7).
     int4_t* const own = stages[wave];
 #pragma unroll
     for (int t = 0; t < kStaged / 2; ++t) {
       const int row = 2 * t + (lane >> 5);
       if (2 * t < a.m) own[row * 32 + ((lane & 31) ^ (row & 7))] = stage[t];
     }
-    const int row = min(r, a.m - 1);
 #pragma unroll
-    for (int p = 0; p < 8; ++p) x[0][0][p] = own[row * 32 + ((4 * p + g) ^ (row & 7))];
+    for (int p = 0; p < 8; ++p) x[0][p] = own[x_row * 32 + ((4 * p + g) ^ (x_row & 7))];
   }
-  float4_t acc[kT];
+
+  float4_t acc;
   auto compute = [&](const Weights& w, int u) {
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
-      const float w_unit = unit_of(w.word, p / 2);
-      const bf8_t w0 = widen<0>(w.piece[p], w_unit), w1 = widen<1>(w.piece[p], w_unit);
-#pragma unroll
-      for (int t = 0; t < kT; ++t) {
-        int4_t codes = x[u][t][p];
-        if constexpr (kT * kU > 1) asm volatile("" : "+v"(codes));  // kept as codes: widened once they would take twice the registers
-        const float x_unit = unit_of(x_word[u][t], p / 2);
-        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w0, widen<0>(codes, x_unit), acc[t], 0, 0, 0);
-        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w1, widen<1>(codes, x_unit), acc[t], 0, 0, 0);
-      }
+      const float w_unit = unit_of(w.word, p / 2), x_unit = unit_of(x_word[u], p / 2);
+      int4_t codes = x[u][p];
+      if constexpr (kU > 1) asm volatile("" : "+v"(codes));  // kept as codes: widened once they would take twice the registers
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen<0>(w.piece[p], w_unit), widen<0>(codes, x_unit), acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen<1>(w.piece[p], w_unit), widen<1>(codes, x_unit), acc, 0, 0, 0);
     }
   };
-  auto finish = [&](int tile, int turn) {
-#pragma unroll
-    for (int t = 0; t < kT; ++t) sums[turn][wave][t][lane] = acc[t];
+  // Thread i of the first 256 gives result i % 16 of the tile and row i / 16 (lane (m, g)
+  // has results 4 g on of row m).
+  const int m = static_cast<int>(threadIdx.x) >> 4, column = static_cast<int>(threadIdx.x) & 15;
+  auto bias_of = [&](int tile) {  // asked for before the next weights are
+    return a.bias != nullptr && threadIdx.x < 256 ? a.bias[min(16 * tile + column, a.n - 1)] : 0.0F;
+  };
+  auto finish = [&](int tile, int turn, float bias) {
+    sums[turn][wave][lane] = acc;
     __syncthreads();
-    // Thread i of the first kT * 256: result i % 16 of the tile and row i / 16 (lane (row, g) had results 4 g on).
-    for (int i = threadIdx.x; i < kT * 256; i += 512) {
-      const int m = i >> 4, n = 16 * tile + (i & 15);
-      const float* at = reinterpret_cast<const float*>(&sums[turn][0][m >> 4][(m & 15) + 16 * ((i & 15) >> 2)]) + (i & 3);
-      float v = 0.0F;
+    const int n = 16 * tile + column;
+    if (threadIdx.x >= 256 || m >= a.m || n >= a.n) return;
+    const float* const at = reinterpret_cast<const float*>(&sums[turn][0][m + 16 * (column >> 2)]) + (column & 3);
+    float v = 0.0F;
 #pragma unroll
-      for (int p = 0; p < 8; ++p) v += at[p * kT * 256];
-      if (m >= a.m || n >= a.n) continue;
-      if (a.parts != nullptr) {
-        a.parts[(static_cast<std::int64_t>(blockIdx.y) * a.m + m) * a.n + n] = v;
-      } else {
-        if (a.bias != nullptr) v += a.bias[n];
-        a.out[m * a.out_stride + n] = activate8(v, a.activation);
-      }
-    }
+    for (int p = 0; p < 8; ++p) v += at[p * 256];
+    a.out[m * a.out_stride + n] = activate8(v + bias, a.activation);
   };
 
   int turn = 0;
   while (true) {
     const int after = tile + static_cast<int>(gridDim.x);
-#pragma unroll
-    for (int t = 0; t < kT; ++t) acc[t] = float4_t{0.0F, 0.0F, 0.0F, 0.0F};
+    const float bias = bias_of(tile);
+    acc = float4_t{0.0F, 0.0F, 0.0F, 0.0F};
 #pragma unroll
     for (int u = 0; u + 1 < kU; ++u) {
       load(next, tile, u + 1);
       compute(now, u);
       now = next;
     }
-    if (after >= a.tiles_n) break;
+    if (after >= a.tiles_n) {
+      compute(now, kU - 1);
+      finish(tile, turn, bias);
+      return;
+    }
     load(next, after, 0);
     compute(now, kU - 1);
-    finish(tile, turn);
+    finish(tile, turn, bias);
     now = next;
     tile = after;
     turn ^= 1;
   }
-  compute(now, kU - 1);
-  finish(tile, turn);
 }
 
-template <int kT, int kU>
-int launch_few_rows(Product8 a, int splits, float* parts, hipStream_t s) {
+template <int kU>
+int launch_few_rows(Product8 a, float* parts, hipStream_t s) {
   a.tiles_n = (a.n + 15) / 16;
-  share_out(a, a.scale_pitch, splits, parts);
-  const int grid = std::max(1, std::min(a.tiles_n, 256 / splits));
-  hipLaunchKernelGGL((few_rows_kernel<kT, kU>), dim3(static_cast<unsigned>(grid), static_cast<unsigned>(splits)), dim3(512), 0, s, a);
+  if (parts != nullptr) {  // the one part of a gated product's results
+    a.out = parts;
+    a.out_stride = a.n;
+    a.bias = nullptr;
+    a.activation = TCX_ACT_NONE;
+  }
+  hipLaunchKernelGGL(few_rows_kernel<kU>, dim3(static_cast<unsigned>(std::min(a.tiles_n, 256))), dim3(512), 0, s, a);
   return check(hipGetLastError(), "linear8 launch");
 }
 
@@ -752,9 +753,9 @@ int run_plan(const Product8& a, const Plan8& plan, float* parts, hipStream_t s) 
     case kFusedGate: return launch_product<256, 256, 128, 64, 1, 2, true>(a, 1, nullptr, s);
     default: break;
   }
-  if (a.scale_pitch <= 8) return launch_few_rows<1, 1>(a, plan.splits, parts, s);
-  if (a.scale_pitch <= 16) return launch_few_rows<1, 2>(a, plan.splits, parts, s);
-  return launch_few_rows<1, 3>(a, plan.splits, parts, s);
+  if (a.scale_pitch <= 8) return launch_few_rows<1>(a, parts, s);
+  if (a.scale_pitch <= 16) return launch_few_rows<2>(a, parts, s);
+  return launch_few_rows<3>(a, parts, s);
 }
 
 // Checks a descriptor and fills what follows from it; `gated`: weights of 2 * outputs rows.
