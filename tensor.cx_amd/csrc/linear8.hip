@@ -30,7 +30,7 @@ struct Product8 {
   std::int64_t out_stride;
   int m, n, blocks, pitch, scale_pitch;  // blocks of 128 features; bytes and words between rows
   int activation;
-  int tiles_m, tiles_n;
+  int tiles_m, tiles_n, whole;  // `whole`: how many of the tiles go to one block each
   FastDiv by_group;  // work items in eight tile rows
   // Sums over shares of the features, one to a row of blocks: share s has `each` blocks
   // (or units of four) and one more if s < extra, and its sums go to parts [s][m][n].
@@ -70,9 +70,11 @@ __device__ __forceinline__ float unit_of(std::uint32_t word, int kt) {
 struct Tile8 {
   int m, n;
 };
-__device__ __forceinline__ Tile8 tile_of(const Product8& a, int block) {
-  const int total = a.tiles_m * a.tiles_n, share = total >> 3, rest = total & 7, xcd = block & 7;
-  const int id = xcd * share + min(xcd, rest) + (block >> 3);
+__device__ __forceinline__ int item_of(int block, int total) {
+  const int share = total >> 3, rest = total & 7, xcd = block & 7;
+  return xcd * share + min(xcd, rest) + (block >> 3);
+}
+__device__ __forceinline__ Tile8 tile_of(const Product8& a, int id) {
   const int group = static_cast<int>(a.by_group(static_cast<std::uint32_t>(id))), in = id - group * 8 * a.tiles_n;
   const int deep = min(a.tiles_m - group * 8, 8);
   if (deep == 8) return {group * 8 + (in & 7), in >> 3};
@@ -127,7 +129,7 @@ __device__ __forceinline__ void wave_lds_done() { asm volatile("s_waitcnt lgkmcn
 // a small tile each would make. Sets of more waves share the barriers.
 //
 // With kGate the tile has 128 columns of gate and the same ones of up, 32 of each by turns,
-// and its results leave in 8 bits: 4096 x (2 x 11264) x 4096 in 609 us, in two launches
+// and its results leave in 8 bits: 4096 x (2 x 11264) x 4096 in 595 us, in two launches
 // with float32 between them 709.
 //
 // The features may be split over the grid's rows (Product8::parts).
@@ -151,16 +153,13 @@ struct Tiles8 {
   static_assert(kSets == 1 ? kWaves * 32 * kStride * 4 <= kScales : kM * kStride * 4 <= kScales);
 };
 template <int kM, int kN, int kWM, int kWN, int kSets, int kStages, bool kGate>
-__global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads)) void product_kernel(Product8 a) {
+__device__ __forceinline__ void product_tile(const Product8& a, Tile8 tile, std::uint8_t* memory) {
   using T = Tiles8<kM, kN, kWM, kWN, kSets, kStages>;
   constexpr int kWavesN = T::kWavesN, kWaves = T::kWaves, kI = T::kI, kJ = T::kJ, kLoads = T::kLoads;
   constexpr int kScaled = T::kScaled;
-  __shared__ __attribute__((aligned(1024))) std::uint8_t memory[T::kLds];
-
   const int lane = threadIdx.x & 63, thread_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int set = thread_wave / kWaves, wave = thread_wave % kWaves;
   std::uint8_t* const lds = memory + set * T::kSetBytes;
-  const Tile8 tile = tile_of(a, static_cast<int>(blockIdx.x));
   const auto [share_first, last] = share_of(a, static_cast<int>(blockIdx.y));
   const int first = share_first + set;
   const int m0 = tile.m * kM, n0 = tile.n * (kGate ? kN / 2 : kN);
@@ -172,7 +171,7 @@ __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads
   // Row of w, from n0 on, that row `row` of w's part of the buffer holds (of gate or up, by bit 5).
   auto w_row = [&](int row) { return min(kGate ? (row >> 6 << 5) + (row & 31) : row, n_last); };
   const std::int64_t w_first = n0 + (kGate && ((wave >> 2) & 1) ? a.outputs : 0);  // a wave's loads are of gate, or of up
-  static_assert(!kGate || (kWaves == 8 && kM == 256 && kN == 256 && kWN == 64 && kSets == 1));
+  static_assert(!kGate || (kWaves == 8 && 2 * kWM == kM && kN == 256 && kWN == 64 && kSets == 1));
   int offset[kLoads];
   bool of_x[kLoads];
 #pragma unroll
@@ -455,13 +454,33 @@ __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads
   }
 }
 
+// With kHalves the tiles past the last whole round of 256, if they leave half the CUs
+// empty, are taken by two blocks each, one for the rows of either half (from tile a.whole
+// on): 4096 x 5120 x 4096, 320 tiles, in 157 us, else 193.
+constexpr int kHalved = 128;
+template <int kM, int kN, int kWM, int kWN, int kSets, int kStages, bool kGate, bool kHalves>
+__global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads)) void product_kernel(Product8 a) {
+  __shared__ __attribute__((aligned(1024))) std::uint8_t memory[Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kLds];
+  const int block = static_cast<int>(blockIdx.x);
+  if constexpr (kHalves) {
+    if (block >= a.whole) {
+      const int rest = a.tiles_m * a.tiles_n - a.whole, second = block - a.whole >= rest ? 1 : 0;
+      Tile8 tile = tile_of(a, a.whole + item_of(block - a.whole - second * rest, rest));
+      tile.m = 2 * tile.m + second;
+      if (tile.m * (kM / 2) < a.m) product_tile<kM / 2, kN, kWM / 2, kWN, kSets, kStages, kGate>(a, tile, memory);
+      return;
+    }
+  }
+  product_tile<kM, kN, kWM, kWN, kSets, kStages, kGate>(a, tile_of(a, item_of(block, a.whole)), memory);
+}
+
 void share_out(Product8& a, int units, int splits, float* parts) {
   a.parts = parts;
   a.each = units / splits;
   a.extra = units % splits;
 }
 
-template <int kM, int kN, int kWM, int kWN, int kSets, int kStages, bool kGate = false>
+template <int kM, int kN, int kWM, int kWN, int kSets, int kStages, bool kGate = false, bool kHalves = false>
 int launch_product(Product8 a, int splits, float* parts, hipStream_t s) {
   a.tiles_m = (a.m + kM - 1) / kM;
   a.tiles_n = kGate ? a.gate_blocks : (a.n + kN - 1) / kN;
@@ -469,9 +488,12 @@ int launch_product(Product8 a, int splits, float* parts, hipStream_t s) {
   share_out(a, a.blocks, splits, parts);
   constexpr int kThreads = Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads;
   const std::int64_t tiles = static_cast<std::int64_t>(a.tiles_m) * a.tiles_n;
-  if (tiles * splits * kThreads > kMaxLaunchWorkItems || tiles >= (std::int64_t{1} << 30))
+  const std::int64_t rest = tiles * splits % 256, halved = kHalves && rest > 0 && rest <= kHalved ? tiles % 256 : 0;
+  if ((tiles + halved) * splits * kThreads > kMaxLaunchWorkItems || tiles >= (std::int64_t{1} << 30))
     return fail(TCX_INVALID_ARGUMENT, "linear8 has too many results");
-  hipLaunchKernelGGL((product_kernel<kM, kN, kWM, kWN, kSets, kStages, kGate>), dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(splits)),
+  a.whole = static_cast<int>(tiles - halved);
+  hipLaunchKernelGGL((product_kernel<kM, kN, kWM, kWN, kSets, kStages, kGate, kHalves>),
+                     dim3(static_cast<unsigned>(tiles + halved), static_cast<unsigned>(splits)),
                      dim3(kThreads), 0, s, a);
   return check(hipGetLastError(), "linear8 launch");
 }
@@ -690,7 +712,8 @@ __global__ __launch_bounds__(256) void gate_kernel(Gate8 a) {
 // The ways to a product, and what a round of blocks on all 256 CUs took, in us: `fixed`
 // (start, first loads, results) and `step` for each block of 128 features, with one
 // block a CU and with as many as fit (n = 4096, 1024 to 8192 features, weights in the
-// cache; few rows and tiles that leave CUs empty a little less).
+// cache; few rows and tiles that leave CUs empty a little less). Of 256 x 256: with halves
+// of at most 128 tiles, and with whole ones.
 struct Way8 {
   int kind, m, n, sets, fit;  // tile, and blocks that a CU holds
   float fixed[2], step[2];
@@ -699,7 +722,7 @@ constexpr Way8 kWays[] = {
     {0, 32, 64, 4, 1, {1.5F, 1.5F}, {0.20F, 0.20F}},   {1, 64, 64, 4, 1, {2.8F, 2.8F}, {0.25F, 0.25F}},
     {2, 64, 64, 2, 2, {3.1F, 3.7F}, {0.40F, 0.535F}},  {3, 128, 64, 2, 1, {2.7F, 2.7F}, {0.535F, 0.535F}},
     {4, 128, 128, 1, 2, {7.0F, 7.7F}, {1.05F, 1.87F}}, {5, 256, 128, 1, 1, {7.0F, 7.0F}, {1.71F, 1.71F}},
-    {6, 256, 256, 1, 1, {13.7F, 13.7F}, {2.75F, 2.75F}},
+    {6, 256, 256, 1, 1, {10.0F, 13.7F}, {1.74F, 2.75F}},
 };
 constexpr int kFewRows = 7, kFusedGate = 8;
 struct Plan8 {
@@ -728,7 +751,8 @@ Plan8 plan_product(const Product8& a, bool gated, std::size_t workspace_bytes) {
       const float steps = static_cast<float>((a.blocks + splits - 1) / splits);
       const std::int64_t rounds = blocks / (256 * w.fit), rest = blocks - rounds * 256 * w.fit;
       float time = static_cast<float>(rounds) * (w.fixed[1] + steps * w.step[1]);
-      if (rest > 0) time += w.fixed[rest > 256] + steps * w.step[rest > 256];
+      const bool full = rest > (w.kind == 6 ? kHalved : 256);
+      if (rest > 0) time += w.fixed[full] + steps * w.step[full];
       time += gated ? join_cost(a, splits + 1) : join_cost(a, splits);
       if (time < least) {
         least = time;
@@ -738,7 +762,10 @@ Plan8 plan_product(const Product8& a, bool gated, std::size_t workspace_bytes) {
   }
   if (gated && (static_cast<std::int64_t>(a.outputs) + 256) * 4 * a.scale_pitch < (std::int64_t{1} << 31)) {
     const std::int64_t tiles = static_cast<std::int64_t>((a.m + 255) / 256) * a.gate_blocks;
-    if (static_cast<float>((tiles + 255) / 256) * (12.0F + static_cast<float>(a.blocks) * 2.75F) < least) best = {kFusedGate, 1};
+    const std::int64_t rest = tiles % 256;
+    float time = static_cast<float>(tiles / 256 + (rest > kHalved ? 1 : 0)) * (12.0F + static_cast<float>(a.blocks) * 2.75F);
+    if (rest > 0 && rest <= kHalved) time += 9.0F + static_cast<float>(a.blocks) * 1.74F;
+    if (time < least) best = {kFusedGate, 1};
   }
   return best;
 }
@@ -750,8 +777,8 @@ int run_plan(const Product8& a, const Plan8& plan, float* parts, hipStream_t s) 
     case 3: return launch_product<128, 64, 64, 32, 2, 2>(a, plan.splits, parts, s);
     case 4: return launch_product<128, 128, 64, 64, 1, 2>(a, plan.splits, parts, s);
     case 5: return launch_product<256, 128, 64, 64, 1, 3>(a, plan.splits, parts, s);
-    case 6: return launch_product<256, 256, 128, 64, 1, 2>(a, plan.splits, parts, s);
-    case kFusedGate: return launch_product<256, 256, 128, 64, 1, 2, true>(a, 1, nullptr, s);
+    case 6: return launch_product<256, 256, 128, 64, 1, 2, false, true>(a, plan.splits, parts, s);
+    case kFusedGate: return launch_product<256, 256, 128, 64, 1, 2, true, true>(a, 1, nullptr, s);
     default: break;
   }
   if (a.scale_pitch <= 8) return launch_few_rows<1>(a, parts, s);

@@ -163,7 +163,7 @@ PRODUCTS = [(1, 1, 1), (1, 16, 128), (1, 100, 300), (1, 4096, 1024), (1, 257, 11
 # Sizes past those above that take each of the tiles: 64 x 64 on four and on two waves, 128 x
 # 64, 128 x 128, 256 x 128 and 256 x 256, with rows, results and features that end inside one
 TILES = [(250, 4001, 1000), (100, 8192, 300), (64, 20000, 200), (700, 3000, 300), (260, 16400, 129), (1025, 4100, 256), (2040, 8190, 300),
-         (3900, 4000, 130), (64, 4096, 11264)]
+         (3900, 4000, 130), (64, 4096, 11264), (3900, 5100, 1300)]
 
 
 @pytest.mark.parametrize("shape", PRODUCTS + TILES, ids=str)
@@ -200,7 +200,7 @@ def test_linear_keeps_every_bit_of_whole_numbers(cx, shape):
 
 
 @pytest.mark.parametrize("activation", ["none", "silu", "gelu"])
-@pytest.mark.parametrize("shape", [(1, 200, 300), (9, 200, 300), (40, 130, 700), (300, 200, 300), (20, 130, 9000), (1025, 4100, 256)], ids=str)
+@pytest.mark.parametrize("shape", [(1, 200, 300), (9, 200, 300), (40, 130, 700), (300, 200, 300), (20, 130, 9000), (1025, 4100, 256), (4100, 5000, 700)], ids=str)
 def test_linear_bias_and_activation(cx, shape, activation):
     rows, outputs, features = shape
     rng = np.random.default_rng(rows)
@@ -263,7 +263,7 @@ def test_linear_of_nothing(cx):
 # rows, outputs, features
 GATED = [(1, 1, 128), (1, 300, 1000), (2, 128, 256), (7, 129, 300), (16, 1100, 384), (33, 513, 640), (70, 256, 100), (129, 260, 1300),
          (300, 140, 513), (520, 900, 256), (1100, 3000, 129), (2050, 1000, 384), (2300, 2570, 200),
-         (64, 11264, 300), (100, 3000, 1000), (260, 2000, 700), (600, 3000, 300), (130, 700, 8000), (40, 300, 9000)]
+         (64, 11264, 300), (100, 3000, 1000), (260, 2000, 700), (600, 3000, 300), (130, 700, 8000), (40, 300, 9000), (4000, 2600, 200)]
 
 
 @pytest.mark.parametrize("bias", [False, True])
