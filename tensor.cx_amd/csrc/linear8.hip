@@ -120,8 +120,8 @@ __device__ __forceinline__ void wave_lds_done() { asm volatile("s_waitcnt lgkmcn
 // into one of kStages buffers in LDS, kStages - 1 steps ahead. Row r's sixteen-byte
 // pieces stand in the order piece ^ (r / 2 & 7): the 64 banks hold two rows, so the reads
 // of sixteen neighbouring rows lie in different banks (8192^3 in 787 us; in the order
-// piece ^ (r & 7), with conflicts in 46 % of the LDS cycles, 793). Words of exponents, of four steps each,
-// have two buffers of their own.
+// piece ^ (r & 7), with conflicts in 46 % of the LDS cycles, 793). Words of exponents, of
+// four steps each, have two buffers of their own.
 //
 // With kSets > 1 there are as many sets of waves, each with the whole tile for every
 // kSets-th step and with LDS of its own; their sums meet at the end. A set of one wave
@@ -506,7 +506,7 @@ int launch_product(Product8 a, int splits, float* parts, hipStream_t s) {
 // of a tile meet in LDS.
 //
 // Bound by reading the weights: 8 x 128256 x 4096 in 95 us, 5.6 TB/s; 1 x 4096 x 4096 in
-// 6.6 (5.8 from the cache), of which 2.4 are the launch. Loads that stay out of the caches
+// 5.8 (4.7 from the cache), of which 2.4 are the launch. Loads that stay out of the caches
 // (106), a unit more under way (97) and two (102), 512 blocks (97) and waves with all
 // features of a tile of their own (124) were slower for the first.
 template <int kU>
@@ -711,20 +711,25 @@ __global__ __launch_bounds__(256) void gate_kernel(Gate8 a) {
 
 // The ways to a product, and what a round of blocks on all 256 CUs took, in us: `fixed`
 // (start, first loads, results) and `step` for each block of 128 features, with one
-// block a CU and with as many as fit (n = 4096, 1024 to 8192 features, weights in the
-// cache; few rows and tiles that leave CUs empty a little less). Of 256 x 256: with halves
-// of at most 128 tiles, and with whole ones.
+// block a CU and with as many as fit, which rounds before the last have (n = 4096, 1024
+// to 8192 features, weights in the cache, few rows a little less; ways 0 and 2: also n up
+// to 128256 with weights from memory). Of 256 x 256: with halves of at most 128 tiles,
+// and with whole ones. Few features over many tiles are for way 2, whose four blocks a CU
+// hide one's start and results behind another's products: 25 x 126974 x 139 in 16 us, way
+// 0 in 30.
 struct Way8 {
   int kind, m, n, sets, fit;  // tile, and blocks that a CU holds
   float fixed[2], step[2];
 };
 constexpr Way8 kWays[] = {
-    {0, 32, 64, 4, 1, {1.5F, 1.5F}, {0.20F, 0.20F}},   {1, 64, 64, 4, 1, {2.8F, 2.8F}, {0.25F, 0.25F}},
-    {2, 64, 64, 2, 2, {3.1F, 3.7F}, {0.40F, 0.535F}},  {3, 128, 64, 2, 1, {2.7F, 2.7F}, {0.535F, 0.535F}},
+    {0, 32, 64, 4, 1, {1.5F, 2.4F}, {0.20F, 0.345F}},  {1, 64, 64, 4, 1, {2.8F, 2.8F}, {0.25F, 0.25F}},
+    {2, 64, 64, 1, 4, {1.4F, 4.2F}, {0.60F, 1.22F}},   {3, 128, 64, 2, 1, {2.7F, 2.7F}, {0.535F, 0.535F}},
     {4, 128, 128, 1, 2, {7.0F, 7.7F}, {1.05F, 1.87F}}, {5, 256, 128, 1, 1, {7.0F, 7.0F}, {1.71F, 1.71F}},
     {6, 256, 256, 1, 1, {10.0F, 13.7F}, {1.74F, 2.75F}},
 };
 constexpr int kFewRows = 7, kFusedGate = 8;
+// A microsecond's reading of weights from memory.
+constexpr float kReads = 5.4e6F;
 struct Plan8 {
   int kind, splits;
 };
@@ -738,21 +743,33 @@ float join_cost(const Product8& a, int splits) {
 // `gated`: the results go through float32 and a second launch to 8 bits, unless the tiles
 // of 256 x 256 do that themselves.
 Plan8 plan_product(const Product8& a, bool gated, std::size_t workspace_bytes) {
-  // Few rows of any number of weights, as far as a wave's registers hold its part of x:
-  // 16 x 22528 x 4096 in 23.5 us (32 x 64 tiles: 24), 1 x 4096 x 4096 in 5.5 (8.9).
-  if (a.m <= 16 && a.scale_pitch <= 24) return {kFewRows, 1};
   Plan8 best{0, 1};
   float least = 1e30F;
+  // Few rows, as far as a wave's registers hold its part of x: a round of 256 tiles takes
+  // its weights' bytes or a chain of 1.8 us for 4096 features. 16 x 22528 x 4096 in 22 us (32 x 64 tiles: 26),
+  // 1 x 4096 x 4096 in 5.8 (8.9); but 8 x 60000 x 1024 in 30 (64 x 64 tiles: 17).
+  if (a.m <= 16 && a.scale_pitch <= 24) {
+    const float chain = 1.8F * static_cast<float>((a.scale_pitch + 7) / 8), row = static_cast<float>(a.pitch) / kReads;
+    least = static_cast<float>(a.n / 4096) * std::max(chain, 4096.0F * row) + std::max(chain, static_cast<float>(a.n % 4096) * row);
+    if (gated) least += join_cost(a, 2);
+    best = {kFewRows, 1};
+  }
   for (const Way8& w : kWays) {
     const std::int64_t tiles = static_cast<std::int64_t>((a.m + w.m - 1) / w.m) * ((a.n + w.n - 1) / w.n);
     for (int splits = 1; splits <= 16; splits = splits < 4 ? splits + 1 : splits * 3 / 2) {
-      const std::int64_t blocks = tiles * splits;
-      if (splits > 1 && (blocks > 256 * w.fit || a.blocks < splits * w.sets || part_bytes(a, splits) > workspace_bytes)) break;
+      const std::int64_t blocks = tiles * splits, fit = 256 * w.fit;
+      if (splits > 1 && (blocks > fit || a.blocks < splits * w.sets || part_bytes(a, splits) > workspace_bytes)) break;
       const float steps = static_cast<float>((a.blocks + splits - 1) / splits);
-      const std::int64_t rounds = blocks / (256 * w.fit), rest = blocks - rounds * 256 * w.fit;
-      float time = static_cast<float>(rounds) * (w.fixed[1] + steps * w.step[1]);
-      const bool full = rest > (w.kind == 6 ? kHalved : 256);
-      if (rest > 0) time += w.fixed[full] + steps * w.step[full];
+      // `full`: 0 with a block on each CU to 1 with as many as fit. Weights that one row of
+      // tiles reads come from memory (split ones, of few outputs, were in the cache when timed).
+      auto round = [&](std::int64_t count, float full) {
+        const float bytes = a.m <= w.m && splits == 1 ? static_cast<float>(count * w.n * kBlock8) / kReads : 0.0F;
+        return w.fixed[0] + full * (w.fixed[1] - w.fixed[0]) + steps * std::max(w.step[0] + full * (w.step[1] - w.step[0]), bytes);
+      };
+      const std::int64_t rounds = (blocks - 1) / fit, rest = blocks - rounds * fit;  // whole ones, and the last's blocks
+      float full = w.fit > 1 ? static_cast<float>((rest - 1) / 256) / static_cast<float>(w.fit - 1) : 0.0F;
+      if (w.kind == 6 && rest > kHalved) full = 1.0F;
+      float time = static_cast<float>(rounds) * round(fit, 1.0F) + round(rest, full);
       time += gated ? join_cost(a, splits + 1) : join_cost(a, splits);
       if (time < least) {
         least = time;
@@ -773,7 +790,7 @@ int run_plan(const Product8& a, const Plan8& plan, float* parts, hipStream_t s) 
   switch (plan.kind) {
     case 0: return launch_product<32, 64, 32, 64, 4, 3>(a, plan.splits, parts, s);
     case 1: return launch_product<64, 64, 64, 64, 4, 2>(a, plan.splits, parts, s);
-    case 2: return launch_product<64, 64, 64, 64, 2, 2>(a, plan.splits, parts, s);
+    case 2: return launch_product<64, 64, 32, 32, 1, 2>(a, plan.splits, parts, s);
     case 3: return launch_product<128, 64, 64, 32, 2, 2>(a, plan.splits, parts, s);
     case 4: return launch_product<128, 128, 64, 64, 1, 2>(a, plan.splits, parts, s);
     case 5: return launch_product<256, 128, 64, 64, 1, 3>(a, plan.splits, parts, s);

@@ -163,7 +163,8 @@ PRODUCTS = [(1, 1, 1), (1, 16, 128), (1, 100, 300), (1, 4096, 1024), (1, 257, 11
 # Sizes past those above that take each of the tiles: 64 x 64 on four and on two waves, 128 x
 # 64, 128 x 128, 256 x 128 and 256 x 256, with rows, results and features that end inside one
 TILES = [(250, 4001, 1000), (100, 8192, 300), (64, 20000, 200), (700, 3000, 300), (260, 16400, 129), (1025, 4100, 256), (2040, 8190, 300),
-         (3900, 4000, 130), (64, 4096, 11264), (3900, 5100, 1300)]
+         (3900, 4000, 130), (64, 4096, 11264), (3900, 5100, 1300),
+         (2, 30000, 300), (600, 12000, 300), (700, 9000, 300)]
 
 
 @pytest.mark.parametrize("shape", PRODUCTS + TILES, ids=str)
