@@ -673,7 +673,8 @@ int tcx_hip_linear8(const int32_t* x_codes, const int32_t* x_scales, const int32
                     const tcx_hip_linear8_desc_t* desc, void* workspace, size_t workspace_bytes, tcx_stream_t stream);
 /* act(x g^T + bias) * (x u^T + bias'), quantised: w holds the `outputs` rows of g, then
  * those of u, bias likewise; codes and scales have `outputs` features a row.
- * out_stride is 0. The workspace must have the query's size (0 for large products). */
+ * out_stride is 0. The workspace must have the query's size (0 for
+ * products that one launch makes). */
 size_t tcx_hip_gated_linear8_workspace_bytes(const tcx_hip_linear8_desc_t* desc);
 int tcx_hip_gated_linear8(const int32_t* x_codes, const int32_t* x_scales, const int32_t* w_codes, const int32_t* w_scales,
                           int32_t* codes, int32_t* scales, const tcx_hip_linear8_desc_t* desc, void* workspace,

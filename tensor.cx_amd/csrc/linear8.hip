@@ -727,7 +727,7 @@ constexpr Way8 kWays[] = {
     {4, 128, 128, 1, 2, {7.0F, 7.7F}, {1.05F, 1.87F}}, {5, 256, 128, 1, 1, {7.0F, 7.0F}, {1.71F, 1.71F}},
     {6, 256, 256, 1, 1, {10.0F, 13.7F}, {1.74F, 2.75F}},
 };
-constexpr int kFewRows = 7, kFusedGate = 8;
+constexpr int kFewRows = 7, kFusedGate = 8, kFusedGate64 = 9;  // from kFusedGate on: gated products in one launch
 // A microsecond's reading of weights from memory.
 constexpr float kReads = 5.4e6F;
 struct Plan8 {
@@ -778,11 +778,20 @@ Plan8 plan_product(const Product8& a, bool gated, std::size_t workspace_bytes) {
     }
   }
   if (gated && (static_cast<std::int64_t>(a.outputs) + 256) * 4 * a.scale_pitch < (std::int64_t{1} << 31)) {
-    const std::int64_t tiles = static_cast<std::int64_t>((a.m + 255) / 256) * a.gate_blocks;
-    const std::int64_t rest = tiles % 256;
-    float time = static_cast<float>(tiles / 256 + (rest > kHalved ? 1 : 0)) * (12.0F + static_cast<float>(a.blocks) * 2.75F);
-    if (rest > 0 && rest <= kHalved) time += 9.0F + static_cast<float>(a.blocks) * 1.74F;
-    if (time < least) best = {kFusedGate, 1};
+    const auto steps = static_cast<float>(a.blocks);
+    auto fused = [&](int kind, float time) {
+      if (time >= least) return;
+      least = time;
+      best = {kind, 1};
+    };
+    const std::int64_t tiles = static_cast<std::int64_t>((a.m + 255) / 256) * a.gate_blocks, rest = tiles % 256;
+    float time = static_cast<float>(tiles / 256 + (rest > kHalved ? 1 : 0)) * (12.0F + steps * 2.75F);
+    if (rest > 0 && rest <= kHalved) time += 9.0F + steps * 1.74F;
+    fused(kFusedGate, time);
+    // Tiles of 64 rows: few features, or too few rows for the others to fill the CUs. 16 x 2 * 256 x
+    // 256 in 7.2 us (in two launches 8.8), 512 x 2 * 4096 x 4096 in 39 (49).
+    const std::int64_t before = (static_cast<std::int64_t>((a.m + 63) / 64) * a.gate_blocks - 1) / 256;
+    fused(kFusedGate64, static_cast<float>(before) * (4.2F + steps * 0.98F) + 3.6F + steps * 0.84F);
   }
   return best;
 }
@@ -796,6 +805,7 @@ int run_plan(const Product8& a, const Plan8& plan, float* parts, hipStream_t s) 
     case 5: return launch_product<256, 128, 64, 64, 1, 3>(a, plan.splits, parts, s);
     case 6: return launch_product<256, 256, 128, 64, 1, 2, false, true>(a, plan.splits, parts, s);
     case kFusedGate: return launch_product<256, 256, 128, 64, 1, 2, true, true>(a, 1, nullptr, s);
+    case kFusedGate64: return launch_product<64, 256, 32, 64, 1, 3, true>(a, 1, nullptr, s);
     default: break;
   }
   if (a.scale_pitch <= 8) return launch_few_rows<1>(a, parts, s);
@@ -900,7 +910,7 @@ size_t tcx_hip_gated_linear8_workspace_bytes(const tcx_hip_linear8_desc_t* desc)
   Product8 a;
   if (product_args(desc, true, a) != TCX_OK || a.m == 0 || a.n == 0 || a.blocks == 0) return 0;
   const Plan8 plan = plan_product(a, true, SIZE_MAX);
-  return plan.kind == kFusedGate ? 0 : part_bytes(a, plan.splits);
+  return plan.kind >= kFusedGate ? 0 : part_bytes(a, plan.splits);
 }
 
 int tcx_hip_gated_linear8(const int32_t* x_codes, const int32_t* x_scales, const int32_t* w_codes, const int32_t* w_scales,
@@ -920,14 +930,14 @@ int tcx_hip_gated_linear8(const int32_t* x_codes, const int32_t* x_scales, const
   Plan8 plan{0, 0};
   if (a.blocks > 0) {
     plan = plan_product(a, true, SIZE_MAX);
-    if (plan.kind != kFusedGate && (workspace == nullptr || workspace_bytes < part_bytes(a, plan.splits)))
+    if (plan.kind < kFusedGate && (workspace == nullptr || workspace_bytes < part_bytes(a, plan.splits)))
       return fail(TCX_INVALID_ARGUMENT, "gated_linear8 needs a workspace of the query's size");
   }
   if (int rc = ready(); rc != TCX_OK) return rc;
   const auto s = static_cast<hipStream_t>(stream);
   a.gate_codes = reinterpret_cast<std::uint32_t*>(codes);
   a.gate_scales = reinterpret_cast<std::uint8_t*>(scales);
-  if (plan.kind == kFusedGate) return run_plan(a, plan, nullptr, s);
+  if (plan.kind >= kFusedGate) return run_plan(a, plan, nullptr, s);
   if (a.blocks > 0)
     if (int rc = run_plan(a, plan, static_cast<float*>(workspace), s); rc != TCX_OK) return rc;
   Gate8 t{};

@@ -80,9 +80,12 @@ def test_products_refuse(gated):
                    {"out_stride": -1}, {"out_stride": 4}, {"workspace": capi.Workspace(ADDRESS + 4, 1 << 30)}):
         refused(call, **change)
     if gated:
-        for change in ({"scales": None}, {"scales": ADDRESS + 2}, {"out": ADDRESS + 4}, {"workspace": None}, {"out_stride": 5},
-                       {"workspace": capi.Workspace(ADDRESS, capi.linear8_workspace_bytes(capi.linear8_desc(2, 200, 5), True) - 1)}):
+        for change in ({"scales": None}, {"scales": ADDRESS + 2}, {"out": ADDRESS + 4}, {"out_stride": 5}):
             refused(call, **change)
+        wanted = capi.linear8_workspace_bytes(capi.linear8_desc(2, 2000, 5), True)
+        assert wanted > 0
+        for workspace in (None, capi.Workspace(ADDRESS, wanted - 1)):
+            refused(call, features=2000, workspace=workspace)
     nothing = dict(x=None, xs=None, w=None, ws=None, out=None, scales=None, workspace=None)
     call(rows=0, **nothing)
     call(outputs=0, **nothing)

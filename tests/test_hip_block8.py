@@ -264,7 +264,8 @@ def test_linear_of_nothing(cx):
 # rows, outputs, features
 GATED = [(1, 1, 128), (1, 300, 1000), (2, 128, 256), (7, 129, 300), (16, 1100, 384), (33, 513, 640), (70, 256, 100), (129, 260, 1300),
          (300, 140, 513), (520, 900, 256), (1100, 3000, 129), (2050, 1000, 384), (2300, 2570, 200),
-         (64, 11264, 300), (100, 3000, 1000), (260, 2000, 700), (600, 3000, 300), (130, 700, 8000), (40, 300, 9000), (4000, 2600, 200)]
+         (64, 11264, 300), (100, 3000, 1000), (260, 2000, 700), (600, 3000, 300), (130, 700, 8000), (40, 300, 9000), (4000, 2600, 200),
+         (7, 129, 2000), (16, 1100, 1500), (64, 11264, 1500), (600, 700, 6000), (1000, 4000, 600)]
 
 
 @pytest.mark.parametrize("bias", [False, True])

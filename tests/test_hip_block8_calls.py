@@ -190,7 +190,7 @@ def test_linear_with_and_without_workspace(capi, shape):
         np.testing.assert_array_equal(seen[0], seen[1])
 
 
-@pytest.mark.parametrize("shape", [(1, 200, 4096), (16, 1000, 2048), (40, 300, 1000), (200, 500, 700), (300, 1300, 512)], ids=str)
+@pytest.mark.parametrize("shape", [(1, 200, 4096), (16, 1000, 2048), (40, 300, 1000), (200, 500, 700), (300, 1300, 512), (100, 5000, 700)], ids=str)
 def test_gated_surroundings(capi, shape):
     """Nothing outside the rows is written; the same call twice gives the same bits, whatever
     the workspace held."""
