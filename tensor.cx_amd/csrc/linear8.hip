@@ -711,21 +711,22 @@ __global__ __launch_bounds__(256) void gate_kernel(Gate8 a) {
 
 // The ways to a product, and what a round of blocks on all 256 CUs took, in us: `fixed`
 // (start, first loads, results) and `step` for each block of 128 features, with one
-// block a CU and with as many as fit, which rounds before the last have (n = 4096, 1024
-// to 8192 features, weights in the cache, few rows a little less; ways 0 and 2: also n up
-// to 128256 with weights from memory). Of 256 x 256: with halves of at most 128 tiles,
-// and with whole ones. Few features over many tiles are for way 2, whose four blocks a CU
-// hide one's start and results behind another's products: 25 x 126974 x 139 in 16 us, way
-// 0 in 30.
+// block a CU and with as many as fit, which rounds before the last have (1024 to 12000
+// features, most weights from memory; ways 0 and 2 also 128 to 1024 features and n up to
+// 128256). Of 256 x 256: with halves of at most 128 tiles, and with whole ones. Few
+// features over many tiles are for way 2, whose four blocks a CU hide one's start and
+// results behind another's products: 25 x 126974 x 139 in 16 us, way 0 in 30. Way 3's step
+// is bound by what the L2s give (24 KB a CU and step, 11 TB/s of all): half the
+// conversions and a third buffer made no difference.
 struct Way8 {
   int kind, m, n, sets, fit;  // tile, and blocks that a CU holds
   float fixed[2], step[2];
 };
 constexpr Way8 kWays[] = {
-    {0, 32, 64, 4, 1, {1.5F, 2.4F}, {0.20F, 0.345F}},  {1, 64, 64, 4, 1, {2.8F, 2.8F}, {0.25F, 0.25F}},
-    {2, 64, 64, 1, 4, {1.4F, 4.2F}, {0.60F, 1.22F}},   {3, 128, 64, 2, 1, {2.7F, 2.7F}, {0.535F, 0.535F}},
-    {4, 128, 128, 1, 2, {7.0F, 7.7F}, {1.05F, 1.87F}}, {5, 256, 128, 1, 1, {7.0F, 7.0F}, {1.71F, 1.71F}},
-    {6, 256, 256, 1, 1, {10.0F, 13.7F}, {1.74F, 2.75F}},
+    {0, 32, 64, 4, 1, {1.5F, 2.4F}, {0.23F, 0.23F}},   {1, 64, 64, 4, 1, {2.8F, 2.8F}, {0.30F, 0.30F}},
+    {2, 64, 64, 1, 4, {1.4F, 4.2F}, {0.75F, 1.22F}},   {3, 128, 64, 2, 1, {2.7F, 2.7F}, {0.58F, 0.58F}},
+    {4, 128, 128, 1, 2, {7.0F, 7.7F}, {1.08F, 1.75F}}, {5, 256, 128, 1, 1, {7.0F, 7.0F}, {1.45F, 1.71F}},
+    {6, 256, 256, 1, 1, {9.5F, 13.7F}, {1.50F, 2.75F}},
 };
 constexpr int kFewRows = 7, kFusedGate = 8, kFusedGate64 = 9;  // from kFusedGate on: gated products in one launch
 // A microsecond's reading of weights from memory.
@@ -786,7 +787,7 @@ Plan8 plan_product(const Product8& a, bool gated, std::size_t workspace_bytes) {
     };
     const std::int64_t tiles = static_cast<std::int64_t>((a.m + 255) / 256) * a.gate_blocks, rest = tiles % 256;
     float time = static_cast<float>(tiles / 256 + (rest > kHalved ? 1 : 0)) * (12.0F + steps * 2.75F);
-    if (rest > 0 && rest <= kHalved) time += 9.0F + steps * 1.74F;
+    if (rest > 0 && rest <= kHalved) time += 9.0F + steps * 1.45F;
     fused(kFusedGate, time);
     // Tiles of 64 rows: few features, or too few rows for the others to fill the CUs. 16 x 2 * 256 x
     // 256 in 7.2 us (in two launches 8.8), 512 x 2 * 4096 x 4096 in 39 (49).

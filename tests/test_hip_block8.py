@@ -164,7 +164,8 @@ PRODUCTS = [(1, 1, 1), (1, 16, 128), (1, 100, 300), (1, 4096, 1024), (1, 257, 11
 # 64, 128 x 128, 256 x 128 and 256 x 256, with rows, results and features that end inside one
 TILES = [(250, 4001, 1000), (100, 8192, 300), (64, 20000, 200), (700, 3000, 300), (260, 16400, 129), (1025, 4100, 256), (2040, 8190, 300),
          (3900, 4000, 130), (64, 4096, 11264), (3900, 5100, 1300),
-         (2, 30000, 300), (600, 12000, 300), (700, 9000, 300)]
+         (2, 30000, 300), (600, 12000, 300), (700, 9000, 300), (1416, 30, 6702), (35, 16925, 2764), (2189, 20, 4691),
+         (614, 1878, 7432), (1524, 646, 5762), (5972, 674, 6026)]
 
 
 @pytest.mark.parametrize("shape", PRODUCTS + TILES, ids=str)
@@ -265,7 +266,8 @@ def test_linear_of_nothing(cx):
 GATED = [(1, 1, 128), (1, 300, 1000), (2, 128, 256), (7, 129, 300), (16, 1100, 384), (33, 513, 640), (70, 256, 100), (129, 260, 1300),
          (300, 140, 513), (520, 900, 256), (1100, 3000, 129), (2050, 1000, 384), (2300, 2570, 200),
          (64, 11264, 300), (100, 3000, 1000), (260, 2000, 700), (600, 3000, 300), (130, 700, 8000), (40, 300, 9000), (4000, 2600, 200),
-         (7, 129, 2000), (16, 1100, 1500), (64, 11264, 1500), (600, 700, 6000), (1000, 4000, 600)]
+         (7, 129, 2000), (16, 1100, 1500), (64, 11264, 1500), (600, 700, 6000), (1000, 4000, 600),
+         (1188, 194, 1064), (359, 1391, 6565), (429, 1155, 4374), (972, 2055, 6498)]
 
 
 @pytest.mark.parametrize("bias", [False, True])
