@@ -751,7 +751,8 @@ Plan8 plan_product(const Product8& a, bool gated, std::size_t workspace_bytes) {
   // 1 x 4096 x 4096 in 5.8 (8.9); but 8 x 60000 x 1024 in 30 (64 x 64 tiles: 17).
   if (a.m <= 16 && a.scale_pitch <= 24) {
     const float chain = 1.8F * static_cast<float>((a.scale_pitch + 7) / 8), row = static_cast<float>(a.pitch) / kReads;
-    least = static_cast<float>(a.n / 4096) * std::max(chain, 4096.0F * row) + std::max(chain, static_cast<float>(a.n % 4096) * row);
+    const int rounds = (a.n - 1) / 4096;  // whole ones before the last
+    least = static_cast<float>(rounds) * std::max(chain, 4096.0F * row) + std::max(chain, static_cast<float>(a.n - rounds * 4096) * row);
     if (gated) least += join_cost(a, 2);
     best = {kFewRows, 1};
   }
