@@ -287,6 +287,29 @@ def test_gated_linear(cx, shape, bias):
     cases.check_near(*words(pair), y, off, str(shape))
 
 
+@pytest.mark.parametrize("shape", [(3, 260, 500), (3, 260, 1000), (40, 260, 2000), (100, 260, 300), (4400, 1410, 200)], ids=str)
+def test_gated_linear_of_what_is_no_number(cx, shape):
+    """A NaN reaches its row (of a weight: its column), not the rest of its block, and nothing
+    behind the last output."""
+    rows, outputs, features = shape
+    rng = np.random.default_rng(rows + features)
+    x, w = f32(rng, rows, features), f32(rng, 2 * outputs, features)
+    def run():
+        pair = cx.hip.gated_linear8(cx.hip.quantise8(hip(cx, x)), cx.hip.quantise8(hip(cx, w)), activation="none")
+        codes, scales = words(pair)
+        return cases.values(codes, scales), 2.0 ** (scales.view(np.uint8).max().astype(float) - 127)
+    clean, unit = run()
+    x[rows // 2, 33], w[17, 0], w[outputs + 130, features - 1] = np.nan, np.inf, np.nan
+    got, unit_too = run()
+    bad = np.zeros(got.shape, bool)
+    bad[rows // 2, :outputs], bad[:, 17], bad[:, 130] = True, True, True
+    assert np.array_equal(np.isnan(got), bad) and (got[:, outputs:] == 0).all()
+    # The same float32 values, each rounded by 2^-4 of itself or 2^-10 of its unit at most, in
+    # blocks whose exponents may differ without the columns that are NaN now.
+    most = np.maximum(np.abs(got), np.abs(clean)) / (1 - 2.0 ** -4) + 2.0 ** -10 * max(unit, unit_too)
+    assert (np.abs(got - clean)[~bad] <= 2 * (2.0 ** -4 * most + 2.0 ** -10 * max(unit, unit_too))[~bad]).all()
+
+
 def test_shapes_of_more_axes(cx):
     rng = np.random.default_rng(1)
     x = cx.hip.quantise8(hip(cx, f32(rng, 2, 3, 200)))
