@@ -517,8 +517,10 @@ __global__ __launch_bounds__(512) void few_rows_kernel(Product8 a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4, units = a.scale_pitch;
 
-  // Blocks past the row's end are zeros in x, so whatever w has there adds nothing; w's are
-  // read from the row's last block. Of few rows each is brought once, 512 bytes of two rows
+  // Blocks past the row's end are zeros in x. There w has the codes of the row's last block, or
+  // of its last unit for a wave without one of its own, with exponents of zero: such values
+  // are finite (with their own exponents they may be infinite, and infinity times zero is
+  // NaN), or NaN where that column is NaN anyway. Of few rows each is brought once, 512 bytes of two rows
   // a load, and spread through the wave's own LDS: 1 x 4096 x 4096 in 6.7 us for 7.4.
   int4_t x[kU][8], stage[kStaged / 2];
   std::uint32_t x_word[kU];
@@ -548,10 +550,10 @@ __global__ __launch_bounds__(512) void few_rows_kernel(Product8 a) {
     std::uint32_t word;
   };
   auto load = [&](Weights& w, int tile, int u) {
-    const int rows = min(a.n - 16 * tile, 16), unit = min(wave + 8 * u, units - 1);
+    const int rows = min(a.n - 16 * tile, 16), own = wave + 8 * u, unit = min(own, units - 1);
     const auto rsrc = row_buffer(a.w, 16 * tile, rows, a.pitch);
     const int row = min(r, rows - 1), at = row * a.pitch + 16 * g;
-    w.word = a.w_scale[static_cast<std::int64_t>(16 * tile + row) * a.scale_pitch + unit];
+    w.word = own < units ? a.w_scale[static_cast<std::int64_t>(16 * tile + row) * a.scale_pitch + unit] : 0;
 #pragma unroll
     for (int p = 0; p < 8; ++p) w.piece[p] = load16(rsrc, at + 64 * (p & 1), min(4 * unit + p / 2, a.blocks - 1) * 128);
   };
