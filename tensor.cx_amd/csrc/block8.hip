@@ -84,6 +84,14 @@ __device__ __forceinline__ float inverse_rms(const Norm8& a, float squares) {
   return 1.0F / sqrtf(squares / static_cast<float>(a.features) + a.epsilon);
 }
 
+// Features [f, f + 4) of the norm; zeros behind the row's end, where zero times an inverse of
+// NaN or infinity would be NaN.
+__device__ __forceinline__ float4_t normed(const Norm8& a, int f, float4_t v, float inverse, float4_t w) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = f + e < a.features ? v[e] * inverse * w[e] : 0.0F;
+  return v;
+}
+
 __device__ __forceinline__ float squares4(float4_t v) { return (v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3]); }
 
 // A block a row, U groups of it in each wave's registers: one read of x and the
@@ -129,8 +137,7 @@ __global__ __launch_bounds__(512) void rmsnorm_kernel(Norm8 a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float4_t w = a.weight != nullptr ? load_features(a.weight, p.feature + 64 * h, a.features) : float4_t{1.0F, 1.0F, 1.0F, 1.0F};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[u][h][e] = v[u][h][e] * inverse * w[e];
+        v[u][h] = normed(a, p.feature + 64 * h, v[u][h], inverse, w);
       }
       store_group(a.codes + row * a.blocks * 32, a.scales + row * a.groups * 4, p, a.blocks, encode_block(v[u]));
     }
@@ -164,8 +171,7 @@ __global__ __launch_bounds__(512) void rmsnorm_long_kernel(Norm8 a) {
         v[h] = read(p.feature + 64 * h);
         if (a.sum != nullptr) store_features(a.sum + row * a.sum_stride, p.feature + 64 * h, a.features, v[h]);
         const float4_t w = a.weight != nullptr ? load_features(a.weight, p.feature + 64 * h, a.features) : float4_t{1.0F, 1.0F, 1.0F, 1.0F};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[h][e] = v[h][e] * inverse * w[e];
+        v[h] = normed(a, p.feature + 64 * h, v[h], inverse, w);
       }
       store_group(a.codes + row * a.blocks * 32, a.scales + row * a.groups * 4, p, a.blocks, encode_block(v));
     }

@@ -1,5 +1,5 @@
 """GPU tests of 8-bit rows and products at the ends of the format: weights next to
-float32's largest value and past it."""
+float32's largest value and past it, rows of which a norm makes no numbers."""
 
 from __future__ import annotations
 
@@ -85,3 +85,23 @@ def test_linear_of_weights_past_the_largest(cx, rows, blocks):
     np.testing.assert_array_equal(got[:, ::2], np.sign(x[:, :1]) * np.full((rows, outputs // 2), np.inf, np.float32))
     expected, off = cases.product(cases.values(*words(x_pair)), cases.values(*cases.pack(w_codes[1::2], w_exponents[1::2])))
     assert (np.abs(got[:, 1::2] - expected) <= off).all()
+
+
+# Rows that one wave holds, each number of groups a wave holds, and rows read twice; the last
+# block partly filled, alone in its group and not.
+@pytest.mark.parametrize("features", [1, 300, 1000, 1537, 5000, 8321, 16385, 32700, 33001, 70001])
+@pytest.mark.parametrize("weight", [False, True])
+def test_rmsnorm_leaves_zeros_behind_the_last_feature(cx, features, weight):
+    """Codes behind the last feature are zeros whatever the row's norm is: of a NaN, of
+    an infinity, of zeros with no epsilon (zero over zero); the row itself goes by the formula."""
+    rng = np.random.default_rng(features)
+    x = f32(rng, 5, features)
+    x[1, features // 2], x[2, 0], x[3] = np.nan, -np.inf, 0
+    w = hip(cx, 1 + 0.3 * f32(rng, features)) if weight else None
+    for given in ({}, {"residual": hip(cx, np.zeros_like(x))}):
+        codes, scales, *_ = cx.hip.rmsnorm8(hip(cx, x), w, eps=0.0, **given)
+        c, e = cases.unpack(*words((codes, scales)))
+        assert (c[:, features:] == 0).all(), f"rows {np.flatnonzero((c[:, features:] != 0).any(1)).tolist()}"
+        got = cases.values(*words((codes, scales)))[:, :features]
+        assert np.isnan(got[1]).all() and np.isnan(got[2, 0]) and (got[2, 1:] == 0).all() and np.isnan(got[3]).all()
+        assert np.isfinite(got[[0, 4]]).all()
