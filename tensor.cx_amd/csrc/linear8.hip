@@ -95,8 +95,9 @@ __device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, void* lds, 
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voffset, soffset, 0, 0);
 }
 
-// An offset past every buffer here (of at most 256 rows of 2^22 bytes), with any scalar
-// offset added: such a load gives zeros.
+// An offset past every buffer here (of at most 256 rows of 2^22 bytes): such a load gives
+// zeros. Scalar offsets stay inside their buffer, with such a load too: whether they count in
+// the check, or are taken from the buffer's size before it, then makes no difference.
 constexpr int kNowhere = 0x7fff0000;
 // Four bytes a lane straight into LDS.
 __device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t r, void* lds, int voffset, int soffset) {
@@ -531,7 +532,8 @@ __global__ __launch_bounds__(512) void few_rows_kernel(Product8 a) {
     for (int t = 0; t < kStaged / 2; ++t) {
       const int row = 2 * t + (lane >> 5), at = 16 * (lane & 31);
       if (2 * t < a.m)
-        stage[t] = load16(x_rsrc, row < a.m && wave < units && at < (a.blocks - 4 * wave) * 128 ? row * a.pitch + at : kNowhere, wave * 512);
+        stage[t] = load16(x_rsrc, row < a.m && wave < units && at < (a.blocks - 4 * wave) * 128 ? row * a.pitch + at : kNowhere,
+                          wave < units ? wave * 512 : 0);
     }
   }
   const int x_row = min(r, a.m - 1);
@@ -542,7 +544,8 @@ __global__ __launch_bounds__(512) void few_rows_kernel(Product8 a) {
     if (staged) continue;
 #pragma unroll
     for (int p = 0; p < 8; ++p)
-      x[u][p] = load16(x_rsrc, unit < units && 4 * unit + p / 2 < a.blocks ? x_row * a.pitch + 16 * g + 64 * p : kNowhere, unit * 512);
+      x[u][p] = load16(x_rsrc, unit < units && 4 * unit + p / 2 < a.blocks ? x_row * a.pitch + 16 * g + 64 * p : kNowhere,
+                       unit < units ? unit * 512 : 0);
   }
 
   struct Weights {
