@@ -332,6 +332,36 @@ def test_two_threads(capi, runtime):
         same(layer.results(), want)
 
 
+def test_two_threads_results(capi, runtime):
+    """Calls of two threads at the same time, each on its own stream, buffers and workspaces:
+    what every turn of each gives is what its calls give alone."""
+    layers, streams = [Layer(capi, 6, 7), Layer(capi, 7, 130, 512, 600)], [runtime.stream(), runtime.stream()]
+    turns, failures, start = 4, [], threading.Barrier(2)
+
+    def results(layer, s, turn):
+        layer.refill(turn)
+        for _ in range(8):  # the norm's sum goes to its residual: each time another one
+            layer.run(s)
+        runtime.hipStreamSynchronize(s)
+        return layer.results()
+
+    def work(layer, s, alone):
+        try:
+            start.wait(60)
+            for turn in range(3 * turns):
+                same(results(layer, s, turn % turns), alone[turn % turns])
+        except BaseException as e:  # noqa: BLE001 - reported by the test's thread
+            failures.append(e)
+
+    expected = [[results(layer, s, turn) for turn in range(turns)] for layer, s in zip(layers, streams)]
+    threads = [threading.Thread(target=work, args=args) for args in zip(layers, streams, expected)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
+
+
 def test_past_32_bit_offsets(capi):
     """Rows 5 GB into their matrices: codes, float32 rows and results."""
     rng = np.random.default_rng(41)
