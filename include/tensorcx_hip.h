@@ -679,6 +679,17 @@ size_t tcx_hip_gated_linear8_workspace_bytes(const tcx_hip_linear8_desc_t* desc)
 int tcx_hip_gated_linear8(const int32_t* x_codes, const int32_t* x_scales, const int32_t* w_codes, const int32_t* w_scales,
                           int32_t* codes, int32_t* scales, const tcx_hip_linear8_desc_t* desc, void* workspace,
                           size_t workspace_bytes, tcx_stream_t stream);
+/* How a call would run with a workspace of that many bytes (a gated one has what it needs):
+ * in tiles of tile_rows x tile_outputs results, each by as many `sets` of waves that share the
+ * features, in `splits` parts over blocks, with `launches` launches (2: parts are joined, or
+ * float32 results gated, in the second) and workspace_bytes of the workspace. Few rows, tiles of
+ * 16 x 16, keep `units` of 512 features in a wave's registers; else units is 0. Refused
+ * without rows, outputs or features. */
+typedef struct {
+  int32_t tile_rows, tile_outputs, sets, units, splits, launches;
+  size_t workspace_bytes;
+} tcx_hip_linear8_plan_t;
+int tcx_hip_linear8_plan(const tcx_hip_linear8_desc_t* desc, int gated, size_t workspace_bytes, tcx_hip_linear8_plan_t* plan);
 
 #ifdef __cplusplus
 }

@@ -746,6 +746,8 @@ std::size_t part_bytes(const Product8& a, int splits) {
 float join_cost(const Product8& a, int splits) {
   return splits == 1 ? 0.0F : 4.5F + (splits + 1) * 4.0F * static_cast<float>(a.m) * static_cast<float>(a.n) / 4.5e6F;
 }
+// Units of the features that a wave holds of few rows.
+int few_rows_units(const Product8& a) { return (a.scale_pitch + 7) / 8; }
 // `gated`: the results go through float32 and a second launch to 8 bits, unless the tiles
 // of 256 x 256 do that themselves.
 Plan8 plan_product(const Product8& a, bool gated, std::size_t workspace_bytes) {
@@ -755,7 +757,7 @@ Plan8 plan_product(const Product8& a, bool gated, std::size_t workspace_bytes) {
   // its weights' bytes or a chain of 1.8 us for 4096 features. 16 x 22528 x 4096 in 22 us (32 x 64 tiles: 26),
   // 1 x 4096 x 4096 in 5.8 (8.9); but 8 x 60000 x 1024 in 30 (64 x 64 tiles: 17).
   if (a.m <= 16 && a.scale_pitch <= 24) {
-    const float chain = 1.8F * static_cast<float>((a.scale_pitch + 7) / 8), row = static_cast<float>(a.pitch) / kReads;
+    const float chain = 1.8F * static_cast<float>(few_rows_units(a)), row = static_cast<float>(a.pitch) / kReads;
     const int rounds = (a.n - 1) / 4096;  // whole ones before the last
     least = static_cast<float>(rounds) * std::max(chain, 4096.0F * row) + std::max(chain, static_cast<float>(a.n - rounds * 4096) * row);
     if (gated) least += join_cost(a, 2);
@@ -815,9 +817,11 @@ int run_plan(const Product8& a, const Plan8& plan, float* parts, hipStream_t s) 
     case kFusedGate64: return launch_product<64, 256, 32, 64, 1, 3, true>(a, 1, nullptr, s);
     default: break;
   }
-  if (a.scale_pitch <= 8) return launch_few_rows<1>(a, parts, s);
-  if (a.scale_pitch <= 16) return launch_few_rows<2>(a, parts, s);
-  return launch_few_rows<3>(a, parts, s);
+  switch (few_rows_units(a)) {
+    case 1: return launch_few_rows<1>(a, parts, s);
+    case 2: return launch_few_rows<2>(a, parts, s);
+    default: return launch_few_rows<3>(a, parts, s);
+  }
 }
 
 // Checks a descriptor and fills what follows from it; `gated`: weights of 2 * outputs rows.
@@ -867,6 +871,29 @@ int operand_args(const std::int32_t* x_codes, const std::int32_t* x_scales, cons
 }  // namespace tcx
 
 extern "C" {
+
+int tcx_hip_linear8_plan(const tcx_hip_linear8_desc_t* desc, int gated, size_t workspace_bytes, tcx_hip_linear8_plan_t* plan) {
+  using namespace tcx;
+  if (plan == nullptr) return fail(TCX_INVALID_ARGUMENT, "linear8 plan is null");
+  Product8 a;
+  if (int rc = product_args(desc, gated != 0, a); rc != TCX_OK) return rc;
+  if (a.m == 0 || a.n == 0 || a.blocks == 0) return fail(TCX_INVALID_ARGUMENT, "no linear8 product for these extents");
+  const Plan8 p = plan_product(a, gated != 0, gated != 0 ? SIZE_MAX : workspace_bytes);
+  const bool whole = p.kind >= kFusedGate || (gated == 0 && p.splits == 1);
+  *plan = {16, 16, 8, 0, p.splits, whole ? 1 : 2, whole ? 0 : part_bytes(a, p.splits)};
+  if (p.kind == kFewRows) {
+    plan->units = few_rows_units(a);
+  } else if (p.kind >= kFusedGate) {
+    plan->tile_rows = p.kind == kFusedGate ? 256 : 64;
+    plan->tile_outputs = 128;
+    plan->sets = 1;
+  } else {
+    plan->tile_rows = kWays[p.kind].m;
+    plan->tile_outputs = kWays[p.kind].n;
+    plan->sets = kWays[p.kind].sets;
+  }
+  return TCX_OK;
+}
 
 size_t tcx_hip_linear8_workspace_bytes(const tcx_hip_linear8_desc_t* desc) {
   using namespace tcx;

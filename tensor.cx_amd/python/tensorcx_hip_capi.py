@@ -54,7 +54,7 @@ EXPORTS = [
     "tcx_hip_cache4_attention_f32", "tcx_hip_beam_select_workspace_bytes", "tcx_hip_beam_select_f32",
     "tcx_hip_beam_reorder", "tcx_hip_block8_code_words", "tcx_hip_block8_scale_words", "tcx_hip_quantise8",
     "tcx_hip_dequantise8", "tcx_hip_rmsnorm8", "tcx_hip_linear8_workspace_bytes", "tcx_hip_linear8",
-    "tcx_hip_gated_linear8_workspace_bytes", "tcx_hip_gated_linear8",
+    "tcx_hip_gated_linear8_workspace_bytes", "tcx_hip_gated_linear8", "tcx_hip_linear8_plan",
 ]
 
 
@@ -108,6 +108,11 @@ class Rmsnorm8Desc(ctypes.Structure):
 class Linear8Desc(ctypes.Structure):
     _fields_ = [("rows", ctypes.c_int64), ("features", ctypes.c_int64), ("outputs", ctypes.c_int64),
                 ("bias", ctypes.c_void_p), ("activation", ctypes.c_int32), ("out_stride", ctypes.c_int64)]
+
+
+class Linear8Plan(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("tile_rows", "tile_outputs", "sets", "units", "splits", "launches")] + [
+        ("workspace_bytes", ctypes.c_size_t)]
 
 
 class PoolRuntime(ctypes.Structure):
@@ -205,6 +210,7 @@ def lib() -> ctypes.CDLL:
         for name in ("tcx_hip_linear8", "tcx_hip_gated_linear8"):
             query = getattr(L, name + "_workspace_bytes")
             query.argtypes, query.restype = [ctypes.POINTER(Linear8Desc)], sz
+        L.tcx_hip_linear8_plan.argtypes = [ctypes.POINTER(Linear8Desc), ctypes.c_int, sz, ctypes.POINTER(Linear8Plan)]
         L.tcx_hip_linear8.argtypes = [vp, vp, vp, vp, vp, ctypes.POINTER(Linear8Desc), vp, sz, vp]
         L.tcx_hip_gated_linear8.argtypes = [vp, vp, vp, vp, vp, vp, ctypes.POINTER(Linear8Desc), vp, sz, vp]
         _LIB = L
@@ -561,6 +567,13 @@ def linear8_workspace_bytes(desc: Linear8Desc, gated: bool = False) -> int:
     """Bytes of workspace that linear8 can use (that gated_linear8 needs, with `gated`)."""
     query = lib().tcx_hip_gated_linear8_workspace_bytes if gated else lib().tcx_hip_linear8_workspace_bytes
     return query(ctypes.byref(desc))
+
+
+def linear8_plan(desc: Linear8Desc, gated: bool = False, workspace_bytes: int = ctypes.c_size_t(-1).value) -> Linear8Plan:
+    """How a call would run: tiles, splits and launches (with all the workspace it can use)."""
+    plan = Linear8Plan()
+    check(lib().tcx_hip_linear8_plan(ctypes.byref(desc), int(gated), workspace_bytes, ctypes.byref(plan)), "linear8_plan")
+    return plan
 
 
 def linear8_workspace(desc: Linear8Desc, gated: bool = False) -> DeviceBuffer | None:
