@@ -178,7 +178,7 @@ __device__ __forceinline__ void product_tile(const Product8& a, Tile8 tile, std:
 #pragma unroll
   for (int t = 0; t < kLoads; ++t) {
     const int at = 8 * (t * kWaves + wave), row = at + (lane >> 3);
-    of_x[t] = kM % (8 * kWaves) == 0 ? t * 8 * kWaves < kM : at < kM;
+    of_x[t] = t * 8 * kWaves < kM;
     offset[t] = (of_x[t] ? min(row, m_last) : w_row(row - kM)) * a.pitch + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
   }
   // Exponents: words of 64 rows a load, spread over the waves.
@@ -649,7 +649,7 @@ struct Join8 {
   const float* bias;
   float* out;
   std::int64_t out_stride, part;  // floats between rows of out; between shares
-  int m, n, splits, activation;
+  int n, splits, activation;
   std::uint32_t items;  // four results of a row each
   FastDiv by_row;
 };
@@ -928,7 +928,6 @@ int tcx_hip_linear8(const int32_t* x_codes, const int32_t* x_scales, const int32
   j.out = out;
   j.out_stride = a.out_stride;
   j.part = static_cast<std::int64_t>(a.m) * a.n;
-  j.m = a.m;
   j.n = a.n;
   j.splits = plan.splits;
   j.activation = a.activation;
