@@ -650,7 +650,9 @@ typedef struct {
 } tcx_hip_rmsnorm8_desc_t;
 /* s = x + residual (x for NULL), y = s / sqrt(mean of s^2 + epsilon) * weight (1 for
  * NULL), all float32; y is quantised, and s written to sum unless that is NULL. sum
- * may be x or residual itself, with the same stride. */
+ * may be x or residual itself, with the same stride. A NaN in s makes its row NaN; where the sum of
+ * squares passes float32's largest value (values of some 10^18 and more) finite ones of the row
+ * become 0, and with an epsilon of 0 a sum below its smallest makes NaN. */
 int tcx_hip_rmsnorm8(const float* x, const float* residual, const float* weight, float* sum, int32_t* codes, int32_t* scales,
                      const tcx_hip_rmsnorm8_desc_t* desc, tcx_stream_t stream);
 
@@ -662,7 +664,8 @@ typedef struct {
 } tcx_hip_linear8_desc_t;
 /* out = act(x w^T + bias) of x [rows, features] and w [outputs, features], both in 8
  * bits, as float32. Products are exact and summed in float32, in an order that goes
- * by the sizes and the workspace's; a NaN makes its row (of w: its column) NaN. Scales
+ * by the sizes and the workspace's; a NaN makes its row (of w: its column) NaN, and a
+ * code that stands for 2^128 or more is infinite. Scales
  * hold bytes of 27 to 247 as the functions above write them, and codes and scales
  * behind the last feature are zeros. No more results than 2^23 tiles of 32 x 64 or
  * larger may be asked for. The workspace (16-byte aligned, may be NULL) takes the parts

@@ -100,7 +100,7 @@ __device__ __forceinline__ float squares4(float4_t v) { return (v[0] * v[0] + v[
 // A block a row, U groups of it in each wave's registers: one read of x and the
 // residual, one write of their sum and of the codes. Waves and U are the fewest that hold
 // the row, so a short one has more blocks on a CU. Bound by memory: 8192 x 8192 with
-// residual, weight and sum in 162 us, 5.4 TB/s; 1 x 4096 in 2.8, nearly all of it the launch
+// residual, weight and sum in 163 us, 5.4 TB/s; 1 x 4096 in 2.8, nearly all of it the launch
 // and three dependent steps (load, sum over the block, store).
 template <int U>
 __global__ __launch_bounds__(512) void rmsnorm_kernel(Norm8 a) {

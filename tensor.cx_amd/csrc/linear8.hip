@@ -120,9 +120,10 @@ __device__ __forceinline__ void wave_lds_done() { asm volatile("s_waitcnt lgkmcn
 // step takes a block of 128 features of the tile's rows, brought from memory straight
 // into one of kStages buffers in LDS, kStages - 1 steps ahead. Row r's sixteen-byte
 // pieces stand in the order piece ^ (r / 2 & 7): the 64 banks hold two rows, so the reads
-// of sixteen neighbouring rows lie in different banks (8192^3 in 787 us; in the order
-// piece ^ (r & 7), with conflicts in 46 % of the LDS cycles, 793). Words of exponents, of
-// four steps each, have two buffers of their own.
+// of sixteen neighbouring rows lie in different banks: conflicts in 2 to 3 % of the LDS
+// cycles, where the order piece ^ (r & 7) had 46 % (8192^3 takes 780 to 815 us by the GPU's
+// clock, and the two orders differ by less than that). Words of exponents, of four steps each,
+// have two buffers of their own.
 //
 // With kSets > 1 there are as many sets of waves, each with the whole tile for every
 // kSets-th step and with LDS of its own; their sums meet at the end. A set of one wave
@@ -130,8 +131,8 @@ __device__ __forceinline__ void wave_lds_done() { asm volatile("s_waitcnt lgkmcn
 // a small tile each would make. Sets of more waves share the barriers.
 //
 // With kGate the tile has 128 columns of gate and the same ones of up, 32 of each by turns,
-// and its results leave in 8 bits: 4096 x (2 x 11264) x 4096 in 595 us, in two launches
-// with float32 between them 709.
+// and its results leave in 8 bits: 4096 x (2 x 11264) x 4096 in 580 to 595 us, in two
+// launches with float32 between them 709.
 //
 // The features may be split over the grid's rows (Product8::parts).
 template <int kM, int kN, int kWM, int kWN, int kSets, int kStages>
@@ -457,7 +458,7 @@ __device__ __forceinline__ void product_tile(const Product8& a, Tile8 tile, std:
 
 // With kHalves the tiles past the last whole round of 256, if they leave half the CUs
 // empty, are taken by two blocks each, one for the rows of either half (from tile a.whole
-// on): 4096 x 5120 x 4096, 320 tiles, in 157 us, else 193.
+// on): 4096 x 5120 x 4096, 320 tiles, in 155 us, else 193.
 constexpr int kHalved = 128;
 template <int kM, int kN, int kWM, int kWN, int kSets, int kStages, bool kGate, bool kHalves>
 __global__ __launch_bounds__((Tiles8<kM, kN, kWM, kWN, kSets, kStages>::kThreads)) void product_kernel(Product8 a) {
@@ -521,8 +522,9 @@ __global__ __launch_bounds__(512) void few_rows_kernel(Product8 a) {
   // Blocks past the row's end are zeros in x. There w has the codes of the row's last block, or
   // of its last unit for a wave without one of its own, with exponents of zero: such values
   // are finite (with their own exponents they may be infinite, and infinity times zero is
-  // NaN), or NaN where that column is NaN anyway. Of few rows each is brought once, 512 bytes of two rows
-  // a load, and spread through the wave's own LDS: 1 x 4096 x 4096 in 6.7 us for 7.4.
+  // NaN), or NaN where that column is NaN anyway. Of up to kStaged rows each is brought once, 512
+  // bytes of two rows a load, and spread through the wave's own LDS: 0.7 us less for 1 x 4096 x
+  // 4096 than lanes that each load their own pieces.
   int4_t x[kU][8], stage[kStaged / 2];
   std::uint32_t x_word[kU];
   const auto x_rsrc = row_buffer(a.x, 0, a.m, a.pitch);
@@ -720,9 +722,16 @@ __global__ __launch_bounds__(256) void gate_kernel(Gate8 a) {
 // features, most weights from memory; ways 0 and 2 also 128 to 1024 features and n up to
 // 128256). Of 256 x 256: with halves of at most 128 tiles, and with whole ones. Few
 // features over many tiles are for way 2, whose four blocks a CU hide one's start and
-// results behind another's products: 25 x 126974 x 139 in 16 us, way 0 in 30. Way 3's step
+// results behind another's products: 25 x 126974 x 139 in 13 us, way 0 in 30. Way 3's step
 // is bound by what the L2s give (24 KB a CU and step, 11 TB/s of all): half the
 // conversions and a third buffer made no difference.
+//
+// The reading of weights bounds a step only of unsplit tiles here, not of shares nor of the
+// gated tiles: for few rows of wide ones the times are told too short. The choice is near the
+// bytes' time all the same for 1 and 16 x 2 * 28672 x 8192 (99 to 102 us, 88 reading), 2 * 18432 x
+// 7168 (60 to 62, 49) and 1 x 8192 x 28672 (45, 44), not for 1 x 2 * 8192 x 8192 (38, 25: 64 x 64
+// tiles in four shares). The gated tiles of 64 rows want more of the L2s than they give: 39 us
+// for 512 x 2 * 4096 x 4096, told 30.
 struct Way8 {
   int kind, m, n, sets, fit;  // tile, and blocks that a CU holds
   float fixed[2], step[2];
